@@ -392,6 +392,64 @@ int sapa_deform_fused_backward(const void *grad_out, const void *query, const vo
                                void *grad_query, void *grad_key, void *grad_value, void *grad_offset,
                                int B, int Cq, int C, int H, int W, int P, int s, int G, int dtype, void *stream);
 
+/* ------------------------------------------------------------------ attention over sequences of tokens ------------- */
+/* The global counterpart of the local attention above: every query token sees the keys of its own sequence.  No counterpart in
+ * the reference.
+ *
+ * Sequences lie packed one behind the other: tokens [offsets[b], offsets[b + 1]) of `query` are sequence b.  Its keys are
+ *   packed  (page_table == NULL): tokens [key_offsets[b], key_offsets[b + 1]) of `key` and `value`;
+ *   paged   : positions 0 .. key_lengths[b] - 1; position p lies in slot p % page of page page_table[b * max_pages + p / page].
+ * Token i of a sequence of Lq tokens and Lk keys sees the keys j <= i + Lk - Lq if `causal`, and all of them otherwise.
+ * `heads` query heads share `groups` key / value heads: query head h reads head h / (heads / groups).
+ *   out[t, h, :] = sum_j softmax_j(scale * <query[t, h], key[j]>) value[j]          (0 where a token sees no key)
+ * What a token does not see has no part in its output, whatever it holds.  The lengths are read on the device and taken within bounds: an
+ * offset outside the tensor counts as the nearest one inside, a sequence whose end lies before its begin as empty.  A page number outside
+ * [0, pages), or a position that the table has no page for, is never read: tokens that see it get NaN.
+ *
+ * Rows (dim channels) are dense; all other strides are free, in elements, and multiples of 16 bytes, as the addresses are.  `out` and the
+ * gradients are dense [tokens, heads, dim] and overwritten, `lse` is [tokens, heads] float32; in rows of no sequence all of them are 0.
+ * dtype: SAPA_F32, SAPA_F16, SAPA_BF16; dim: a multiple of 8 up to 128; heads / groups up to 128. */
+typedef struct sapa_attention {
+    const void *query, *key, *value;
+    void *out;
+    float *lse;                     /* log of the sum of exp(scale * <q, k>), for the backward pass; may be NULL; -inf: no key seen */
+    const int *offsets;             /* [B + 1] */
+    const int *key_offsets;         /* [B + 1], packed */
+    const int *page_table;          /* [B, max_pages], paged */
+    const int *key_lengths;         /* [B], paged */
+    long long query_strides[2];     /* of a token, of a head */
+    long long key_strides[3];       /* of a token (packed) or a slot of a page, of a head, of a page */
+    long long value_strides[3];
+    int B, tokens, keys;            /* keys: tokens of `key` and `value`, packed */
+    int pages, page, max_pages;     /* paged: pages of the cache, slots of a page, entries of a row of the table */
+    int heads, groups, dim, causal;
+    float scale;
+} sapa_attention;
+
+/* Forward.  Workspace: sapa_attention_workspace() bytes (may be 0), 256-byte aligned.  Deterministic. */
+size_t sapa_attention_workspace(const sapa_attention *a, int dtype);
+int sapa_attention_forward(const sapa_attention *a, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+/* Gradients of the packed form from grad_out (its strides: of a token, of a head); a->out and a->lse are the forward's.  Deterministic.
+ * Workspace: sapa_attention_backward_workspace() bytes, 256-byte aligned. */
+size_t sapa_attention_backward_workspace(const sapa_attention *a, int dtype);
+int sapa_attention_backward(const sapa_attention *a, const void *grad_out, long long grad_token_stride, long long grad_head_stride,
+                            void *grad_query, void *grad_key, void *grad_value, void *workspace, size_t workspace_bytes, int dtype,
+                            void *stream);
+
+/* Writes new keys and values into a paged cache: token i of sequence b, of Lq new tokens, goes to position key_lengths[b] - Lq + i, so that
+ * key_lengths already counts them.  Tokens before position 0, of no sequence, or of a page outside the cache are not written; every other
+ * byte of the cache stays as it is.  Of tokens that share a slot, each 16 bytes
+ * kept are those of one of them.  Any dtype of the four; rows that are multiples of 16 bytes. */
+typedef struct sapa_paged_rows {
+    const void *key, *value;        /* [tokens, groups, dim] */
+    void *key_pages, *value_pages;  /* [pages, page, groups, dim] */
+    const int *offsets, *page_table, *key_lengths;
+    long long key_strides[2], value_strides[2];                 /* of a token, of a head */
+    long long key_page_strides[3], value_page_strides[3];       /* of a slot, of a head, of a page */
+    int B, tokens, pages, page, max_pages, groups, dim;
+} sapa_paged_rows;
+int sapa_paged_write(const sapa_paged_rows *a, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

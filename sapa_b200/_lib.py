@@ -58,6 +58,9 @@ _SIGNATURES = {
     "sapa_projections_forward": [_vp, _i, _vp, _sz, _i, _i, _vp],
     "sapa_projections_backward": [_vp, _i, _vp, _sz, _i, _i, _vp],
     "sapa_deform_fused_backward_dense": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "sapa_attention_forward": [_vp, _vp, _sz, _i, _vp],
+    "sapa_attention_backward": [_vp, _vp, ctypes.c_longlong, ctypes.c_longlong, _vp, _vp, _vp, _vp, _sz, _i, _vp],
+    "sapa_paged_write": [_vp, _i, _vp],
     "sapa_deform_fused_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
 }
 EXPORTS = sorted(list(_SIGNATURES) + ["sapa_last_error", "sapa_last_kernels", "sapa_abi_version", "sapa_fused_backward_workspace",
@@ -65,6 +68,7 @@ EXPORTS = sorted(list(_SIGNATURES) + ["sapa_last_error", "sapa_last_kernels", "s
                                            "sapa_deform_fused_backward_scatter_bytes", "sapa_project_workspace",
                                            "sapa_project_rows_workspace", "sapa_project_list_workspace", "sapa_projections_workspace",
                                            "sapa_projections_backward_workspace",
+                                           "sapa_attention_workspace", "sapa_attention_backward_workspace",
                                            "sapa_fused_backward_static_capacity", "sapa_wait_timeout_flags"])
 
 
@@ -109,6 +113,9 @@ def lib() -> ctypes.CDLL:
     handle.sapa_project_list_workspace.argtypes = [_vp, _i, _i]
     handle.sapa_project_list_workspace.restype = ctypes.c_size_t
     for name in ("sapa_projections_workspace", "sapa_projections_backward_workspace"):
+        getattr(handle, name).argtypes = [_vp, _i]
+        getattr(handle, name).restype = ctypes.c_size_t
+    for name in ("sapa_attention_workspace", "sapa_attention_backward_workspace"):
         getattr(handle, name).argtypes = [_vp, _i]
         getattr(handle, name).restype = ctypes.c_size_t
     handle.sapa_fused_backward_static_capacity.argtypes = []

@@ -1,0 +1,64 @@
+"""Attention over sequences of tokens: the global counterpart of the local operators (``qk``, ``av``, ``sapa_fused``), for the encoders and
+decoders around an upsampler.  The reference has no such operator.
+
+``packed_attention`` takes whole sequences packed one behind the other and is differentiable; ``paged_attention`` takes new tokens, one or
+many a sequence, over a cache of keys and values in pages, into which ``paged_write`` puts the new keys and values.  Checks, allocation and
+the autograd node are native (``csrc/host_attention.inc``), the kernels are in ``csrc/attention.cu``.
+"""
+from __future__ import annotations
+
+from torch.autograd import Function
+
+from . import _lib
+
+
+def packed_attention(query, key, value, offsets, key_offsets=None, causal=True, scale=None):
+    """``out[t, h] = sum_j softmax_j(scale * <query[t, h], key[j, g]>) value[j, g]`` over the keys j that token t sees; g is the key head that
+    query head h shares, ``h // (heads // groups)``.  Differentiable with respect to query, key and value.
+
+    ``query`` [T, heads, dim]; ``key``, ``value`` [S, groups, dim]: float32, float16 or bfloat16, dim a multiple of 8 up to 128, any strides (a
+    tensor whose rows are not dense and 16-byte aligned is copied).  ``offsets`` [B + 1], int32 on the device: sequence b is the tokens
+    ``offsets[b]`` to ``offsets[b + 1]``, and its keys ``key_offsets[b]`` to ``key_offsets[b + 1]`` (``offsets`` where not given).  With ``causal``
+    token i of a sequence sees the keys j <= i + keys - tokens, without it all of its sequence.  ``scale``: 1 / sqrt(dim) where not given.
+
+    A token that sees no key gets 0, and so do rows of no sequence.  What a token does not see has no part in its output or in any
+    gradient, not even if it is infinite or NaN.  The lengths stay on the device: the call can be captured into a graph and replayed with
+    others.  Deterministic."""
+    if _lib.transformed():
+        return PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, causal, scale)
+    return (_lib.host or _lib.load_host()).packed_attention(query, key, value, offsets, key_offsets, causal, scale)
+
+
+class PackedAttentionFunction(Function):
+    """``packed_attention`` for traces and transforms."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, offsets, key_offsets, causal, scale):
+        out, lse, scale = _lib.load_host().packed_attention_forward(query, key, value, offsets, key_offsets, causal, scale)
+        ctx.config = (causal, scale)
+        ctx.save_for_backward(query, key, value, out, lse, offsets, offsets if key_offsets is None else key_offsets)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return (*_lib.load_host().packed_attention_backward(grad_output, *ctx.saved_tensors, *ctx.config), None, None, None, None)
+
+
+def paged_attention(query, key_pages, value_pages, page_table, key_lengths, offsets, causal=True, scale=None):
+    """Attention of new tokens over a paged cache; forward only.
+
+    ``query`` [T, heads, dim], packed as in :func:`packed_attention`; ``key_pages``, ``value_pages`` [pages, page, groups, dim] of any strides that are
+    multiples of 16 bytes; ``page_table`` [B, most pages] and ``key_lengths`` [B], int32 on the device.  Position p of sequence b lies in slot
+    ``p % page`` of page ``page_table[b, p // page]``; its keys are the positions below ``key_lengths[b]``, which counts the new tokens: with ``causal``
+    token i of Lq sees the positions up to ``key_lengths[b] - Lq + i``.
+
+    Entries of the table behind a sequence's last page are not read.  A token that sees a position whose page number lies outside the
+    cache, or that the table has no entry for, gets NaN; the page is not read."""
+    return (_lib.host or _lib.load_host()).paged_attention(query, key_pages, value_pages, page_table, key_lengths, offsets, causal, scale)
+
+
+def paged_write(key, value, key_pages, value_pages, page_table, key_lengths, offsets):
+    """Put new keys and values, [T, groups, dim] packed by ``offsets``, into the cache in place: token i of the Lq new ones of sequence b goes to
+    position ``key_lengths[b] - Lq + i``, so ``key_lengths`` already counts them.  Positions below 0 or without a page inside the cache
+    are skipped; nothing else of the cache is touched.  No two tokens of a call may go to the same slot."""
+    (_lib.host or _lib.load_host()).paged_write(key, value, key_pages, value_pages, page_table, key_lengths, offsets)

@@ -18,13 +18,13 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libsapa_b200.so")
 SOURCES = ["api.cu", "sapa_b.cu", "sapa_mma.cu", "sapa_tma.cu", "sapa_gath_mma.cu", "sapa_d.cu", "sapa_proj.cu", "sapa_proj_mm.cu",
-           "sapa_nhwc.cu"]
-HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "tma_util.cuh"), os.path.join(CSRC, "umma_util.cuh"), os.path.join(CSRC, "finite.cuh"), os.path.join(CSRC, "sapa_gath_umma.cuh"), os.path.join(CSRC, "sapa_strip.cuh"), os.path.join(CSRC, "sapa_strip_fwd.cuh"), os.path.join(CSRC, "sapa_strip_sim.cuh"), os.path.join(CSRC, "sapa_strip_sim16.cuh"), os.path.join(CSRC, "proj_mm.h"), os.path.join(CSRC, "sapa_wide16.cuh"), os.path.join(CSRC, "sapa_gath_wide16.cuh"),
+           "sapa_nhwc.cu", "attention.cu"]
+HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "tma_util.cuh"), os.path.join(CSRC, "umma_util.cuh"), os.path.join(CSRC, "finite.cuh"), os.path.join(CSRC, "sapa_gath_umma.cuh"), os.path.join(CSRC, "sapa_strip.cuh"), os.path.join(CSRC, "sapa_strip_fwd.cuh"), os.path.join(CSRC, "sapa_strip_sim.cuh"), os.path.join(CSRC, "sapa_strip_sim16.cuh"), os.path.join(CSRC, "proj_mm.h"), os.path.join(CSRC, "sapa_wide16.cuh"), os.path.join(CSRC, "sapa_gath_wide16.cuh"), os.path.join(CSRC, "attention.cuh"),
            os.path.join(INCLUDE, "sapa_b200.h")]
 
 HOST = os.path.join(HERE, "_host.so")
 HOST_TAG = os.path.join(HERE, "build", "_host.tag")      # what _host.so was built for
-HOST_SOURCES = [os.path.join(CSRC, f) for f in ("host.cpp", "host_sapa.inc", "host_deform.inc", "host_module.inc")]
+HOST_SOURCES = [os.path.join(CSRC, f) for f in ("host.cpp", "host_sapa.inc", "host_deform.inc", "host_module.inc", "host_attention.inc")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,734 @@
+// attention.cu — attention over sequences of tokens: the entry points, and the kernels on the FP32 pipe, which serve float32 and the pages that
+// the tensor-core kernels (attention_umma.cu) do not take.
+//
+// One pass over the keys with the running maximum m and sum l of the softmax: a tile's scores s change m to m', l to
+// l 2^(m - m') + sum 2^(s - m') and the output sum the same way (base 2, with log2(e) in the scale).  The query heads that share a key head
+// are rows of one block (row = token x head), so that a key is read once for all of them.
+#include "attention.cuh"
+#include "tma_util.cuh"
+
+#include <cmath>
+
+namespace sapa {
+namespace attn {
+
+namespace rows {
+
+constexpr int NT = 256, KT = 64;              // threads; keys of a tile
+constexpr int LEAST = 2;                      // TILEs of a part at least
+template <int RI, int DP> struct Lay {
+    static constexpr int BM = 16 * RI, QS = DP + 4, PS = KT + 4;
+    static constexpr int Q0 = 0, K0 = Q0 + BM * QS, V0 = K0 + KT * QS, P0 = V0 + KT * DP, END = P0 + BM * PS;
+    static constexpr size_t SMEM = (size_t)END * sizeof(float);
+};
+
+template <typename T> __device__ __forceinline__ float4 load4(const T *p);
+template <> __device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 widen(__half2 a, __half2 b) { const float2 x = __half22float2(a), y = __half22float2(b); return make_float4(x.x, x.y, y.x, y.y); }
+__device__ __forceinline__ float4 widen(__nv_bfloat162 a, __nv_bfloat162 b) {
+    const float2 x = __bfloat1622float2(a), y = __bfloat1622float2(b);
+    return make_float4(x.x, x.y, y.x, y.y);
+}
+template <> __device__ __forceinline__ float4 load4(const __half *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    return widen(*reinterpret_cast<const __half2 *>(&u.x), *reinterpret_cast<const __half2 *>(&u.y));
+}
+template <> __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    return widen(*reinterpret_cast<const __nv_bfloat162 *>(&u.x), *reinterpret_cast<const __nv_bfloat162 *>(&u.y));
+}
+__device__ __forceinline__ void store4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+__device__ __forceinline__ bool finite4(float4 v) { return isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w); }
+__device__ __forceinline__ float at(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+template <typename T> __device__ __forceinline__ void put4(T *p, float4 v);
+template <> __device__ __forceinline__ void put4(float *p, float4 v) { store4(p, v); }
+template <typename T> __device__ __forceinline__ void put4(T *p, float4 v) {
+    T e[4] = {from_acc<T>(v.x), from_acc<T>(v.y), from_acc<T>(v.z), from_acc<T>(v.w)};
+    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(e);
+}
+
+}  // namespace rows
+
+// RI: rows of a thread (a block has 16 of them across), DP: channels in shared memory.  256 threads as 16 x 16: rows ty + 16 i, of the scores
+// the keys tx + 16 j, of the output the channels 4 tx + 64 j.  What bounds it: the FP32 pipe and the shared-memory reads that feed it (12 wide loads
+// to 128 FMAs for the scores); with one row a thread (single tokens) reading the keys.
+template <typename T, int RI, int DP>
+__global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __grid_constant__ Args p) {
+    using namespace rows;
+    using L = Lay<RI, DP>;
+    extern __shared__ __align__(16) float sm[];
+    __shared__ Plan plan;
+    __shared__ int bad_page;
+    const sapa_attention &a = p.a;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int group = blockIdx.x % a.groups, tok = L::BM / p.share, D = a.dim;
+    begin_after_previous();
+    if (tid < 32) {
+        const Plan r = plan_at(p, blockIdx.x / a.groups, tok, LEAST, tid);
+        if (tid == 0) { plan = r; bad_page = 0x7fffffff; }
+    }
+    clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, tid, NT);
+    if (a.lse != nullptr) clear_outside(a.lse, a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);
+    __syncthreads();
+    const Item it = plan.it;
+    if (!it.there) return;
+    const Sequence s = sequence_at(a, it.b);
+    const int first = it.block * tok, used = min(tok, s.nq - first) * p.share;          // first token, rows in use
+    int lim[RI];
+    float m[RI], l[RI], o[RI][DP / 16];
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+        const int r = ty + 16 * i;
+        lim[i] = r < used ? sees(s, first + r / p.share, a.causal) : 0;
+        m[i] = -INFINITY; l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) o[i][c] = 0.f;
+    }
+    const int least = sees(s, first, a.causal), most = sees(s, first + used / p.share - 1, a.causal);      // of the block's tokens
+    const int room = min(most, s.bad);                                                   // positions that are there to be read
+    const long long from = (long long)it.part * plan.tiles * TILE, upto = min((long long)room, from + (long long)plan.tiles * TILE);
+    if (tid == 0 && s.bad < most) bad_page = s.bad;
+
+    for (int e = tid; e < L::BM * (DP / 4); e += NT) {
+        const int r = e / (DP / 4), c = e % (DP / 4) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < used && c < D)
+            v = load4(static_cast<const T *>(a.query) + (long long)(s.q0 + first + r / p.share) * a.query_strides[0] +
+                      (long long)(group * p.share + r % p.share) * a.query_strides[1] + c);
+        store4(sm + L::Q0 + r * L::QS + c, v);
+    }
+    for (int k0 = (int)from; k0 < upto; k0 += KT) {
+        const int n = min(KT, (int)upto - k0);
+        bool odd = false;
+        __syncthreads();
+        for (int e = tid; e < KT * (DP / 4); e += NT) {
+            const int r = e / (DP / 4), c = e % (DP / 4) * 4;
+            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+            if (r < n && c < D) {
+                const T *kp = key_row<T>(a, s, it.b, k0 + r, a.key, a.key_strides), *vp = key_row<T>(a, s, it.b, k0 + r, a.value, a.value_strides);
+                if (kp == nullptr) {
+                    atomicMin(&bad_page, k0 + r);
+                } else {
+                    k = load4(kp + group * a.key_strides[1] + c);
+                    v = load4(vp + group * a.value_strides[1] + c);
+                }
+            }
+            odd = odd || !finite4(v);
+            store4(sm + L::K0 + r * L::QS + c, k);
+            store4(sm + L::V0 + r * DP + c, v);
+        }
+        // a value that a row does not see must not reach it, not even as 0 * infinity
+        const bool careful = __syncthreads_or(odd && k0 + KT > least);
+        float sc[RI][4];
+#pragma unroll
+        for (int i = 0; i < RI; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+#pragma unroll 2
+        for (int c = 0; c < DP; c += 4) {
+            float4 k[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4 *>(sm + L::K0 + (tx + 16 * j) * L::QS + c);
+#pragma unroll
+            for (int i = 0; i < RI; ++i) {
+                const float4 q = *reinterpret_cast<const float4 *>(sm + L::Q0 + (ty + 16 * i) * L::QS + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[i][j] = fmaf(q.w, k[j].w, fmaf(q.z, k[j].z, fmaf(q.y, k[j].y, fmaf(q.x, k[j].x, sc[i][j]))));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RI; ++i) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sc[i][j] = k0 + tx + 16 * j < lim[i] && tx + 16 * j < n ? sc[i][j] * p.scale_log2 : -INFINITY;
+                top = fmaxf(top, sc[i][j]);
+            }
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float now = fmaxf(m[i], top), base = now == -INFINITY ? 0.f : now, old = exp2f(m[i] - base);
+            m[i] = now;
+            l[i] *= old;
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) o[i][c] *= old;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w = exp2f(sc[i][j] - base);
+                l[i] += w;
+                sm[L::P0 + (ty + 16 * i) * L::PS + tx + 16 * j] = w;
+            }
+        }
+        __syncwarp();                          // the 16 threads that share a row are in one warp
+        if (!careful) {
+#pragma unroll 2
+            for (int k = 0; k < KT; k += 4) {
+                float4 w[RI];
+#pragma unroll
+                for (int i = 0; i < RI; ++i) w[i] = *reinterpret_cast<const float4 *>(sm + L::P0 + (ty + 16 * i) * L::PS + k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < DP / 64; ++j) {
+                        const float4 v = *reinterpret_cast<const float4 *>(sm + L::V0 + (k + e) * DP + 4 * tx + 64 * j);
+#pragma unroll
+                        for (int i = 0; i < RI; ++i) {
+                            const float x = at(w[i], e);
+                            o[i][4 * j] = fmaf(x, v.x, o[i][4 * j]); o[i][4 * j + 1] = fmaf(x, v.y, o[i][4 * j + 1]);
+                            o[i][4 * j + 2] = fmaf(x, v.z, o[i][4 * j + 2]); o[i][4 * j + 3] = fmaf(x, v.w, o[i][4 * j + 3]);
+                        }
+                    }
+            }
+        } else {
+            for (int k = 0; k < n; ++k)
+#pragma unroll
+                for (int i = 0; i < RI; ++i)
+                    if (k0 + k < lim[i]) {
+                        const float w = sm[L::P0 + (ty + 16 * i) * L::PS + k];
+#pragma unroll
+                        for (int c = 0; c < DP / 16; ++c) o[i][c] = fmaf(w, sm[L::V0 + k * DP + 4 * tx + 64 * (c >> 2) + (c & 3)], o[i][c]);
+                    }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+        const int r = ty + 16 * i;
+        float sum = l[i];
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (r >= used) continue;
+        const bool none = lim[i] <= from, lost = lim[i] > bad_page;       // no key seen here; one that cannot be read
+        const float nan = __int_as_float(0x7fffffff);
+        const int head = group * p.share + r % p.share;
+        const long long row = (long long)(s.q0 + first + r / p.share) * a.heads + head;
+        if (it.parts == 1) {
+            const float inv = none ? 0.f : lost ? nan : 1.f / sum;        // 0 / 0 where every score is -infinity, as the formula has it
+            T *out = static_cast<T *>(a.out) + row * D;
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j)
+                if (4 * tx + 64 * j < D)
+                    put4(out + 4 * tx + 64 * j, none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv));
+            if (a.lse != nullptr && tx == 0) a.lse[row] = none ? -INFINITY : lost || sum == 0.f ? nan : (m[i] + log2f(sum)) * 0.6931471805599453f;
+        } else {
+            const float inv = sum == 0.f ? 0.f : lost ? nan : 1.f / sum;
+            const long long at = ((long long)blockIdx.x * L::BM + r);
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j)
+                if (4 * tx + 64 * j < D)
+                    store4(p.part + at * D + 4 * tx + 64 * j, make_float4(o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv));
+            if (tx == 0) p.part_lse[at] = lost ? nan : sum == 0.f ? -INFINITY : m[i] + log2f(sum);
+        }
+    }
+}
+
+// Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(lse_p - max lse).  A block of the grid per block and group, a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_constant__ Args p, int bm, int tok, int least) {
+    const sapa_attention &a = p.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x % a.groups, D = a.dim;
+    begin_after_previous();
+    const Plan plan = split_at<false>(p, blockIdx.x / a.groups, tok, least, lane);
+    if (!plan.it.there || plan.it.parts == 1) return;
+    const Sequence s = sequence_at(a, plan.it.b);
+    const int first = plan.it.block * tok, used = min(tok, s.nq - first) * p.share;
+    const long long step = (long long)a.groups * bm;                                  // from a part to the next
+    for (int r = warp; r < used; r += 8) {
+        const long long at = ((long long)plan.first * a.groups + group) * bm + r;
+        const int parts = plan.it.parts, lim = sees(s, first + r / p.share, a.causal);
+        float top = -INFINITY;
+        bool lost = false;
+        for (int q = lane; q < parts; q += 32) { const float e = p.part_lse[at + q * step]; top = fmaxf(top, e); lost = lost || e != e; }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        lost = __any_sync(0xffffffffu, lost) || (lim > 0 && top == -INFINITY);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < parts; ++q) {
+            const float e = p.part_lse[at + q * step];
+            if (e == -INFINITY) continue;
+            const float w = exp2f(e - top);
+            sum += w;
+            if (4 * lane < D) {
+                const float4 v = *reinterpret_cast<const float4 *>(p.part + (at + q * step) * D + 4 * lane);
+                acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+            }
+        }
+        const float inv = lost ? __int_as_float(0x7fffffff) : lim <= 0 ? 0.f : 1.f / sum;
+        const long long row = (long long)(s.q0 + first + r / p.share) * a.heads + group * p.share + r % p.share;
+        if (4 * lane < D) rows::put4(static_cast<T *>(a.out) + row * D + 4 * lane, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (a.lse != nullptr && lane == 0) a.lse[row] = lost ? __int_as_float(0x7fffffff) : lim <= 0 ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    }
+}
+
+// ---------------------------------------------------------------------------------- backward
+struct Grads {
+    const void *go;
+    long long go_strides[2];
+    void *gq, *gk, *gv;
+    float *delta;                  // [tokens, heads]: sum over channels of grad_out * out
+};
+
+// delta, and what lies outside the sequences: a warp per token and head.
+template <typename T>
+__global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
+    const sapa_attention &a = p.a;
+    const int lane = threadIdx.x & 31, D = a.dim;
+    begin_after_previous();
+    const long long n = (long long)a.tokens * a.heads, all = (long long)gridDim.x * 8;
+    for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < n; row += all) {
+        float sum = 0.f;
+        if (4 * lane < D) {
+            const float4 x = rows::load4(static_cast<const T *>(a.out) + row * D + 4 * lane);
+            const float4 y = rows::load4(static_cast<const T *>(g.go) + row / a.heads * g.go_strides[0] + row % a.heads * g.go_strides[1] + 4 * lane);
+            sum = x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) g.delta[row] = sum;
+    }
+    clear_outside(static_cast<T *>(g.gq), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
+    clear_outside(static_cast<T *>(g.gk), a.key_offsets, a.B, a.keys, a.groups * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
+    clear_outside(static_cast<T *>(g.gv), a.key_offsets, a.B, a.keys, a.groups * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
+}
+
+namespace grad {
+using namespace rows;
+constexpr int N = 64, WS = N + 4;             // rows and keys of a tile
+template <int DP> struct Lay {
+    static constexpr int XS = DP + 4;
+    static constexpr int Q0 = 0, O0 = N * XS, K0 = 2 * N * XS, V0 = 3 * N * XS, P0 = 4 * N * XS, S0 = P0 + N * WS, L0 = S0 + N * WS, END = L0 + 2 * N;
+    static constexpr size_t SMEM = (size_t)END * sizeof(float);
+};
+}  // namespace grad
+
+// KEYS: gradients of 64 keys and values, over the rows that see them; otherwise those of 64 query rows, over the keys that they see.  P and dS of
+// a tile are formed again from the scores, lse and delta: P = 2^(s - lse), dS = P (dP - delta); no atomics.
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
+    using namespace grad;
+    using L = grad::Lay<DP>;
+    extern __shared__ __align__(16) float sm[];
+    __shared__ Item item;
+    const sapa_attention &a = p.a;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.dim;
+    const int share = p.share, heads_at_once = min(share, N), tok = N / heads_at_once;       // of a row tile; more heads than rows: in turns
+    const int turns = KEYS ? (share + N - 1) / N : 1;
+    const int slots = KEYS ? a.groups : a.groups * ((share + N - 1) / N);
+    const int slot = blockIdx.x % slots, group = KEYS ? slot : slot % a.groups;
+    begin_after_previous();
+    if (tid < 32) {
+        const Item r = KEYS ? block_at<false>(blockIdx.x / slots, a.B, tid, [&](int b) { return (sequence_at(a, b).nk + N - 1) / N; })
+                            : block_at<true>(blockIdx.x / slots, a.B, tid, [&](int b) { return (sequence_at(a, b).nq + tok - 1) / tok; });
+        if (tid == 0) item = r;
+    }
+    __syncthreads();
+    if (!item.there) return;
+    const int b = item.b, block = item.block;
+    const Sequence s = sequence_at(a, b);
+
+    auto load_keys = [&](int k0) {             // returns whether something is not finite among the keys
+        bool odd = false;
+        for (int e = tid; e < N * (DP / 4); e += NT) {
+            const int r = e / (DP / 4), c = e % (DP / 4) * 4;
+            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+            if (k0 + r < s.nk && c < D) {
+                k = load4(static_cast<const T *>(a.key) + (long long)(s.k0 + k0 + r) * a.key_strides[0] + group * a.key_strides[1] + c);
+                v = load4(static_cast<const T *>(a.value) + (long long)(s.k0 + k0 + r) * a.value_strides[0] + group * a.value_strides[1] + c);
+            }
+            odd = odd || !finite4(k);
+            store4(sm + L::K0 + r * L::XS + c, k);
+            store4(sm + L::V0 + r * L::XS + c, v);
+        }
+        return odd;
+    };
+    auto load_queries = [&](int i0, int h0, int used) {
+        bool odd = false;
+        for (int e = tid; e < N * (DP / 4); e += NT) {
+            const int r = e / (DP / 4), c = e % (DP / 4) * 4;
+            float4 q = make_float4(0.f, 0.f, 0.f, 0.f), o = q;
+            if (r < used) {
+                const long long t = s.q0 + i0 + r / heads_at_once, h = group * share + h0 + r % heads_at_once;
+                if (c < D && h0 + r % heads_at_once < share) {
+                    q = load4(static_cast<const T *>(a.query) + t * a.query_strides[0] + h * a.query_strides[1] + c);
+                    o = load4(static_cast<const T *>(g.go) + t * g.go_strides[0] + h * g.go_strides[1] + c);
+                }
+            }
+            odd = odd || !finite4(q) || !finite4(o);
+            store4(sm + L::Q0 + r * L::XS + c, q);
+            store4(sm + L::O0 + r * L::XS + c, o);
+        }
+        for (int r = tid; r < N; r += NT) {
+            float e = 0.f, d = 0.f;
+            if (r < used && h0 + r % heads_at_once < share) {
+                const long long at = (long long)(s.q0 + i0 + r / heads_at_once) * a.heads + group * share + h0 + r % heads_at_once;
+                e = a.lse[at] * 1.4426950408889634f;
+                d = g.delta[at];
+            }
+            sm[L::L0 + r] = e;
+            sm[L::L0 + N + r] = d;
+        }
+        return odd;
+    };
+    float x[4][DP / 16], y[4][DP / 16];        // KEYS: of values, of keys; otherwise y: of queries
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) x[i][c] = y[i][c] = 0.f;
+
+    // a tile: rows of tokens from i0, heads from h0; keys from k0
+    auto tile = [&](int i0, int h0, int used, int k0, bool odd) {
+        int lim[4];
+        bool whole = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = ty + 16 * i;
+            lim[i] = r < used && h0 + r % heads_at_once < share ? sees(s, i0 + r / heads_at_once, a.causal) : 0;
+            whole = whole && (lim[i] >= k0 + N);
+        }
+        const bool careful = __syncthreads_or(odd);
+        float sc[4][4], dp[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[i][j] = dp[i][j] = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 4) {
+            float4 k[4], v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                k[j] = *reinterpret_cast<const float4 *>(sm + L::K0 + (tx + 16 * j) * L::XS + c);
+                v[j] = *reinterpret_cast<const float4 *>(sm + L::V0 + (tx + 16 * j) * L::XS + c);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 q = *reinterpret_cast<const float4 *>(sm + L::Q0 + (ty + 16 * i) * L::XS + c);
+                const float4 o = *reinterpret_cast<const float4 *>(sm + L::O0 + (ty + 16 * i) * L::XS + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sc[i][j] = fmaf(q.w, k[j].w, fmaf(q.z, k[j].z, fmaf(q.y, k[j].y, fmaf(q.x, k[j].x, sc[i][j]))));
+                    dp[i][j] = fmaf(o.w, v[j].w, fmaf(o.z, v[j].z, fmaf(o.y, v[j].y, fmaf(o.x, v[j].x, dp[i][j]))));
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = ty + 16 * i;
+            const float lse = sm[L::L0 + r], delta = sm[L::L0 + N + r];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = tx + 16 * j;
+                const float w = k0 + k < lim[i] ? exp2f(fmaf(sc[i][j], p.scale_log2, -lse)) : 0.f;
+                const float ds = k0 + k < lim[i] ? w * (dp[i][j] - delta) : 0.f;
+                if (KEYS) {
+                    sm[L::P0 + r * WS + k] = w;
+                    sm[L::S0 + r * WS + k] = ds;
+                } else {
+                    sm[L::S0 + k * WS + r] = ds;
+                }
+            }
+        }
+        __syncthreads();
+        if (!careful) {
+#pragma unroll 2
+            for (int n = 0; n < N; ++n) {      // rows (KEYS) or keys
+                const float4 w = KEYS ? *reinterpret_cast<const float4 *>(sm + L::P0 + n * WS + 4 * ty) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 ds = *reinterpret_cast<const float4 *>(sm + L::S0 + n * WS + 4 * ty);
+#pragma unroll
+                for (int j = 0; j < DP / 64; ++j) {
+                    const float4 f = *reinterpret_cast<const float4 *>(sm + (KEYS ? L::Q0 : L::K0) + n * L::XS + 4 * tx + 64 * j);
+                    const float4 o = KEYS ? *reinterpret_cast<const float4 *>(sm + L::O0 + n * L::XS + 4 * tx + 64 * j) : f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (KEYS) x[i][4 * j + e] = fmaf(at(w, i), at(o, e), x[i][4 * j + e]);
+                            y[i][4 * j + e] = fmaf(at(ds, i), at(f, e), y[i][4 * j + e]);
+                        }
+                }
+            }
+        } else {                               // what is not seen must not reach a gradient, not even as 0 * infinity
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = KEYS ? n : 4 * ty + i, k = KEYS ? 4 * ty + i : n;
+                    if (r >= used || h0 + r % heads_at_once >= share || k0 + k >= sees(s, i0 + r / heads_at_once, a.causal)) continue;
+#pragma unroll
+                    for (int c = 0; c < DP / 16; ++c) {
+                        const int col = 4 * tx + 64 * (c >> 2) + (c & 3);
+                        if (KEYS) x[i][c] = fmaf(sm[L::P0 + n * WS + 4 * ty + i], sm[L::O0 + n * L::XS + col], x[i][c]);
+                        y[i][c] = fmaf(sm[L::S0 + n * WS + 4 * ty + i], sm[(KEYS ? L::Q0 : L::K0) + n * L::XS + col], y[i][c]);
+                    }
+                }
+        }
+    };
+
+    if (KEYS) {
+        const int k0 = block * N;
+        load_keys(k0);
+        const int from = a.causal ? (int)max(0ll, (long long)k0 - s.nk + s.nq) : 0;      // the first token that sees one of them
+        for (int i0 = from; i0 < s.nq; i0 += tok)
+            for (int turn = 0; turn < turns; ++turn) {
+                const int used = min(tok, s.nq - i0) * heads_at_once;
+                __syncthreads();
+                const bool odd = load_queries(i0, turn * N, used);
+                tile(i0, turn * N, used, k0, odd);
+            }
+    } else {
+        const int i0 = block * tok, h0 = slot / a.groups * N, used = min(tok, s.nq - i0) * heads_at_once;
+        const int most = sees(s, i0 + used / heads_at_once - 1, a.causal);
+        load_queries(i0, h0, used);
+        for (int k0 = 0; k0 < most; k0 += N) {
+            __syncthreads();
+            const bool odd = load_keys(k0);
+            tile(i0, h0, used, k0, odd);
+        }
+    }
+    // the scores' scale is in the gradients of queries and keys
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = 4 * ty + i;
+        long long row;
+        if (KEYS) {
+            if (block * N + n >= s.nk) continue;
+            row = (long long)(s.k0 + block * N + n) * a.groups + group;
+        } else {
+            const int i0 = block * tok, h = slot / a.groups * N + n % heads_at_once;
+            if (n >= min(tok, s.nq - i0) * heads_at_once || h >= share) continue;
+            row = (long long)(s.q0 + i0 + n / heads_at_once) * a.heads + group * share + h;
+        }
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+            const int c = 4 * tx + 64 * j;
+            if (c >= D) continue;
+            const float f = a.scale;
+            put4(static_cast<T *>(KEYS ? g.gk : g.gq) + row * D + c, make_float4(y[i][4 * j] * f, y[i][4 * j + 1] * f, y[i][4 * j + 2] * f, y[i][4 * j + 3] * f));
+            if (KEYS) put4(static_cast<T *>(g.gv) + row * D + c, make_float4(x[i][4 * j], x[i][4 * j + 1], x[i][4 * j + 2], x[i][4 * j + 3]));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------- writing into a paged cache
+// A thread moves 16 bytes of a token's key row and of its value row.  What bounds it: reading and writing them once; for single tokens the launch.
+__global__ void __launch_bounds__(256) sapa_paged_write_kernel(const __grid_constant__ sapa_paged_rows a, int esize) {
+    begin_after_previous();
+    const int chunks = a.dim * esize / 16, per_row = a.groups * chunks;
+    const long long n = (long long)a.tokens * per_row;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const int t = (int)(i / per_row), rest = (int)(i % per_row), group = rest / chunks, c = rest % chunks;
+        // the first sequence whose end lies behind the token
+        int lo = 0, hi = a.B;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (a.offsets[mid + 1] > t) hi = mid; else lo = mid + 1;
+        }
+        if (lo == a.B || t < a.offsets[lo]) continue;
+        const long long at = (long long)a.key_lengths[lo] - min(a.offsets[lo + 1], a.tokens) + t;
+        if (at < 0 || at >= (long long)a.max_pages * a.page) continue;
+        const int page = a.page_table[(long long)lo * a.max_pages + at / a.page], slot = (int)(at % a.page);
+        if ((unsigned)page >= (unsigned)a.pages) continue;
+        auto move = [&](const void *from, const long long (&fs)[2], void *to, const long long (&ts)[3]) {
+            const char *src = static_cast<const char *>(from) + ((long long)t * fs[0] + group * fs[1]) * esize + 16 * c;
+            char *dst = static_cast<char *>(to) + (page * ts[2] + slot * ts[0] + group * ts[1]) * esize + 16 * c;
+            *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+        };
+        move(a.key, a.key_strides, a.key_pages, a.key_page_strides);
+        move(a.value, a.value_strides, a.value_pages, a.value_page_strides);
+    }
+}
+
+// ---------------------------------------------------------------------------------- host side
+static int check(const sapa_attention *a, int dtype, const char *fn) {
+    SAPA_REQUIRE(a != nullptr, SAPA_ERR_ARGUMENT, "%s: the arguments are NULL", fn);
+    SAPA_REQUIRE(dtype == SAPA_F32 || dtype == SAPA_F16 || dtype == SAPA_BF16, SAPA_ERR_DTYPE, "%s: dtype code %d is not supported", fn, dtype);
+    SAPA_REQUIRE(a->B >= 0 && a->tokens >= 0 && a->keys >= 0, SAPA_ERR_ARGUMENT, "%s: negative size", fn);
+    SAPA_REQUIRE(a->heads > 0 && a->groups > 0 && a->heads % a->groups == 0, SAPA_ERR_ARGUMENT, "%s: %d heads do not share %d key heads evenly", fn, a->heads, a->groups);
+    SAPA_REQUIRE(a->heads / a->groups <= 128, SAPA_ERR_UNSUPPORTED, "%s: more than 128 heads share a key head", fn);
+    SAPA_REQUIRE(a->dim > 0 && a->dim <= 128 && a->dim % 8 == 0, SAPA_ERR_UNSUPPORTED, "%s: dim %d is not a multiple of 8 up to 128", fn, a->dim);
+    SAPA_REQUIRE(std::isfinite(a->scale), SAPA_ERR_ARGUMENT, "%s: the scale is not finite", fn);
+    SAPA_REQUIRE(a->offsets != nullptr, SAPA_ERR_ARGUMENT, "%s: offsets is NULL", fn);
+    if (a->page_table != nullptr) {
+        SAPA_REQUIRE(a->key_lengths != nullptr, SAPA_ERR_ARGUMENT, "%s: key_lengths is NULL", fn);
+        SAPA_REQUIRE(a->pages > 0 && a->page > 0 && a->max_pages > 0, SAPA_ERR_ARGUMENT, "%s: pages, page and max_pages must be positive", fn);
+        SAPA_REQUIRE((long long)a->max_pages * a->page < 0x7fffff00ll, SAPA_ERR_UNSUPPORTED, "%s: more than 2^31 positions", fn);
+    } else {
+        SAPA_REQUIRE(a->key_offsets != nullptr, SAPA_ERR_ARGUMENT, "%s: key_offsets is NULL", fn);
+    }
+    const long long quantum = 16 / (long long)dtype_size(dtype);
+    for (long long s : {a->query_strides[0], a->query_strides[1], a->key_strides[0], a->key_strides[1], a->value_strides[0], a->value_strides[1]})
+        SAPA_REQUIRE(s >= 0 && s % quantum == 0, SAPA_ERR_ALIGNMENT, "%s: strides must be multiples of 16 bytes", fn);
+    if (a->page_table != nullptr)
+        SAPA_REQUIRE(a->key_strides[2] >= 0 && a->value_strides[2] >= 0 && a->key_strides[2] % quantum == 0 && a->value_strides[2] % quantum == 0, SAPA_ERR_ALIGNMENT,
+                     "%s: strides must be multiples of 16 bytes", fn);
+    if (a->tokens == 0) return SAPA_OK;
+    SAPA_REQUIRE(a->query != nullptr && a->out != nullptr, SAPA_ERR_ARGUMENT, "%s: query or out is NULL", fn);
+    SAPA_REQUIRE(a->keys == 0 || (a->key != nullptr && a->value != nullptr), SAPA_ERR_ARGUMENT, "%s: key or value is NULL", fn);
+    SAPA_REQUIRE(all_aligned16(a->query, a->key, a->value, a->out), SAPA_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", fn);
+    return SAPA_OK;
+}
+
+static Args args_of(const sapa_attention *a) {
+    Args p{};
+    p.a = *a;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.share = a->heads / a->groups;
+    return p;
+}
+
+// Blocks of `tok` tokens that all sequences together can have.
+static long long most_blocks(const sapa_attention &a, long long total, int tok) {
+    const long long n = total / tok + a.B;
+    return n < total ? n : total;
+}
+
+// A forward of this call: rows of a block, whether its keys are split, and the room that takes.
+struct Shape {
+    bool umma, narrow;
+    int bm, tok, split;
+    long long blocks, grid;        // blocks x groups at most; items at most
+    size_t part, lse, bytes;       // of the workspace
+};
+static Shape shape_of(const Args &p, int dtype, int sms) {
+    const sapa_attention &a = p.a;
+    Shape s{};
+    s.umma = false;
+    // single tokens and short chunks: 16 rows a block, as long as an average sequence has no more
+    s.narrow = p.share <= 16 && (long long)a.tokens * p.share <= 16ll * a.B;
+    s.bm = s.narrow ? 16 : 128;
+    s.tok = s.bm / p.share;
+    s.blocks = most_blocks(a, a.tokens, s.tok) * a.groups;
+    s.grid = s.blocks;
+    // few blocks: their keys are split so that every SM has items
+    const long long keys = a.page_table != nullptr ? (long long)a.max_pages * a.page : a.keys;
+    if (s.blocks < 4ll * sms && keys > TILE) {
+        s.split = 4 * sms;
+        s.grid = s.blocks + s.split;
+        s.part = (size_t)s.grid * s.bm * a.dim * sizeof(float);
+        s.lse = (size_t)s.grid * s.bm * sizeof(float);
+        s.bytes = (s.part + s.lse + 255) / 256 * 256;
+    }
+    return s;
+}
+
+static int sm_count(const char *fn, int &sms) { return tmau::device_sms(fn, sms); }
+
+template <typename T, int RI, int DP> static int run_rows(const Args &p, const Shape &s, cudaStream_t st) {
+    using L = rows::Lay<RI, DP>;
+    int sms = 0;
+    if (int e = tmau::prepare_launch((const void *)sapa_attention_rows_kernel<T, RI, DP>, (int)L::SMEM, "sapa_attention_rows_kernel", sms)) return e;
+    launch_next(sapa_attention_rows_kernel<T, RI, DP>, dim3((unsigned)s.grid), dim3(rows::NT), L::SMEM, st, p);
+    return check_launch("sapa_attention_rows_kernel");
+}
+
+template <typename T, int DP, bool KEYS> static int run_grad(const Args &p, const Grads &g, long long blocks, cudaStream_t st) {
+    using L = grad::Lay<DP>;
+    int sms = 0;
+    if (blocks == 0) return SAPA_OK;
+    if (int e = tmau::prepare_launch((const void *)sapa_attention_rows_grad_kernel<T, DP, KEYS>, (int)L::SMEM, "sapa_attention_rows_grad_kernel", sms)) return e;
+    launch_next(sapa_attention_rows_grad_kernel<T, DP, KEYS>, dim3((unsigned)blocks), dim3(rows::NT), L::SMEM, st, p, g);
+    return check_launch(KEYS ? "sapa_attention_rows_grad_kernel<keys>" : "sapa_attention_rows_grad_kernel<queries>");
+}
+
+}  // namespace attn
+}  // namespace sapa
+
+using namespace sapa;
+using namespace sapa::attn;
+
+extern "C" size_t sapa_attention_workspace(const sapa_attention *a, int dtype) {
+    int sms = 0;
+    if (check(a, dtype, "sapa_attention_workspace") != SAPA_OK || a->tokens == 0 || a->B == 0 || sm_count("sapa_attention_workspace", sms) != SAPA_OK) return 0;
+    return shape_of(args_of(a), dtype, sms).bytes;
+}
+
+extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, size_t workspace_bytes, int dtype, void *stream) {
+    const char *fn = "sapa_attention_forward";
+    trace_reset();
+    if (int e = check(a, dtype, fn)) return e;
+    if (a->tokens == 0) return SAPA_OK;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int sms = 0;
+    if (int e = sm_count(fn, sms)) return e;
+    Args p = args_of(a);
+    Shape s = shape_of(p, dtype, sms);
+    if (s.grid == 0) s.grid = 1;                     // no sequence: every row is cleared
+    SAPA_REQUIRE(s.grid < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
+    if (s.split > 0) {
+        SAPA_REQUIRE(workspace != nullptr && workspace_bytes >= s.bytes, SAPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, s.bytes, workspace_bytes);
+        SAPA_REQUIRE(aligned16(workspace), SAPA_ERR_ALIGNMENT, "%s: the workspace must be 256-byte aligned", fn);
+        p.split = s.split;
+        p.part = static_cast<float *>(workspace);
+        p.part_lse = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.part);
+    }
+    return SAPA_DISPATCH_FAST(dtype, [&]() -> int {
+        int e;
+        if (s.narrow) e = a->dim <= 64 ? run_rows<scalar_t, 1, 64>(p, s, st) : run_rows<scalar_t, 1, 128>(p, s, st);
+        else e = a->dim <= 64 ? run_rows<scalar_t, 8, 64>(p, s, st) : run_rows<scalar_t, 8, 128>(p, s, st);
+        if (e != SAPA_OK || s.split == 0) return e;
+        launch_next(sapa_attention_join_kernel<scalar_t>, dim3((unsigned)s.blocks), dim3(256), 0, st, p, s.bm, s.tok, rows::LEAST);
+        return check_launch("sapa_attention_join_kernel");
+    });
+}
+
+extern "C" size_t sapa_attention_backward_workspace(const sapa_attention *a, int dtype) {
+    if (check(a, dtype, "sapa_attention_backward_workspace") != SAPA_OK) return 0;
+    return ((size_t)a->tokens * a->heads * sizeof(float) + 255) / 256 * 256;
+}
+
+extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad_out, long long grad_token_stride, long long grad_head_stride,
+                                       void *grad_query, void *grad_key, void *grad_value, void *workspace, size_t workspace_bytes, int dtype,
+                                       void *stream) {
+    const char *fn = "sapa_attention_backward";
+    trace_reset();
+    if (int e = check(a, dtype, fn)) return e;
+    SAPA_REQUIRE(a->page_table == nullptr, SAPA_ERR_UNSUPPORTED, "%s: the paged form has no gradients", fn);
+    if (a->tokens == 0 && a->keys == 0) return SAPA_OK;
+    const long long quantum = 16 / (long long)dtype_size(dtype);
+    SAPA_REQUIRE(a->tokens == 0 || (grad_out != nullptr && grad_query != nullptr && a->lse != nullptr), SAPA_ERR_ARGUMENT, "%s: grad_out, grad_query or lse is NULL", fn);
+    SAPA_REQUIRE(a->keys == 0 || (grad_key != nullptr && grad_value != nullptr), SAPA_ERR_ARGUMENT, "%s: grad_key or grad_value is NULL", fn);
+    SAPA_REQUIRE(all_aligned16(grad_out, grad_query, grad_key, grad_value, workspace) && grad_token_stride >= 0 && grad_head_stride >= 0 &&
+                     grad_token_stride % quantum == 0 && grad_head_stride % quantum == 0,
+                 SAPA_ERR_ALIGNMENT, "%s: tensors and strides must be 16-byte aligned", fn);
+    const size_t need = sapa_attention_backward_workspace(a, dtype);
+    SAPA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), SAPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, workspace_bytes);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const Args p = args_of(a);
+    Grads g{grad_out, {grad_token_stride, grad_head_stride}, grad_query, grad_key, grad_value, static_cast<float *>(workspace)};
+    int sms = 0;
+    if (int e = sm_count(fn, sms)) return e;
+    const long long rows8 = ((long long)a->tokens * a->heads + 7) / 8, delta_grid = rows8 < 16ll * sms ? (rows8 > 0 ? rows8 : 1) : 16ll * sms;
+    const int slots = (p.share + grad::N - 1) / grad::N, tok = grad::N / (p.share < grad::N ? p.share : grad::N);
+    const long long key_blocks = most_blocks(*a, a->keys, grad::N) * a->groups, query_blocks = most_blocks(*a, a->tokens, tok) * a->groups * slots;
+    SAPA_REQUIRE(key_blocks < 0x7fffffffll && query_blocks < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
+    return SAPA_DISPATCH_FAST(dtype, [&]() -> int {
+        launch_next(sapa_attention_delta_kernel<scalar_t>, dim3((unsigned)delta_grid), dim3(256), 0, st, p, g);
+        if (int e = check_launch("sapa_attention_delta_kernel")) return e;
+        if (a->dim <= 64) {
+            if (int e = run_grad<scalar_t, 64, true>(p, g, key_blocks, st)) return e;
+            return run_grad<scalar_t, 64, false>(p, g, query_blocks, st);
+        }
+        if (int e = run_grad<scalar_t, 128, true>(p, g, key_blocks, st)) return e;
+        return run_grad<scalar_t, 128, false>(p, g, query_blocks, st);
+    });
+}
+
+extern "C" int sapa_paged_write(const sapa_paged_rows *a, int dtype, void *stream) {
+    const char *fn = "sapa_paged_write";
+    trace_reset();
+    SAPA_REQUIRE(a != nullptr, SAPA_ERR_ARGUMENT, "%s: the arguments are NULL", fn);
+    const long long esize = (long long)dtype_size(dtype);
+    SAPA_REQUIRE(esize != 0, SAPA_ERR_DTYPE, "%s: dtype code %d is not supported", fn, dtype);
+    SAPA_REQUIRE(a->B >= 0 && a->tokens >= 0 && a->groups > 0 && a->dim > 0 && a->pages > 0 && a->page > 0 && a->max_pages > 0, SAPA_ERR_ARGUMENT, "%s: sizes must be positive", fn);
+    SAPA_REQUIRE(a->dim * esize % 16 == 0, SAPA_ERR_UNSUPPORTED, "%s: rows must be multiples of 16 bytes", fn);
+    for (long long s : {a->key_strides[0], a->key_strides[1], a->value_strides[0], a->value_strides[1], a->key_page_strides[0], a->key_page_strides[1],
+                        a->key_page_strides[2], a->value_page_strides[0], a->value_page_strides[1], a->value_page_strides[2]})
+        SAPA_REQUIRE(s >= 0 && s * esize % 16 == 0, SAPA_ERR_ALIGNMENT, "%s: strides must be multiples of 16 bytes", fn);
+    if (a->tokens == 0 || a->B == 0) return SAPA_OK;
+    SAPA_REQUIRE(a->key != nullptr && a->value != nullptr && a->key_pages != nullptr && a->value_pages != nullptr, SAPA_ERR_ARGUMENT, "%s: a tensor is NULL", fn);
+    SAPA_REQUIRE(a->offsets != nullptr && a->page_table != nullptr && a->key_lengths != nullptr, SAPA_ERR_ARGUMENT, "%s: offsets, page_table or key_lengths is NULL", fn);
+    SAPA_REQUIRE(all_aligned16(a->key, a->value, a->key_pages, a->value_pages), SAPA_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", fn);
+    int sms = 0;
+    if (int e = sm_count(fn, sms)) return e;
+    const long long blocks = ((long long)a->tokens * a->groups * (a->dim * esize / 16) + 255) / 256;
+    launch_next(sapa_paged_write_kernel, dim3((unsigned)(blocks < 16ll * sms ? blocks : 16ll * sms)), dim3(256), 0, static_cast<cudaStream_t>(stream), *a, (int)esize);
+    return check_launch("sapa_paged_write_kernel");
+}

@@ -1,0 +1,189 @@
+// attention.cuh — what the kernels of attention over sequences share: the call's arguments on the device, where a sequence's tokens and keys
+// are, and which of them a block of the grid takes.
+#pragma once
+
+#include "common.cuh"
+
+namespace sapa {
+namespace attn {
+
+struct Args {
+    sapa_attention a;
+    float scale_log2;              // scale * log2(e): the softmax runs in base 2
+    int share;                     // query heads of a key head
+    int split;                     // > 0: items that a sequence's keys are spread over, see Plan
+    float *part, *part_lse;        // outputs of the parts of split sequences, float32
+};
+
+// Tokens and keys of a sequence, within the tensors whatever the offsets say.
+struct Sequence {
+    int q0, nq;                    // first token, tokens
+    int k0, nk;                    // first key (packed), keys
+    int bad;                       // paged: first position that the table has no page for
+};
+__device__ __forceinline__ int within(int v, int lo, int hi) { return min(max(v, lo), hi); }
+__device__ __forceinline__ Sequence sequence_at(const sapa_attention &a, int b) {
+    Sequence s;
+    s.q0 = within(a.offsets[b], 0, a.tokens);
+    s.nq = within(a.offsets[b + 1], s.q0, a.tokens) - s.q0;
+    s.k0 = 0;
+    s.bad = 0x7fffffff;
+    if (a.page_table != nullptr) {
+        s.nk = max(a.key_lengths[b], 0);
+        const long long room = (long long)a.max_pages * a.page;
+        if (s.nk > room) s.bad = (int)room;
+    } else {
+        s.k0 = within(a.key_offsets[b], 0, a.keys);
+        s.nk = within(a.key_offsets[b + 1], s.k0, a.keys) - s.k0;
+    }
+    return s;
+}
+// keys that token i of the sequence sees
+__device__ __forceinline__ int sees(const Sequence &s, int i, bool causal) {
+    return causal ? (int)min((long long)s.nk, max(0ll, (long long)s.nk - s.nq + i + 1)) : s.nk;
+}
+
+// A block's work: `rows` rows (tokens x query heads of one key head, the heads of a token next to each other) of a sequence.
+struct Item {
+    int b, block, part, parts;     // sequence, block of `tok` tokens in it, part of its keys
+    bool there;
+};
+__device__ __forceinline__ int warp_sum(int v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ int warp_scan(int v, int lane) {      // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// The blocks of all sequences in the order in which they are started, found by a whole warp; `count(b)` = blocks of sequence b.  Ordered by
+// their place from the sequence's end (FROM_END: a causal token's work grows with its place) or begin, so that what takes longest
+// is started first and short items fill the end.  The place is searched for by halving, each time adding up the sequences' counts.
+template <bool FROM_END, typename Count>
+__device__ __forceinline__ Item block_at(int index, int B, int lane, Count count) {
+    Item it{0, 0, 0, 1, false};
+    int most = 0;
+    long long total = 0;
+    for (int b = lane; b < B; b += 32) { const int n = count(b); most = max(most, n); total += n; }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    if (index >= total) return it;
+    // levels: FROM_END takes places most - 1 first; before(l) = blocks at the first l levels
+    int lo = 0, hi = most;                              // before(lo) <= index < before(hi)
+    long long below = 0;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        int sum = 0;
+        for (int b = lane; b < B; b += 32) { const int n = count(b); sum += FROM_END ? max(0, n - (most - mid)) : min(n, mid); }
+        sum = warp_sum(sum);
+        if (sum <= index) { lo = mid; below = sum; } else hi = mid;
+    }
+    const int place = FROM_END ? most - 1 - lo : lo;
+    int left = index - (int)below;                      // the left-th sequence with such a block
+    for (int b0 = 0; b0 < B; b0 += 32) {
+        const int b = b0 + lane;
+        const unsigned has = __ballot_sync(0xffffffffu, b < B && count(b) > place);
+        const int n = __popc(has);
+        if (left < n) {
+            unsigned m = has;
+            for (int i = 0; i < left; ++i) m &= m - 1;
+            it.b = b0 + __ffs(m) - 1;
+            it.block = place;
+            it.there = true;
+            return it;
+        }
+        left -= n;
+    }
+    return it;
+}
+
+// Where a block that is split finds its part: the keys of every sequence are cut into parts of `tiles` tiles of TILE keys, as many as make about
+// `split` items of all sequences together (their lengths are known on the device alone).  A sequence's blocks all have as many parts as its
+// whole length gives; of a causal block the last ones may see nothing and are empty.
+constexpr int TILE = 128;
+struct Plan {
+    Item it;
+    int tiles;                     // TILEs of a part
+    int first;                     // number of the block's first part among all
+};
+// The index-th item (PARTS) or block (!PARTS) of all sequences, by a whole warp.  tok: tokens of a block.
+template <bool PARTS>
+__device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int least, int lane) {
+    const sapa_attention &a = p.a;
+    Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
+    unsigned long long work = 0;
+    for (int b = lane; b < a.B; b += 32) {
+        const Sequence s = sequence_at(a, b);
+        work += (unsigned long long)((s.nq + tok - 1) / tok) * (unsigned)((min(s.nk, s.bad) + TILE - 1) / TILE);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+    r.tiles = (int)max((work * a.groups + p.split - 1) / (unsigned)p.split, (unsigned long long)least);
+    int before = 0, items = 0;     // blocks or items of the sequences before; their items
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int b = b0 + lane;
+        int blocks = 0, parts = 1;
+        if (b < a.B) {
+            const Sequence s = sequence_at(a, b);
+            blocks = (s.nq + tok - 1) / tok;
+            parts = max(1, ((min(s.nk, s.bad) + TILE - 1) / TILE + r.tiles - 1) / r.tiles);
+        }
+        const int mine = PARTS ? blocks * parts : blocks, upto = warp_scan(mine, lane), ends = warp_scan(blocks * parts, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, index < before + upto);
+        if (hit != 0u) {
+            const int from = __ffs(hit) - 1;
+            const int at = index - before - __shfl_sync(0xffffffffu, upto - mine, from);
+            r.it.parts = __shfl_sync(0xffffffffu, parts, from);
+            r.it.b = b0 + from;
+            r.it.block = PARTS ? at / r.it.parts : at;
+            r.it.part = PARTS ? at % r.it.parts : 0;
+            r.it.there = true;
+            r.first = items + __shfl_sync(0xffffffffu, ends - blocks * parts, from) + r.it.block * r.it.parts;
+            return r;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+        items += __shfl_sync(0xffffffffu, ends, 31);
+    }
+    return r;
+}
+// The work of block `index` (group apart) of a forward kernel, by a whole warp.
+__device__ __forceinline__ Plan plan_at(const Args &p, int index, int tok, int least, int lane) {
+    if (p.split > 0) return split_at<true>(p, index, tok, least, lane);
+    Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
+    r.it = block_at<true>(index, p.a.B, lane, [&](int b) { return (sequence_at(p.a, b).nq + tok - 1) / tok; });
+    return r;
+}
+
+// First element of the row at a position of a sequence's keys; nullptr where the table has no page for it.
+template <typename T>
+__device__ __forceinline__ const T *key_row(const sapa_attention &a, const Sequence &s, int b, int position, const void *base, const long long (&strides)[3]) {
+    if (a.page_table == nullptr) return static_cast<const T *>(base) + (long long)(s.k0 + position) * strides[0];
+    const int n = position / a.page;
+    if (n >= a.max_pages) return nullptr;
+    const int page = a.page_table[(long long)b * a.max_pages + n];
+    if ((unsigned)page >= (unsigned)a.pages) return nullptr;
+    return static_cast<const T *>(base) + (long long)page * strides[2] + (long long)(position % a.page) * strides[0];
+}
+
+// Rows of no sequence (before the first, behind the last) of a dense [rows, width] tensor: zeros, each block of the grid a share.
+template <typename T>
+__device__ __forceinline__ void clear_outside(T *x, const int *offsets, int B, int rows, int width, long long block, long long blocks, int tid, int threads) {
+    const int begin = B > 0 ? within(offsets[0], 0, rows) : 0, end = B > 0 ? within(offsets[B], begin, rows) : 0;
+    const long long n = (long long)(begin + rows - end) * width;
+    for (long long i = block * threads + tid; i < n; i += blocks * threads) {
+        const long long row = i / width;
+        x[(row < begin ? row : row - begin + end) * width + i % width] = from_acc<T>(0.f);
+    }
+}
+
+}  // namespace attn
+}  // namespace sapa

@@ -13,6 +13,7 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
 #include <string>
 
 #include "../../include/sapa_b200.h"
@@ -38,7 +39,9 @@ struct Api {
     SAPA_FN(sapa_deform_fused_backward_workspace) SAPA_FN(sapa_deform_fused_backward_scatter_bytes)                       \
     SAPA_FN(sapa_project_workspace) SAPA_FN(sapa_project_forward) SAPA_FN(sapa_project_list_workspace)                    \
     SAPA_FN(sapa_project_list_forward) SAPA_FN(sapa_projections_workspace) SAPA_FN(sapa_projections_forward)              \
-    SAPA_FN(sapa_projections_backward_workspace) SAPA_FN(sapa_projections_backward)
+    SAPA_FN(sapa_projections_backward_workspace) SAPA_FN(sapa_projections_backward)                                       \
+    SAPA_FN(sapa_attention_workspace) SAPA_FN(sapa_attention_forward) SAPA_FN(sapa_attention_backward_workspace)          \
+    SAPA_FN(sapa_attention_backward) SAPA_FN(sapa_paged_write)
     SAPA_FNS
 #undef SAPA_FN
 };
@@ -143,6 +146,7 @@ void check_window(int64_t K, int64_t s) {
 #include "host_sapa.inc"
 #include "host_deform.inc"
 #include "host_module.inc"
+#include "host_attention.inc"
 
 }  // namespace
 
@@ -168,4 +172,9 @@ PYBIND11_MODULE(_host, m) {
     m.def("project_module", native(&project_module));
     m.def("project", native(&project));
     m.def("project_workspace", native(&project_workspace));
+    m.def("packed_attention", native(&packed_attention));
+    m.def("packed_attention_forward", native(&packed_attention_forward));
+    m.def("packed_attention_backward", native(&packed_bwd));
+    m.def("paged_attention", native(&paged_attention));
+    m.def("paged_write", native(&paged_write));
 }
