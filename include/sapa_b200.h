@@ -63,7 +63,7 @@ int sapa_abi_version(void);
 /* The TMA kernels never spin without a limit: a wait on a shared-memory barrier that gives up (which only a
  * malfunction can cause) makes the kernel return early and sets a flag on the device.  This reads the flags of the
  * current device: 0 = no wait ever gave up, bit 0 = fused forward / backward stage 1, bit 1 = gradient gather,
- * bit 2 = projection GEMM,
+ * bit 2 = projection GEMM, bit 3 = attention over sequences,
  * -1 = the flags could not be read.  Reading a raised flag clears it and resets the tile schedulers of that kernel
  * family (a CTA that gave up leaves its scheduler counters dirty), so the library is usable again afterwards.
  * It synchronises the device; meant for tests and for diagnosing wrong results, not for the hot path.

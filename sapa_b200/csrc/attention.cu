@@ -15,7 +15,6 @@ namespace attn {
 namespace rows {
 
 constexpr int NT = 256, KT = 64;              // threads; keys of a tile
-constexpr int LEAST = 2;                      // TILEs of a part at least
 template <int RI, int DP> struct Lay {
     static constexpr int BM = 16 * RI, QS = DP + 4, PS = KT + 4;
     static constexpr int Q0 = 0, K0 = Q0 + BM * QS, V0 = K0 + KT * QS, P0 = V0 + KT * DP, END = P0 + BM * PS;
@@ -64,7 +63,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
     const int group = blockIdx.x % a.groups, tok = L::BM / p.share, D = a.dim;
     begin_after_previous();
     if (tid < 32) {
-        const Plan r = plan_at(p, blockIdx.x / a.groups, tok, LEAST, tid);
+        const Plan r = plan_at(p, blockIdx.x / a.groups, tok, tid);
         if (tid == 0) { plan = r; bad_page = 0x7fffffff; }
     }
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, tid, NT);
@@ -223,11 +222,11 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
 
 // Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(lse_p - max lse).  A block of the grid per block and group, a warp per row.
 template <typename T>
-__global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_constant__ Args p, int bm, int tok, int least) {
+__global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_constant__ Args p, int bm, int tok) {
     const sapa_attention &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x % a.groups, D = a.dim;
     begin_after_previous();
-    const Plan plan = split_at<false>(p, blockIdx.x / a.groups, tok, least, lane);
+    const Plan plan = split_at<false>(p, blockIdx.x / a.groups, tok, lane);
     if (!plan.it.there || plan.it.parts == 1) return;
     const Sequence s = sequence_at(a, plan.it.b);
     const int first = plan.it.block * tok, used = min(tok, s.nq - first) * p.share;
@@ -590,17 +589,24 @@ struct Shape {
 static Shape shape_of(const Args &p, int dtype, int sms) {
     const sapa_attention &a = p.a;
     Shape s{};
-    s.umma = false;
-    // single tokens and short chunks: 16 rows a block, as long as an average sequence has no more
-    s.narrow = p.share <= 16 && (long long)a.tokens * p.share <= 16ll * a.B;
-    s.bm = s.narrow ? 16 : 128;
-    s.tok = s.bm / p.share;
+    s.umma = umma_takes(a, dtype);
+    if (s.umma) {
+        // short sequences: a row tile a block, as long as an average sequence has no more rows
+        s.narrow = (long long)a.tokens * p.share <= 128ll * a.B;
+        s.tok = 128 / p.share * (s.narrow ? 1 : 2);
+        s.bm = s.tok * p.share;
+    } else {
+        // single tokens and short chunks: 16 rows a block, as long as an average sequence has no more
+        s.narrow = p.share <= 16 && (long long)a.tokens * p.share <= 16ll * a.B;
+        s.bm = s.narrow ? 16 : 128;
+        s.tok = s.bm / p.share;
+    }
     s.blocks = most_blocks(a, a.tokens, s.tok) * a.groups;
     s.grid = s.blocks;
     // few blocks: their keys are split so that every SM has items
     const long long keys = a.page_table != nullptr ? (long long)a.max_pages * a.page : a.keys;
-    if (s.blocks < 4ll * sms && keys > TILE) {
-        s.split = 4 * sms;
+    if (s.blocks < 4ll * sms && keys > 2 * TILE) {
+        s.split = (s.umma ? 3 : 4) * sms;
         s.grid = s.blocks + s.split;
         s.part = (size_t)s.grid * s.bm * a.dim * sizeof(float);
         s.lse = (size_t)s.grid * s.bm * sizeof(float);
@@ -656,15 +662,17 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
         SAPA_REQUIRE(workspace != nullptr && workspace_bytes >= s.bytes, SAPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, s.bytes, workspace_bytes);
         SAPA_REQUIRE(aligned16(workspace), SAPA_ERR_ALIGNMENT, "%s: the workspace must be 256-byte aligned", fn);
         p.split = s.split;
+        p.least = 2;
         p.part = static_cast<float *>(workspace);
         p.part_lse = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.part);
     }
     return SAPA_DISPATCH_FAST(dtype, [&]() -> int {
         int e;
-        if (s.narrow) e = a->dim <= 64 ? run_rows<scalar_t, 1, 64>(p, s, st) : run_rows<scalar_t, 1, 128>(p, s, st);
+        if (s.umma) e = umma_forward(p, !s.narrow, s.grid, dtype, st);
+        else if (s.narrow) e = a->dim <= 64 ? run_rows<scalar_t, 1, 64>(p, s, st) : run_rows<scalar_t, 1, 128>(p, s, st);
         else e = a->dim <= 64 ? run_rows<scalar_t, 8, 64>(p, s, st) : run_rows<scalar_t, 8, 128>(p, s, st);
         if (e != SAPA_OK || s.split == 0) return e;
-        launch_next(sapa_attention_join_kernel<scalar_t>, dim3((unsigned)s.blocks), dim3(256), 0, st, p, s.bm, s.tok, rows::LEAST);
+        launch_next(sapa_attention_join_kernel<scalar_t>, dim3((unsigned)s.blocks), dim3(256), 0, st, p, s.bm, s.tok);
         return check_launch("sapa_attention_join_kernel");
     });
 }

@@ -11,7 +11,7 @@ struct Args {
     sapa_attention a;
     float scale_log2;              // scale * log2(e): the softmax runs in base 2
     int share;                     // query heads of a key head
-    int split;                     // > 0: items that a sequence's keys are spread over, see Plan
+    int split, least;              // > 0: items that the keys of all sequences are spread over, and tiles of an item at least, see Plan
     float *part, *part_lse;        // outputs of the parts of split sequences, float32
 };
 
@@ -106,8 +106,8 @@ __device__ __forceinline__ Item block_at(int index, int B, int lane, Count count
     return it;
 }
 
-// Where a block that is split finds its part: the keys of every sequence are cut into parts of `tiles` tiles of TILE keys, as many as make about
-// `split` items of all sequences together (their lengths are known on the device alone).  A sequence's blocks all have as many parts as its
+// Where a block that is split finds its part: the keys of every sequence are cut into parts of even lengths, tiles of TILE keys,
+// so many that all sequences together make about `split` items (their lengths are known on the device alone).  A sequence's blocks all have as many parts as its
 // whole length gives; of a causal block the last ones may see nothing and are empty.
 constexpr int TILE = 128;
 struct Plan {
@@ -117,7 +117,7 @@ struct Plan {
 };
 // The index-th item (PARTS) or block (!PARTS) of all sequences, by a whole warp.  tok: tokens of a block.
 template <bool PARTS>
-__device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int least, int lane) {
+__device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int lane) {
     const sapa_attention &a = p.a;
     Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
     unsigned long long work = 0;
@@ -127,15 +127,17 @@ __device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int 
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-    r.tiles = (int)max((work * a.groups + p.split - 1) / (unsigned)p.split, (unsigned long long)least);
+    const int most = (int)max((work * a.groups + p.split - 1) / (unsigned)p.split, (unsigned long long)p.least);      // tiles of a part
     int before = 0, items = 0;     // blocks or items of the sequences before; their items
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         const int b = b0 + lane;
-        int blocks = 0, parts = 1;
+        int blocks = 0, parts = 1, tiles = 0;
         if (b < a.B) {
             const Sequence s = sequence_at(a, b);
             blocks = (s.nq + tok - 1) / tok;
-            parts = max(1, ((min(s.nk, s.bad) + TILE - 1) / TILE + r.tiles - 1) / r.tiles);
+            tiles = (min(s.nk, s.bad) + TILE - 1) / TILE;
+            parts = max(1, (tiles + most - 1) / most);
+            tiles = (tiles + parts - 1) / parts;
         }
         const int mine = PARTS ? blocks * parts : blocks, upto = warp_scan(mine, lane), ends = warp_scan(blocks * parts, lane);
         const unsigned hit = __ballot_sync(0xffffffffu, index < before + upto);
@@ -143,6 +145,7 @@ __device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int 
             const int from = __ffs(hit) - 1;
             const int at = index - before - __shfl_sync(0xffffffffu, upto - mine, from);
             r.it.parts = __shfl_sync(0xffffffffu, parts, from);
+            r.tiles = __shfl_sync(0xffffffffu, tiles, from);
             r.it.b = b0 + from;
             r.it.block = PARTS ? at / r.it.parts : at;
             r.it.part = PARTS ? at % r.it.parts : 0;
@@ -156,12 +159,16 @@ __device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int 
     return r;
 }
 // The work of block `index` (group apart) of a forward kernel, by a whole warp.
-__device__ __forceinline__ Plan plan_at(const Args &p, int index, int tok, int least, int lane) {
-    if (p.split > 0) return split_at<true>(p, index, tok, least, lane);
+__device__ __forceinline__ Plan plan_at(const Args &p, int index, int tok, int lane) {
+    if (p.split > 0) return split_at<true>(p, index, tok, lane);
     Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
     r.it = block_at<true>(index, p.a.B, lane, [&](int b) { return (sequence_at(p.a, b).nq + tok - 1) / tok; });
     return r;
 }
+
+// Tensor-core forward (attention_umma.cu): what it takes, and its launch; wide: two row tiles a block.
+bool umma_takes(const sapa_attention &a, int dtype);
+int umma_forward(const Args &p, bool wide, long long grid, int dtype, cudaStream_t st);
 
 // First element of the row at a position of a sequence's keys; nullptr where the table has no page for it.
 template <typename T>

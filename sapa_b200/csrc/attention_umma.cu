@@ -1,0 +1,99 @@
+// attention_umma.cu — launches of the tensor-core kernels of attention over sequences.
+#include "attention.cuh"
+#include "tma_util.cuh"
+
+namespace sapa {
+namespace attn {
+
+__device__ int g_wait_timeout = 0;
+
+}  // namespace attn
+}  // namespace sapa
+
+#include "attention_umma.cuh"
+
+namespace sapa {
+namespace attn {
+
+namespace um {
+
+// rows of 64 channels: dims and strides (in elements) of the axes behind the channels
+static bool encode(CUtensorMap *map, const void *base, int dim, int rank, const long long *dims, const long long *strides, const int *boxes, bool half) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return false;
+    cuuint64_t d[4] = {(cuuint64_t)dim}, st[3];
+    cuuint32_t box[4] = {64u}, one[4] = {1u, 1u, 1u, 1u};
+    for (int i = 0; i < rank; ++i) {
+        d[i + 1] = (cuuint64_t)dims[i];
+        st[i] = (cuuint64_t)strides[i] * 2;
+        box[i + 1] = (cuuint32_t)boxes[i];
+    }
+    const CUtensorMapDataType type = half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    auto call = [&]() {
+        return fn(map, type, (cuuint32_t)rank + 1, const_cast<void *>(base), d, st, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = call();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {                            // a thread without a context: the runtime's no-op binds the device's
+        cudaFree(nullptr);
+        r = call();
+    }
+    last_encode_result() = (int)r;
+    return r == CUDA_SUCCESS;
+}
+
+template <typename T, int D, bool WIDE, bool PAGED>
+static int launch(const Args &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, long long grid, cudaStream_t st) {
+    using L = um::Lay<D, WIDE>;
+    int sms = 0;
+    if (int e = prepare_launch((const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED>, L::SMEM, "sapa_attention_umma_kernel", sms)) return e;
+    launch_next(sapa_attention_umma_kernel<T, D, WIDE, PAGED>, dim3((unsigned)grid), dim3(NT), L::SMEM, st, q, k, v, p);
+    return check_launch(WIDE ? "sapa_attention_umma_kernel<wide>" : "sapa_attention_umma_kernel<narrow>");
+}
+
+}  // namespace um
+
+bool umma_takes(const sapa_attention &a, int dtype) {
+    if (dtype == SAPA_F32) return false;
+    if (a.page_table == nullptr) return a.keys > 0;
+    return a.page >= 8 && (a.page & (a.page - 1)) == 0;               // pages that a tile of 128 keys holds whole, or that hold it
+}
+
+int umma_forward(const Args &p, bool wide, long long grid, int dtype, cudaStream_t st) {
+    using namespace um;
+    const sapa_attention &a = p.a;
+    const bool half = dtype == SAPA_F16, paged = a.page_table != nullptr;
+    CUtensorMap q, k, v;
+    const int tok = ROWS / p.share;
+    const long long qd[2] = {a.heads, a.tokens}, qs[2] = {a.query_strides[1], a.query_strides[0]};
+    const int qb[2] = {p.share, tok};
+    bool good = encode(&q, a.query, a.dim, 2, qd, qs, qb, half);
+    const int rows = a.page < KT ? a.page : KT;
+    const long long kd[3] = {a.groups, paged ? a.page : a.keys, a.pages}, ks[3] = {a.key_strides[1], a.key_strides[0], a.key_strides[2]},
+                    vs[3] = {a.value_strides[1], a.value_strides[0], a.value_strides[2]};
+    const int kb[3] = {1, paged ? rows : KT, 1};
+    good = good && encode(&k, a.key, a.dim, paged ? 3 : 2, kd, ks, kb, half) && encode(&v, a.value, a.dim, paged ? 3 : 2, kd, vs, kb, half);
+    SAPA_REQUIRE(good, SAPA_ERR_LAUNCH, "sapa_attention_forward: cuTensorMapEncodeTiled failed (%d)", last_encode_result());
+    auto pick = [&](auto t) -> int {
+        using T = decltype(t);
+        if (a.dim <= 64) {
+            if (wide) return paged ? launch<T, 64, true, true>(p, q, k, v, grid, st) : launch<T, 64, true, false>(p, q, k, v, grid, st);
+            return paged ? launch<T, 64, false, true>(p, q, k, v, grid, st) : launch<T, 64, false, false>(p, q, k, v, grid, st);
+        }
+        if (wide) return paged ? launch<T, 128, true, true>(p, q, k, v, grid, st) : launch<T, 128, true, false>(p, q, k, v, grid, st);
+        return paged ? launch<T, 128, false, true>(p, q, k, v, grid, st) : launch<T, 128, false, false>(p, q, k, v, grid, st);
+    };
+    return half ? pick(__half()) : pick(__nv_bfloat16());
+}
+
+// Flag of this family's bounded waits on the current device, cleared when it was raised; -1: it cannot be read.
+int wait_timeout_flag() {
+    int flag = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(&flag, g_wait_timeout, sizeof(int)) != cudaSuccess) return -1;
+    if (flag != 0 && cudaMemcpyToSymbol(g_wait_timeout, &zero, sizeof(int)) != cudaSuccess) return -1;
+    return flag;
+}
+
+}  // namespace attn
+}  // namespace sapa

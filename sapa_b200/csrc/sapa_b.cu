@@ -555,6 +555,7 @@ int launch_fused_tma_slots(int mode, const void *q, const void *k, const void *v
 
 int tma_wait_timeout_flag();
 int proj_wait_timeout_flag();
+namespace attn { int wait_timeout_flag(); }      // attention_umma.cu
 int launch_wait_selftest(cudaStream_t st);
 int gath_wait_timeout_flag();
 // tensor-core transposed aggregation (sapa_gath_mma.cu)
@@ -728,9 +729,9 @@ using namespace sapa;
 extern "C" {
 
 int sapa_wait_timeout_flags(void) {
-    const int a = tma_wait_timeout_flag(), b = gath_wait_timeout_flag(), c = proj_wait_timeout_flag();
-    if (a < 0 || b < 0 || c < 0) return -1;
-    return (a ? 1 : 0) | (b ? 2 : 0) | (c ? 4 : 0);
+    const int a = tma_wait_timeout_flag(), b = gath_wait_timeout_flag(), c = proj_wait_timeout_flag(), d = attn::wait_timeout_flag();
+    if (a < 0 || b < 0 || c < 0 || d < 0) return -1;
+    return (a ? 1 : 0) | (b ? 2 : 0) | (c ? 4 : 0) | (d ? 8 : 0);
 }
 
 int sapa_selftest_wait_timeout(void *stream) {

@@ -416,3 +416,8 @@ def test_transforms_and_refusals():
         sapa_b200.paged_attention(q.detach(), c.key.transpose(2, 3).contiguous().transpose(2, 3), c.value, c.table, c.lengths, off)
     with pytest.raises(RuntimeError, match="the cache holds"):
         sapa_b200.paged_attention(q.detach().half(), c.key, c.value, c.table, c.lengths, off)
+
+
+def test_no_wait_gave_up():
+    from sapa_b200 import _lib
+    assert _lib.wait_timeout_flags("cuda") == 0
