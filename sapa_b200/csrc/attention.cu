@@ -260,30 +260,36 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------------------------- backward
-struct Grads {
-    const void *go;
-    long long go_strides[2];
-    void *gq, *gk, *gv;
-    float *delta;                  // [tokens, heads]: sum over channels of grad_out * out
-};
-
-// delta, and what lies outside the sequences: a warp per token and head.
+// delta, and what lies outside the sequences: 16 lanes per token and head, 8 channels each.  Reads grad_out and out once, which bounds it.
 template <typename T>
 __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     const sapa_attention &a = p.a;
-    const int lane = threadIdx.x & 31, D = a.dim;
+    const int lane = threadIdx.x & 15, c = 8 * lane, D = a.dim;
     begin_after_previous();
-    const long long n = (long long)a.tokens * a.heads, all = (long long)gridDim.x * 8;
-    for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < n; row += all) {
+    const long long n = (long long)a.tokens * a.heads, all = (long long)gridDim.x * 16;
+    for (long long row0 = (long long)blockIdx.x * 16; row0 < n; row0 += all) {
+        const long long row = row0 + (threadIdx.x >> 4);
+        const long long t = row / a.heads;
+        const int h = (int)(row % a.heads);
         float sum = 0.f;
-        if (4 * lane < D) {
-            const float4 x = rows::load4(static_cast<const T *>(a.out) + row * D + 4 * lane);
-            const float4 y = rows::load4(static_cast<const T *>(g.go) + row / a.heads * g.go_strides[0] + row % a.heads * g.go_strides[1] + 4 * lane);
-            sum = x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+        if (row < n && c < D) {
+            const T *o = static_cast<const T *>(a.out) + row * D + c, *y = static_cast<const T *>(g.go) + t * g.go_strides[0] + h * g.go_strides[1] + c;
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 u = rows::load4(o + e), v = rows::load4(y + e);
+                sum = fmaf(u.w, v.w, fmaf(u.z, v.z, fmaf(u.y, v.y, fmaf(u.x, v.x, sum))));
+            }
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) g.delta[row] = sum;
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane != 0 || row >= n) continue;
+        if (g.nlse != nullptr) {
+            const long long at = ((long long)(h / p.share) * a.tokens + t) * p.share + h % p.share;
+            g.delta[at] = sum;
+            g.nlse[at] = -1.4426950408889634f * a.lse[row];
+        } else {
+            g.delta[row] = sum;
+        }
     }
     clear_outside(static_cast<T *>(g.gq), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
     clear_outside(static_cast<T *>(g.gk), a.key_offsets, a.B, a.keys, a.groups * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
@@ -300,11 +306,12 @@ template <int DP> struct Lay {
 };
 }  // namespace grad
 
-// KEYS: gradients of 64 keys and values, over the rows that see them; otherwise those of 64 query rows, over the keys that they see.  P and dS of
+// float32.  KEYS: gradients of 64 keys and values, over the rows that see them; otherwise those of 64 query rows, over the keys that they see.  P and dS of
 // a tile are formed again from the scores, lse and delta: P = 2^(s - lse), dS = P (dP - delta); no atomics.
-template <typename T, int DP, bool KEYS>
+template <int DP, bool KEYS>
 __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     using namespace grad;
+    using T = float;
     using L = grad::Lay<DP>;
     extern __shared__ __align__(16) float sm[];
     __shared__ Item item;
@@ -573,12 +580,6 @@ static Args args_of(const sapa_attention *a) {
     return p;
 }
 
-// Blocks of `tok` tokens that all sequences together can have.
-static long long most_blocks(const sapa_attention &a, long long total, int tok) {
-    const long long n = total / tok + a.B;
-    return n < total ? n : total;
-}
-
 // A forward of this call: rows of a block, whether its keys are split, and the room that takes.
 struct Shape {
     bool umma, narrow;
@@ -625,12 +626,12 @@ template <typename T, int RI, int DP> static int run_rows(const Args &p, const S
     return check_launch("sapa_attention_rows_kernel");
 }
 
-template <typename T, int DP, bool KEYS> static int run_grad(const Args &p, const Grads &g, long long blocks, cudaStream_t st) {
+template <int DP, bool KEYS> static int run_grad(const Args &p, const Grads &g, long long blocks, cudaStream_t st) {
     using L = grad::Lay<DP>;
     int sms = 0;
     if (blocks == 0) return SAPA_OK;
-    if (int e = tmau::prepare_launch((const void *)sapa_attention_rows_grad_kernel<T, DP, KEYS>, (int)L::SMEM, "sapa_attention_rows_grad_kernel", sms)) return e;
-    launch_next(sapa_attention_rows_grad_kernel<T, DP, KEYS>, dim3((unsigned)blocks), dim3(rows::NT), L::SMEM, st, p, g);
+    if (int e = tmau::prepare_launch((const void *)sapa_attention_rows_grad_kernel<DP, KEYS>, (int)L::SMEM, "sapa_attention_rows_grad_kernel", sms)) return e;
+    launch_next(sapa_attention_rows_grad_kernel<DP, KEYS>, dim3((unsigned)blocks), dim3(rows::NT), L::SMEM, st, p, g);
     return check_launch(KEYS ? "sapa_attention_rows_grad_kernel<keys>" : "sapa_attention_rows_grad_kernel<queries>");
 }
 
@@ -679,7 +680,8 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
 
 extern "C" size_t sapa_attention_backward_workspace(const sapa_attention *a, int dtype) {
     if (check(a, dtype, "sapa_attention_backward_workspace") != SAPA_OK) return 0;
-    return ((size_t)a->tokens * a->heads * sizeof(float) + 255) / 256 * 256;
+    // delta, and in 16 bits lse in another order
+    return ((size_t)a->tokens * a->heads * sizeof(float) + 255) / 256 * 256 * (dtype == SAPA_F32 ? 1 : 2);
 }
 
 extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad_out, long long grad_token_stride, long long grad_head_stride,
@@ -700,22 +702,31 @@ extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad
     SAPA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), SAPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need, workspace_bytes);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const Args p = args_of(a);
-    Grads g{grad_out, {grad_token_stride, grad_head_stride}, grad_query, grad_key, grad_value, static_cast<float *>(workspace)};
+    if (a->tokens == 0 || a->keys == 0) {            // nothing is seen: every gradient is zero
+        const size_t row = (size_t)a->dim * dtype_size(dtype), queries = (size_t)a->tokens * a->heads * row, keys = (size_t)a->keys * a->groups * row;
+        if (queries != 0) cudaMemsetAsync(grad_query, 0, queries, st);
+        if (keys != 0) { cudaMemsetAsync(grad_key, 0, keys, st); cudaMemsetAsync(grad_value, 0, keys, st); }
+        return check_launch("memset");
+    }
+    const bool umma = dtype != SAPA_F32;
+    Grads g{grad_out, {grad_token_stride, grad_head_stride}, grad_query, grad_key, grad_value, static_cast<float *>(workspace),
+            umma ? reinterpret_cast<float *>(static_cast<char *>(workspace) + need / 2) : nullptr};
     int sms = 0;
     if (int e = sm_count(fn, sms)) return e;
-    const long long rows8 = ((long long)a->tokens * a->heads + 7) / 8, delta_grid = rows8 < 16ll * sms ? (rows8 > 0 ? rows8 : 1) : 16ll * sms;
+    const long long rows16 = ((long long)a->tokens * a->heads + 15) / 16, delta_grid = rows16 < 16ll * sms ? (rows16 > 0 ? rows16 : 1) : 16ll * sms;
     const int slots = (p.share + grad::N - 1) / grad::N, tok = grad::N / (p.share < grad::N ? p.share : grad::N);
     const long long key_blocks = most_blocks(*a, a->keys, grad::N) * a->groups, query_blocks = most_blocks(*a, a->tokens, tok) * a->groups * slots;
     SAPA_REQUIRE(key_blocks < 0x7fffffffll && query_blocks < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
     return SAPA_DISPATCH_FAST(dtype, [&]() -> int {
         launch_next(sapa_attention_delta_kernel<scalar_t>, dim3((unsigned)delta_grid), dim3(256), 0, st, p, g);
         if (int e = check_launch("sapa_attention_delta_kernel")) return e;
+        if (umma) return umma_backward(p, g, dtype, st);
         if (a->dim <= 64) {
-            if (int e = run_grad<scalar_t, 64, true>(p, g, key_blocks, st)) return e;
-            return run_grad<scalar_t, 64, false>(p, g, query_blocks, st);
+            if (int e = run_grad<64, true>(p, g, key_blocks, st)) return e;
+            return run_grad<64, false>(p, g, query_blocks, st);
         }
-        if (int e = run_grad<scalar_t, 128, true>(p, g, key_blocks, st)) return e;
-        return run_grad<scalar_t, 128, false>(p, g, query_blocks, st);
+        if (int e = run_grad<128, true>(p, g, key_blocks, st)) return e;
+        return run_grad<128, false>(p, g, query_blocks, st);
     });
 }
 

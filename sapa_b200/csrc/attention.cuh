@@ -166,9 +166,24 @@ __device__ __forceinline__ Plan plan_at(const Args &p, int index, int tok, int l
     return r;
 }
 
+// Of a backward pass
+struct Grads {
+    const void *go;                // grad_out
+    long long go_strides[2];
+    void *gq, *gk, *gv;
+    float *delta;                  // sum over channels of grad_out * out: [tokens, heads], or like nlse where that is there
+    float *nlse;                   // -log2(e) lse as the tensor-core kernels read it: [groups, tokens, heads of a group]; or NULL
+};
+
 // Tensor-core forward (attention_umma.cu): what it takes, and its launch; wide: two row tiles a block.
 bool umma_takes(const sapa_attention &a, int dtype);
 int umma_forward(const Args &p, bool wide, long long grid, int dtype, cudaStream_t st);
+int umma_backward(const Args &p, const Grads &g, int dtype, cudaStream_t st);
+// Blocks of `tok` tokens that all sequences together can have.
+inline long long most_blocks(const sapa_attention &a, long long total, int tok) {
+    const long long n = total / tok + a.B;
+    return n < total ? n : total;
+}
 
 // First element of the row at a position of a sequence's keys; nullptr where the table has no page for it.
 template <typename T>

@@ -11,6 +11,7 @@ __device__ int g_wait_timeout = 0;
 }  // namespace sapa
 
 #include "attention_umma.cuh"
+#include "attention_umma_grad.cuh"
 
 namespace sapa {
 namespace attn {
@@ -84,6 +85,42 @@ int umma_forward(const Args &p, bool wide, long long grid, int dtype, cudaStream
         return paged ? launch<T, 128, false, true>(p, q, k, v, grid, st) : launch<T, 128, false, false>(p, q, k, v, grid, st);
     };
     return half ? pick(__half()) : pick(__nv_bfloat16());
+}
+
+namespace umg {
+
+template <typename T, int D>
+static int launch(const Args &p, const Grads &g, const CUtensorMap &q, const CUtensorMap &o, const CUtensorMap &k, const CUtensorMap &v, long long key_blocks,
+                  long long query_blocks, cudaStream_t st) {
+    int sms = 0;
+    constexpr int KEYS = KeyLay<D>::SMEM, QUERIES = QueryLay<D>::SMEM;
+    if (int e = prepare_launch((const void *)sapa_attention_umma_keys_kernel<T, D>, KEYS, "sapa_attention_umma_keys_kernel", sms)) return e;
+    if (int e = prepare_launch((const void *)sapa_attention_umma_queries_kernel<T, D>, QUERIES, "sapa_attention_umma_queries_kernel", sms)) return e;
+    launch_next(sapa_attention_umma_keys_kernel<T, D>, dim3((unsigned)key_blocks), dim3(NT), KEYS, st, q, o, k, v, p, g);
+    if (int e = check_launch("sapa_attention_umma_keys_kernel")) return e;
+    launch_next(sapa_attention_umma_queries_kernel<T, D>, dim3((unsigned)query_blocks), dim3(NT), QUERIES, st, q, o, k, v, p, g);
+    return check_launch("sapa_attention_umma_queries_kernel");
+}
+
+}  // namespace umg
+
+int umma_backward(const Args &p, const Grads &g, int dtype, cudaStream_t st) {
+    using namespace um;
+    const sapa_attention &a = p.a;
+    const bool half = dtype == SAPA_F16;
+    CUtensorMap q, o, k, v;
+    const int tok = ROWS / p.share, qb[2] = {p.share, tok}, kb[2] = {1, KT};
+    const long long qd[2] = {a.heads, a.tokens}, qs[2] = {a.query_strides[1], a.query_strides[0]}, os[2] = {g.go_strides[1], g.go_strides[0]};
+    const long long kd[2] = {a.groups, a.keys}, ks[2] = {a.key_strides[1], a.key_strides[0]}, vs[2] = {a.value_strides[1], a.value_strides[0]};
+    const bool good = encode(&q, a.query, a.dim, 2, qd, qs, qb, half) && encode(&o, g.go, a.dim, 2, qd, os, qb, half) &&
+                      encode(&k, a.key, a.dim, 2, kd, ks, kb, half) && encode(&v, a.value, a.dim, 2, kd, vs, kb, half);
+    SAPA_REQUIRE(good, SAPA_ERR_LAUNCH, "sapa_attention_backward: cuTensorMapEncodeTiled failed (%d)", last_encode_result());
+    const long long key_blocks = most_blocks(a, a.keys, KT) * a.groups, query_blocks = most_blocks(a, a.tokens, tok) * a.groups;
+    SAPA_REQUIRE(key_blocks < 0x7fffffffll && query_blocks < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "sapa_attention_backward: too many blocks");
+    if (key_blocks == 0 || query_blocks == 0) return SAPA_OK;         // no sequence
+    if (half) return a.dim <= 64 ? umg::launch<__half, 64>(p, g, q, o, k, v, key_blocks, query_blocks, st) : umg::launch<__half, 128>(p, g, q, o, k, v, key_blocks, query_blocks, st);
+    return a.dim <= 64 ? umg::launch<__nv_bfloat16, 64>(p, g, q, o, k, v, key_blocks, query_blocks, st)
+                       : umg::launch<__nv_bfloat16, 128>(p, g, q, o, k, v, key_blocks, query_blocks, st);
 }
 
 // Flag of this family's bounded waits on the current device, cleared when it was raised; -1: it cannot be read.
