@@ -323,8 +323,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(cons
     const int slot = blockIdx.x % slots, group = KEYS ? slot : slot % a.groups;
     begin_after_previous();
     if (tid < 32) {
-        const Item r = KEYS ? block_at<false>(blockIdx.x / slots, a.B, tid, [&](int b) { return (sequence_at(a, b).nk + N - 1) / N; })
-                            : block_at<true>(blockIdx.x / slots, a.B, tid, [&](int b) { return (sequence_at(a, b).nq + tok - 1) / tok; });
+        const Item r = KEYS ? block_at<false>(a, blockIdx.x / slots, tid, KeyBlocks{a.causal != 0, tok, N}) : block_at<true>(a, blockIdx.x / slots, tid, QueryBlocks{a.causal != 0, tok, N});
         if (tid == 0) item = r;
     }
     __syncthreads();
@@ -606,7 +605,7 @@ static Shape shape_of(const Args &p, int dtype, int sms) {
     s.grid = s.blocks;
     // few blocks: their keys are split so that every SM has items
     const long long keys = a.page_table != nullptr ? (long long)a.max_pages * a.page : a.keys;
-    if (s.blocks < 4ll * sms && keys > 2 * TILE) {
+    if (s.blocks < 2ll * sms && keys > 2 * TILE) {
         s.split = (s.umma ? 3 : 4) * sms;
         s.grid = s.blocks + s.split;
         s.part = (size_t)s.grid * s.bm * a.dim * sizeof(float);

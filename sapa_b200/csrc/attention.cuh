@@ -62,48 +62,74 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {      // inclusive
     return v;
 }
 
-// The blocks of all sequences in the order in which they are started, found by a whole warp; `count(b)` = blocks of sequence b.  Ordered by
-// their place from the sequence's end (FROM_END: a causal token's work grows with its place) or begin, so that what takes longest
-// is started first and short items fill the end.  The place is searched for by halving, each time adding up the sequences' counts.
-template <bool FROM_END, typename Count>
-__device__ __forceinline__ Item block_at(int index, int B, int lane, Count count) {
+// The blocks of all sequences in the order in which they are started, found by a whole warp: those with the most work first, so that short ones
+// fill the end.  `at_least(s, w)`: blocks of a sequence with at least w units of work, all for w = 0; `units(s)`: the most that one of its blocks has.
+// LAST: a sequence's blocks have the more work the later they come (a causal token sees the more keys), otherwise the less.  The amount of work is
+// searched for by halving, each time adding up the sequences' counts; each lane keeps the first of its sequences in registers.
+template <bool LAST, typename Units, typename Count>
+__device__ __forceinline__ Item block_at(const sapa_attention &a, int index, int lane, Units units, Count at_least) {
     Item it{0, 0, 0, 1, false};
-    int most = 0;
-    long long total = 0;
-    for (int b = lane; b < B; b += 32) { const int n = count(b); most = max(most, n); total += n; }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-    }
-    if (index >= total) return it;
-    // levels: FROM_END takes places most - 1 first; before(l) = blocks at the first l levels
-    int lo = 0, hi = most;                              // before(lo) <= index < before(hi)
-    long long below = 0;
+    Sequence mine{0, 0, 0, 0, 0};
+    if (lane < a.B) mine = sequence_at(a, lane);
+    auto all = [&](int w) {
+        int n = at_least(mine, w);
+        for (int b = lane + 32; b < a.B; b += 32) n += at_least(sequence_at(a, b), w);
+        return warp_sum(n);
+    };
+    if (index >= all(0)) return it;
+    int most = units(mine);
+    for (int b = lane + 32; b < a.B; b += 32) most = max(most, units(sequence_at(a, b)));
+    int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) + 1, behind = 0;      // all(lo) > index >= all(hi) = behind
     while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        int sum = 0;
-        for (int b = lane; b < B; b += 32) { const int n = count(b); sum += FROM_END ? max(0, n - (most - mid)) : min(n, mid); }
-        sum = warp_sum(sum);
-        if (sum <= index) { lo = mid; below = sum; } else hi = mid;
+        const int mid = lo + (hi - lo) / 2, n = all(mid);
+        if (n > index) lo = mid; else { hi = mid; behind = n; }
     }
-    const int place = FROM_END ? most - 1 - lo : lo;
-    int left = index - (int)below;                      // the left-th sequence with such a block
-    for (int b0 = 0; b0 < B; b0 += 32) {
+    int left = index - behind;                          // among the blocks with just lo units
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
         const int b = b0 + lane;
-        const unsigned has = __ballot_sync(0xffffffffu, b < B && count(b) > place);
-        const int n = __popc(has);
-        if (left < n) {
-            unsigned m = has;
-            for (int i = 0; i < left; ++i) m &= m - 1;
-            it.b = b0 + __ffs(m) - 1;
-            it.block = place;
+        if (b0 > 0) mine = b < a.B ? sequence_at(a, b) : Sequence{0, 0, 0, 0, 0};
+        const int more = at_least(mine, hi), here = at_least(mine, lo) - more, upto = warp_scan(here, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, left < upto);
+        if (hit != 0u) {
+            const int from = __ffs(hit) - 1, before = more + left - (upto - here);      // blocks of the sequence with no less work in front of it
+            it.b = b0 + from;
+            it.block = __shfl_sync(0xffffffffu, LAST ? at_least(mine, 0) - 1 - before : before, from);
             it.there = true;
             return it;
         }
-        left -= n;
+        left -= __shfl_sync(0xffffffffu, upto, 31);
     }
     return it;
+}
+__device__ __forceinline__ int tiles_of(int n, int tile) { return (int)(((unsigned)n + (unsigned)tile - 1) / (unsigned)tile); }
+// Blocks of `tok` tokens, by the tiles of `tile` keys that they go over (what a block's last token sees)
+struct QueryBlocks {
+    bool causal;
+    int tok, tile;
+    __device__ __forceinline__ int units(const Sequence &s) const { return tiles_of(min(s.nk, s.bad), tile); }
+    __device__ __forceinline__ int at_least(const Sequence &s, int w) const {
+        const int n = tiles_of(s.nq, tok), seen = (w - 1) * tile;                     // one key more is needed
+        if (w == 0) return n;
+        if (min(s.nk, s.bad) <= seen) return 0;
+        const int token = seen - s.nk + s.nq;                                         // the first that sees so many
+        return !causal || token <= 0 ? n : token >= s.nq ? 0 : n - (int)((unsigned)token / (unsigned)tok);
+    }
+};
+// Blocks of `tile` keys, by the tiles of `tok` tokens that see them
+struct KeyBlocks {
+    bool causal;
+    int tok, tile;
+    __device__ __forceinline__ int units(const Sequence &s) const { return tiles_of(s.nq, tok); }
+    __device__ __forceinline__ int at_least(const Sequence &s, int w) const {
+        const int n = tiles_of(s.nk, tile), last = s.nq - (w - 1) * tok - 1;          // the last token that a block may begin with
+        if (w == 0) return n;
+        if (last < 0) return 0;
+        const int key = last + s.nk - s.nq;                                           // the last key that it sees
+        return !causal ? n : key < 0 ? 0 : min(n, (int)((unsigned)key / (unsigned)tile) + 1);
+    }
+};
+template <bool LAST, typename Blocks> __device__ __forceinline__ Item block_at(const sapa_attention &a, int index, int lane, const Blocks &k) {
+    return block_at<LAST>(a, index, lane, [&](const Sequence &s) { return k.units(s); }, [&](const Sequence &s, int w) { return k.at_least(s, w); });
 }
 
 // Where a block that is split finds its part: the keys of every sequence are cut into parts of even lengths, tiles of TILE keys,
@@ -162,7 +188,7 @@ __device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int 
 __device__ __forceinline__ Plan plan_at(const Args &p, int index, int tok, int lane) {
     if (p.split > 0) return split_at<true>(p, index, tok, lane);
     Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
-    r.it = block_at<true>(index, p.a.B, lane, [&](int b) { return (sequence_at(p.a, b).nq + tok - 1) / tok; });
+    r.it = block_at<true>(p.a, index, lane, QueryBlocks{p.a.causal != 0, tok, TILE});
     return r;
 }
 

@@ -314,6 +314,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
             const bool mine = r < tile_tok * p.share && token < s.nq;
             const int lim = mine ? sees(s, token, a.causal) : 0;
             const int least = tile_first < s.nq ? min(sees(s, tile_first, a.causal), min(s.bad, s.nk)) : 0;      // keys that all its rows see
+            const int seen = min(s.nk, s.bad);                        // what lies behind is nobody's
             const bool busy = __any_sync(0xffffffffu, mine);
             const bool turned = p.scale_log2 <= 0.f;                  // the largest score is not the largest product
             const float scale = turned ? 1.f : p.scale_log2;
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 if (part) {
                     const int rel = j - j0, load = WIDE ? 2 * rel + 1 : rel == all - 1 ? 2 * all - 1 : 2 * rel + 2, stage = load % NST;
                     if (!mbar_wait_warp(full + 8 * stage, (load / NST) & 1)) { ok = false; break; }
-                    if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r)) { atomicMin(&odd_first, j); atomicMax(&odd_last, j); }
+                    if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r) && k0 + r < seen) { atomicMin(&odd_first, k0 + r); atomicMax(&odd_last, k0 + r); }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
                 if (busy) {
@@ -394,6 +395,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
             float other = 0.f, own = 1.f;                             // what the two halves' sums count
             bool join = false;
             if (!WIDE) {
+                asm volatile("bar.sync 1, 256;\n" ::: "memory");      // the other half's products have read the stages too
                 if (t == 1) {
                     if (busy && steps > 0) {
                         handed[r] = make_float2(m, sum);
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                         o[e] = none ? 0.f : o[e] * inv;
                     }
                     if (odd1 >= 0 && !none && sum != 0.f) {           // rare: values that are not finite and that this row sees
-                        for (int k = odd0 * KT; k < min(lim, (odd1 + 1) * KT); ++k) {
+                        for (int k = odd0; k <= min(lim - 1, odd1); ++k) {
                             const T *v = key_row<T>(a, s, it.b, k, a.value, a.value_strides);
                             if (v == nullptr) continue;
                             v += group * a.value_strides[1] + c;

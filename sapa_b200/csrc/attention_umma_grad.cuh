@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_keys_kernel(con
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     begin_after_previous();
     if (warp == 0) {
-        const Item r = block_at<false>(blockIdx.x / a.groups, a.B, lane, [&](int b) { return (sequence_at(a, b).nk + KT - 1) / KT; });
+        const Item r = block_at<false>(a, blockIdx.x / a.groups, lane, KeyBlocks{a.causal != 0, tok, KT});
         if (lane == 0) item = r;
     }
     tc_fence_before();
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_keys_kernel(con
                 if (part) {                                           // dP has been computed from dO as it is, S from Q
                     if (!mbar_wait_warp(dpfull, i & 1)) { ok = false; break; }
                     if (half == 0) {
-                        if (clean_row<T, D>(base + L::O0 + st * L::TILE_BYTES, r)) { atomicMin(&odd_first, i); atomicMax(&odd_last, i); }
+                        if (clean_row<T, D>(base + L::O0 + st * L::TILE_BYTES, r) && r < used) { atomicMin(&odd_first, i * rows + r); atomicMax(&odd_last, i * rows + r); }
                     } else {
                         (void)clean_row<T, D>(base + L::Q0 + st * L::TILE_BYTES, r);
                     }
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_keys_kernel(con
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = n > 0 ? o[e] * factor : 0.f;
                 if (half == 0 && odd1 >= 0) {                         // rare: rows of dO with something not finite that see this value
-                    for (int row = odd0 * rows; row < min((odd1 + 1) * rows, (s.nq - from) * p.share); ++row) {
+                    for (int row = odd0; row <= odd1; ++row) {
                         const int i = from + row / p.share;
                         if (key >= sees(s, i, a.causal)) continue;
                         const T *v = static_cast<const T *>(g.go) + (long long)(s.q0 + i) * g.go_strides[0] + (long long)(group * p.share + row % p.share) * g.go_strides[1] + c;
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_queries_kernel(
     }
     begin_after_previous();
     if (warp == 0) {
-        const Item r = block_at<true>(blockIdx.x / a.groups, a.B, lane, [&](int b) { return (sequence_at(a, b).nq + tok - 1) / tok; });
+        const Item r = block_at<true>(a, blockIdx.x / a.groups, lane, QueryBlocks{a.causal != 0, tok, KT});
         if (lane == 0) item = r;
     }
     tc_fence_before();
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_queries_kernel(
                     x[c] = ex2_ftz(u.x); x[c + 1] = ex2_ftz(u.y);
                 }
                 if (part && half == 0) {                              // the scores have been computed from the keys as they are
-                    if (clean_row<T, D>(base + L::K0 + st * L::TILE_BYTES, r)) { atomicMin(&odd_first, i); atomicMax(&odd_last, i); }
+                    if (clean_row<T, D>(base + L::K0 + st * L::TILE_BYTES, r) && k0 + r < s.nk) { atomicMin(&odd_first, k0 + r); atomicMax(&odd_last, k0 + r); }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
                 if (!mbar_wait_warp(dpfull, i & 1)) { ok = false; break; }
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_queries_kernel(
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = n > 0 && lim > 0 ? o[e] * a.scale : 0.f;
                 if (odd1 >= 0) {                                      // rare: keys with something not finite that this row sees
-                    for (int k = odd0 * KT; k < min(lim, (odd1 + 1) * KT); ++k) {
+                    for (int k = odd0; k <= min(lim - 1, odd1); ++k) {
                         const T *v = static_cast<const T *>(a.key) + (long long)(s.k0 + k) * a.key_strides[0] + group * a.key_strides[1] + c;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
