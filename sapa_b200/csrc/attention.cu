@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
     const int group = blockIdx.x % a.groups, tok = L::BM / p.share, D = a.dim;
     begin_after_previous();
     if (tid < 32) {
-        const Plan r = plan_at(p, blockIdx.x / a.groups, tok, tid);
+        const Plan r = ForwardPlans(p, tok, tid).at(blockIdx.x / a.groups);
         if (tid == 0) { plan = r; bad_page = 0x7fffffff; }
     }
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, tid, NT);
@@ -220,20 +220,27 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
     }
 }
 
-// Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(lse_p - max lse).  A block of the grid per block and group, a warp per row.
+// Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(lse_p - max lse).  Grid: a block and group, 16 of its rows; a warp per row, whose
+// lanes first weigh the parts and then take 4 channels each.  Bound by the latency of its few loads; four parts are on their way at once.
 template <typename T>
 __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_constant__ Args p, int bm, int tok) {
     const sapa_attention &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x % a.groups, D = a.dim;
+    __shared__ Plan shared_plan;
     begin_after_previous();
-    const Plan plan = split_at<false>(p, blockIdx.x / a.groups, tok, lane);
+    if (warp == 0) {
+        const Plan r = split_at<false>(p, blockIdx.x / a.groups, tok, part_tiles(p, tok, lane), lane);
+        if (lane == 0) shared_plan = r;
+    }
+    __syncthreads();
+    const Plan plan = shared_plan;
     if (!plan.it.there || plan.it.parts == 1) return;
     const Sequence s = sequence_at(a, plan.it.b);
-    const int first = plan.it.block * tok, used = min(tok, s.nq - first) * p.share;
+    const int first = plan.it.block * tok, used = min(tok, s.nq - first) * p.share, parts = plan.it.parts;
     const long long step = (long long)a.groups * bm;                                  // from a part to the next
-    for (int r = warp; r < used; r += 8) {
+    for (int r = blockIdx.y * 16 + warp; r < min(used, (int)blockIdx.y * 16 + 16); r += 8) {
         const long long at = ((long long)plan.first * a.groups + group) * bm + r;
-        const int parts = plan.it.parts, lim = sees(s, first + r / p.share, a.causal);
+        const int lim = sees(s, first + r / p.share, a.causal);
         float top = -INFINITY;
         bool lost = false;
         for (int q = lane; q < parts; q += 32) { const float e = p.part_lse[at + q * step]; top = fmaxf(top, e); lost = lost || e != e; }
@@ -242,14 +249,24 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
         lost = __any_sync(0xffffffffu, lost) || (lim > 0 && top == -INFINITY);
         float sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int q = 0; q < parts; ++q) {
-            const float e = p.part_lse[at + q * step];
-            if (e == -INFINITY) continue;
-            const float w = exp2f(e - top);
-            sum += w;
-            if (4 * lane < D) {
-                const float4 v = *reinterpret_cast<const float4 *>(p.part + (at + q * step) * D + 4 * lane);
-                acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+        const float *from = p.part + at * D + 4 * lane;
+        for (int q0 = 0; q0 < parts; q0 += 32) {
+            const float e = q0 + lane < parts ? p.part_lse[at + (q0 + lane) * step] : -INFINITY;
+            const float mine = e == -INFINITY ? 0.f : exp2f(e - top);
+            const int n = min(32, parts - q0);
+            for (int q = 0; q < n; q += 4) {
+                float4 v[4];
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {                                         // a part that a row sees nothing of counts 0, and holds 0
+                    w[i] = __shfl_sync(0xffffffffu, mine, q + i);
+                    v[i] = q + i < n && 4 * lane < D ? *reinterpret_cast<const float4 *>(from + (q0 + q + i) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum += w[i];
+                    acc.x = fmaf(w[i], v[i].x, acc.x); acc.y = fmaf(w[i], v[i].y, acc.y); acc.z = fmaf(w[i], v[i].z, acc.z); acc.w = fmaf(w[i], v[i].w, acc.w);
+                }
             }
         }
         const float inv = lost ? __int_as_float(0x7fffffff) : lim <= 0 ? 0.f : 1.f / sum;
@@ -323,7 +340,8 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(cons
     const int slot = blockIdx.x % slots, group = KEYS ? slot : slot % a.groups;
     begin_after_previous();
     if (tid < 32) {
-        const Item r = KEYS ? block_at<false>(a, blockIdx.x / slots, tid, KeyBlocks{a.causal != 0, tok, N}) : block_at<true>(a, blockIdx.x / slots, tid, QueryBlocks{a.causal != 0, tok, N});
+        const Item r = KEYS ? InOrder<false, KeyBlocks>(a, KeyBlocks{a.causal != 0, tok, N}, tid).at(blockIdx.x / slots)
+                            : InOrder<true, QueryBlocks>(a, QueryBlocks{a.causal != 0, tok, N}, tid).at(blockIdx.x / slots);
         if (tid == 0) item = r;
     }
     __syncthreads();
@@ -582,7 +600,7 @@ static Args args_of(const sapa_attention *a) {
 // A forward of this call: rows of a block, whether its keys are split, and the room that takes.
 struct Shape {
     bool umma, narrow;
-    int bm, tok, split;
+    int bm, tok, split, rows;      // rows: of a block that can be in use
     long long blocks, grid;        // blocks x groups at most; items at most
     size_t part, lse, bytes;       // of the workspace
 };
@@ -602,6 +620,7 @@ static Shape shape_of(const Args &p, int dtype, int sms) {
         s.tok = s.bm / p.share;
     }
     s.blocks = most_blocks(a, a.tokens, s.tok) * a.groups;
+    s.rows = (a.tokens < s.tok ? a.tokens : s.tok) * p.share;
     s.grid = s.blocks;
     // few blocks: their keys are split so that every SM has items
     const long long keys = a.page_table != nullptr ? (long long)a.max_pages * a.page : a.keys;
@@ -672,7 +691,7 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
         else if (s.narrow) e = a->dim <= 64 ? run_rows<scalar_t, 1, 64>(p, s, st) : run_rows<scalar_t, 1, 128>(p, s, st);
         else e = a->dim <= 64 ? run_rows<scalar_t, 8, 64>(p, s, st) : run_rows<scalar_t, 8, 128>(p, s, st);
         if (e != SAPA_OK || s.split == 0) return e;
-        launch_next(sapa_attention_join_kernel<scalar_t>, dim3((unsigned)s.blocks), dim3(256), 0, st, p, s.bm, s.tok);
+        launch_next(sapa_attention_join_kernel<scalar_t>, dim3((unsigned)s.blocks, (unsigned)ceil_div(s.rows, 16)), dim3(256), 0, st, p, s.bm, s.tok);
         return check_launch("sapa_attention_join_kernel");
     });
 }

@@ -62,45 +62,64 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {      // inclusive
     return v;
 }
 
-// The blocks of all sequences in the order in which they are started, found by a whole warp: those with the most work first, so that short ones
-// fill the end.  `at_least(s, w)`: blocks of a sequence with at least w units of work, all for w = 0; `units(s)`: the most that one of its blocks has.
-// LAST: a sequence's blocks have the more work the later they come (a causal token sees the more keys), otherwise the less.  The amount of work is
-// searched for by halving, each time adding up the sequences' counts; each lane keeps the first of its sequences in registers.
-template <bool LAST, typename Units, typename Count>
-__device__ __forceinline__ Item block_at(const sapa_attention &a, int index, int lane, Units units, Count at_least) {
-    Item it{0, 0, 0, 1, false};
-    Sequence mine{0, 0, 0, 0, 0};
-    if (lane < a.B) mine = sequence_at(a, lane);
-    auto all = [&](int w) {
-        int n = at_least(mine, w);
-        for (int b = lane + 32; b < a.B; b += 32) n += at_least(sequence_at(a, b), w);
+// The blocks of all sequences in the order of their work, found by a whole warp: those with the most first, so that short ones fill the end.
+// `Blocks::at_least(s, w)`: blocks of a sequence with at least w units of work, all for w = 0; `units(s)`: the most that one of its blocks has.  LAST: a
+// sequence's blocks have the more work the later they come (a causal token sees the more keys), otherwise the less.  The amount of work is searched
+// for by halving, each time adding up the sequences' counts; each lane keeps the first of its sequences in registers.  A block of the grid asks for
+// growing indices, so the search goes on from the last one's: mostly nothing is added up again.
+template <bool LAST, typename Blocks> struct InOrder {
+    const sapa_attention &a;
+    const Blocks kind;
+    const int lane;
+    Sequence own;
+    int total, lo, hi, upto, behind;                    // all(lo) = upto > index >= behind = all(hi)
+    __device__ __forceinline__ InOrder(const sapa_attention &args, const Blocks &k, int l, bool wanted = true)
+        : a(args), kind(k), lane(l), own{0, 0, 0, 0, 0}, total(0), lo(0), hi(0), upto(0), behind(0) {
+        if (!wanted) return;
+        if (lane < a.B) own = sequence_at(a, lane);
+        int most = kind.units(own);
+        for (int b = lane + 32; b < a.B; b += 32) most = max(most, kind.units(sequence_at(a, b)));
+        total = all(0);
+        hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) + 1;
+        lo = hi;
+        upto = behind = 0;
+    }
+    __device__ __forceinline__ int all(int w) const {
+        int n = kind.at_least(own, w);
+        for (int b = lane + 32; b < a.B; b += 32) n += kind.at_least(sequence_at(a, b), w);
         return warp_sum(n);
-    };
-    if (index >= all(0)) return it;
-    int most = units(mine);
-    for (int b = lane + 32; b < a.B; b += 32) most = max(most, units(sequence_at(a, b)));
-    int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) + 1, behind = 0;      // all(lo) > index >= all(hi) = behind
-    while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2, n = all(mid);
-        if (n > index) lo = mid; else { hi = mid; behind = n; }
     }
-    int left = index - behind;                          // among the blocks with just lo units
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        const int b = b0 + lane;
-        if (b0 > 0) mine = b < a.B ? sequence_at(a, b) : Sequence{0, 0, 0, 0, 0};
-        const int more = at_least(mine, hi), here = at_least(mine, lo) - more, upto = warp_scan(here, lane);
-        const unsigned hit = __ballot_sync(0xffffffffu, left < upto);
-        if (hit != 0u) {
-            const int from = __ffs(hit) - 1, before = more + left - (upto - here);      // blocks of the sequence with no less work in front of it
-            it.b = b0 + from;
-            it.block = __shfl_sync(0xffffffffu, LAST ? at_least(mine, 0) - 1 - before : before, from);
-            it.there = true;
-            return it;
+    __device__ __forceinline__ Item at(int index) {
+        Item it{0, 0, 0, 1, false};
+        if (index >= total) return it;
+        if (index >= upto) {
+            hi = lo;
+            behind = upto;
+            lo = 0;
+            upto = total;
+            while (hi - lo > 1) {
+                const int mid = lo + (hi - lo) / 2, n = all(mid);
+                if (n > index) { lo = mid; upto = n; } else { hi = mid; behind = n; }
+            }
         }
-        left -= __shfl_sync(0xffffffffu, upto, 31);
+        int left = index - behind;                      // among the blocks with just lo units
+        for (int b0 = 0; b0 < a.B; b0 += 32) {
+            const int b = b0 + lane;
+            const Sequence s = b0 == 0 ? own : b < a.B ? sequence_at(a, b) : Sequence{0, 0, 0, 0, 0};
+            const int more = kind.at_least(s, hi), here = kind.at_least(s, lo) - more, end = warp_scan(here, lane);
+            const unsigned hit = __ballot_sync(0xffffffffu, left < end);
+            if (hit != 0u) {
+                const int from = __ffs(hit) - 1, before = more + left - (end - here);      // blocks of the sequence with no less work in front of it
+                it.b = b0 + from;
+                it.block = __shfl_sync(0xffffffffu, LAST ? kind.at_least(s, 0) - 1 - before : before, from);
+                it.there = true;
+                return it;
+            }
+            left -= __shfl_sync(0xffffffffu, end, 31);
+        }
+        return it;
     }
-    return it;
-}
+};
 __device__ __forceinline__ int tiles_of(int n, int tile) { return (int)(((unsigned)n + (unsigned)tile - 1) / (unsigned)tile); }
 // Blocks of `tok` tokens, by the tiles of `tile` keys that they go over (what a block's last token sees)
 struct QueryBlocks {
@@ -128,10 +147,6 @@ struct KeyBlocks {
         return !causal ? n : key < 0 ? 0 : min(n, (int)((unsigned)key / (unsigned)tile) + 1);
     }
 };
-template <bool LAST, typename Blocks> __device__ __forceinline__ Item block_at(const sapa_attention &a, int index, int lane, const Blocks &k) {
-    return block_at<LAST>(a, index, lane, [&](const Sequence &s) { return k.units(s); }, [&](const Sequence &s, int w) { return k.at_least(s, w); });
-}
-
 // Where a block that is split finds its part: the keys of every sequence are cut into parts of even lengths, tiles of TILE keys,
 // so many that all sequences together make about `split` items (their lengths are known on the device alone).  A sequence's blocks all have as many parts as its
 // whole length gives; of a causal block the last ones may see nothing and are empty.
@@ -141,19 +156,22 @@ struct Plan {
     int tiles;                     // TILEs of a part
     int first;                     // number of the block's first part among all
 };
-// The index-th item (PARTS) or block (!PARTS) of all sequences, by a whole warp.  tok: tokens of a block.
-template <bool PARTS>
-__device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int lane) {
-    const sapa_attention &a = p.a;
-    Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
+// Tiles of a part at most, for all sequences
+__device__ __forceinline__ int part_tiles(const Args &p, int tok, int lane) {
     unsigned long long work = 0;
-    for (int b = lane; b < a.B; b += 32) {
-        const Sequence s = sequence_at(a, b);
+    for (int b = lane; b < p.a.B; b += 32) {
+        const Sequence s = sequence_at(p.a, b);
         work += (unsigned long long)((s.nq + tok - 1) / tok) * (unsigned)((min(s.nk, s.bad) + TILE - 1) / TILE);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-    const int most = (int)max((work * a.groups + p.split - 1) / (unsigned)p.split, (unsigned long long)p.least);      // tiles of a part
+    return (int)max((work * p.a.groups + p.split - 1) / (unsigned)p.split, (unsigned long long)p.least);
+}
+// The index-th item (PARTS) or block (!PARTS) of all sequences, by a whole warp.  tok: tokens of a block; most: of part_tiles.
+template <bool PARTS>
+__device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int most, int lane) {
+    const sapa_attention &a = p.a;
+    Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
     int before = 0, items = 0;     // blocks or items of the sequences before; their items
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         const int b = b0 + lane;
@@ -184,13 +202,18 @@ __device__ __forceinline__ Plan split_at(const Args &p, int index, int tok, int 
     }
     return r;
 }
-// The work of block `index` (group apart) of a forward kernel, by a whole warp.
-__device__ __forceinline__ Plan plan_at(const Args &p, int index, int tok, int lane) {
-    if (p.split > 0) return split_at<true>(p, index, tok, lane);
-    Plan r{{0, 0, 0, 1, false}, 0x7fffffff / TILE, 0};
-    r.it = block_at<true>(p.a, index, lane, QueryBlocks{p.a.causal != 0, tok, TILE});
-    return r;
-}
+// The work of a forward kernel's blocks (group apart), by a whole warp, for growing indices.
+struct ForwardPlans {
+    const Args &p;
+    const int tok, lane, most;
+    InOrder<true, QueryBlocks> order;
+    __device__ __forceinline__ ForwardPlans(const Args &args, int t, int l)
+        : p(args), tok(t), lane(l), most(args.split > 0 ? part_tiles(args, t, l) : 0), order(args.a, QueryBlocks{args.a.causal != 0, t, TILE}, l, args.split == 0) {}
+    __device__ __forceinline__ Plan at(int index) {
+        if (p.split > 0) return split_at<true>(p, index, tok, most, lane);
+        return Plan{order.at(index), 0x7fffffff / TILE, 0};
+    }
+};
 
 // Of a backward pass
 struct Grads {
@@ -203,7 +226,7 @@ struct Grads {
 
 // Tensor-core forward (attention_umma.cu): what it takes, and its launch; wide: two row tiles a block.
 bool umma_takes(const sapa_attention &a, int dtype);
-int umma_forward(const Args &p, bool wide, long long grid, int dtype, cudaStream_t st);
+int umma_forward(const Args &p, bool wide, long long items, int dtype, cudaStream_t st);
 int umma_backward(const Args &p, const Grads &g, int dtype, cudaStream_t st);
 // Blocks of `tok` tokens that all sequences together can have.
 inline long long most_blocks(const sapa_attention &a, long long total, int tok) {

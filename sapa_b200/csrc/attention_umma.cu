@@ -44,11 +44,16 @@ static bool encode(CUtensorMap *map, const void *base, int dim, int rank, const 
 }
 
 template <typename T, int D, bool WIDE, bool PAGED>
-static int launch(const Args &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, long long grid, cudaStream_t st) {
+static int launch(const Args &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, long long items, cudaStream_t st) {
     using L = um::Lay<D, WIDE>;
     int sms = 0;
     if (int e = prepare_launch((const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED>, L::SMEM, "sapa_attention_umma_kernel", sms)) return e;
-    launch_next(sapa_attention_umma_kernel<T, D, WIDE, PAGED>, dim3((unsigned)grid), dim3(NT), L::SMEM, st, q, k, v, p);
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, (const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED>) == cudaSuccess ? f.numRegs : -1;
+    }();
+    SAPA_REQUIRE(regs == um::REGS, SAPA_ERR_LAUNCH, "sapa_attention_umma_kernel: built with %d registers, its warps would wait for %d", regs, um::REGS);
+    launch_next(sapa_attention_umma_kernel<T, D, WIDE, PAGED>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), L::SMEM, st, q, k, v, p, (int)items);
     return check_launch(WIDE ? "sapa_attention_umma_kernel<wide>" : "sapa_attention_umma_kernel<narrow>");
 }
 
@@ -60,7 +65,7 @@ bool umma_takes(const sapa_attention &a, int dtype) {
     return a.page >= 8 && (a.page & (a.page - 1)) == 0;               // pages that a tile of 128 keys holds whole, or that hold it
 }
 
-int umma_forward(const Args &p, bool wide, long long grid, int dtype, cudaStream_t st) {
+int umma_forward(const Args &p, bool wide, long long items, int dtype, cudaStream_t st) {
     using namespace um;
     const sapa_attention &a = p.a;
     const bool half = dtype == SAPA_F16, paged = a.page_table != nullptr;
@@ -78,11 +83,11 @@ int umma_forward(const Args &p, bool wide, long long grid, int dtype, cudaStream
     auto pick = [&](auto t) -> int {
         using T = decltype(t);
         if (a.dim <= 64) {
-            if (wide) return paged ? launch<T, 64, true, true>(p, q, k, v, grid, st) : launch<T, 64, true, false>(p, q, k, v, grid, st);
-            return paged ? launch<T, 64, false, true>(p, q, k, v, grid, st) : launch<T, 64, false, false>(p, q, k, v, grid, st);
+            if (wide) return paged ? launch<T, 64, true, true>(p, q, k, v, items, st) : launch<T, 64, true, false>(p, q, k, v, items, st);
+            return paged ? launch<T, 64, false, true>(p, q, k, v, items, st) : launch<T, 64, false, false>(p, q, k, v, items, st);
         }
-        if (wide) return paged ? launch<T, 128, true, true>(p, q, k, v, grid, st) : launch<T, 128, true, false>(p, q, k, v, grid, st);
-        return paged ? launch<T, 128, false, true>(p, q, k, v, grid, st) : launch<T, 128, false, false>(p, q, k, v, grid, st);
+        if (wide) return paged ? launch<T, 128, true, true>(p, q, k, v, items, st) : launch<T, 128, true, false>(p, q, k, v, items, st);
+        return paged ? launch<T, 128, false, true>(p, q, k, v, items, st) : launch<T, 128, false, false>(p, q, k, v, items, st);
     };
     return half ? pick(__half()) : pick(__nv_bfloat16());
 }
@@ -96,9 +101,9 @@ static int launch(const Args &p, const Grads &g, const CUtensorMap &q, const CUt
     constexpr int KEYS = KeyLay<D>::SMEM, QUERIES = QueryLay<D>::SMEM;
     if (int e = prepare_launch((const void *)sapa_attention_umma_keys_kernel<T, D>, KEYS, "sapa_attention_umma_keys_kernel", sms)) return e;
     if (int e = prepare_launch((const void *)sapa_attention_umma_queries_kernel<T, D>, QUERIES, "sapa_attention_umma_queries_kernel", sms)) return e;
-    launch_next(sapa_attention_umma_keys_kernel<T, D>, dim3((unsigned)key_blocks), dim3(NT), KEYS, st, q, o, k, v, p, g);
+    launch_next(sapa_attention_umma_keys_kernel<T, D>, dim3((unsigned)key_blocks), dim3(umg::THREADS), KEYS, st, q, o, k, v, p, g);
     if (int e = check_launch("sapa_attention_umma_keys_kernel")) return e;
-    launch_next(sapa_attention_umma_queries_kernel<T, D>, dim3((unsigned)query_blocks), dim3(NT), QUERIES, st, q, o, k, v, p, g);
+    launch_next(sapa_attention_umma_queries_kernel<T, D>, dim3((unsigned)query_blocks), dim3(umg::THREADS), QUERIES, st, q, o, k, v, p, g);
     return check_launch("sapa_attention_umma_queries_kernel");
 }
 

@@ -1,6 +1,7 @@
 // attention_umma.cuh — attention over sequences in 16 bits on the 5th-generation tensor cores, forward.  Included by attention_umma.cu.
 //
-// A block takes 128-row tiles (row = token x query head of one key head) against tiles of 128 keys:
+// A block an SM, items in turn: 128-row tiles (row = token x query head of one key head) against tiles of 128 keys.
+//   * a warp finds the items, one ahead (they follow from lengths that only the device knows);
 //   * a warp loads queries, keys and values with TMA (rows of 64 channels, 128-byte swizzle; of a paged cache a box a page);
 //   * a warp issues S = Q K^T (both operands K-major in shared memory) and O += P V (P in tensor memory, V as TMA lands it, MN-major);
 //   * a warpgroup for each of two S / O accumulators: a thread holds a row, 128 scores in registers, so maximum and sum need no shuffles; it writes P,
@@ -24,7 +25,10 @@ namespace um {
 using namespace ummau;
 
 constexpr int KT = TILE, ROWS = 128, BLOCK_BYTES = 128 * 128;         // keys of a tile, rows of a tile; 128 rows of 64 channels
-constexpr int MMA_WARP = 8, LOAD_WARP = 9, NT = 10 * 32;
+constexpr int MMA_WARP = 8, LOAD_WARP = 9, PLAN_WARP = 10, NT = 12 * 32;
+// registers a thread: 168 at launch, then what the softmax needs for a row of scores and the other four warps for theirs (multiples of 8)
+constexpr int REGS = 168, SOFTMAX_REGS = 208, OTHER_REGS = 88;
+static_assert(8 * 32 * SOFTMAX_REGS + 4 * 32 * OTHER_REGS <= NT * REGS, "a block draws on what it was launched with");
 constexpr unsigned HI = (1024u >> 4) | (1u << 14) | (2u << 29);       // 8 rows of 128 bytes, descriptor version 1, 128-byte swizzle
 constexpr float GROWTH = 8.f;                                         // powers of two
 
@@ -34,7 +38,16 @@ template <int D, bool WIDE> struct Lay {
     static constexpr int Q0 = 0, KV0 = Q_BYTES;
     static constexpr int NEED = KV0 + NST * STAGE + 1024, SMEM = NEED < 120 * 1024 ? 120 * 1024 : NEED;      // one block an SM: tensor memory
     static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
-    static_assert(SMEM <= 227 * 1024 && NST * STAGE >= ROWS * D * 4, "shared memory");      // the odd tiles' sums are handed over in it
+    static_assert(SMEM <= 225 * 1024 && NST >= 3, "shared memory");      // with the 2 KB that a block holds besides
+};
+
+// An item of a block: `tok` tokens of a sequence, one key head, key tiles from j0
+struct Work {
+    bool there;
+    int b, group, index, parts;    // index: of the item among all
+    int first, j0, all, n0, n1;    // first token; key tiles, of all and of each accumulator
+    Sequence s;
+    int bad_page, odd_first, odd_last;      // first position without a page; keys with a value that is not finite and not seen by every row
 };
 
 __device__ __forceinline__ void tc_ld32(unsigned taddr, float *r) {
@@ -109,128 +122,164 @@ template <typename T> __device__ __forceinline__ void store_row(T *to, const flo
 
 template <typename T, int D, bool WIDE, bool PAGED>
 __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                                                                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args p) {
+                                                                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args p, const int most_items) {
     using namespace um;
     using L = um::Lay<D, WIDE>;
     constexpr int NST = L::NST;
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) unsigned long long bars[1 + 2 * NST + 4];
+    __shared__ __align__(8) unsigned long long bars[2 + 2 * NST + 4 + 4 + 4];
     __shared__ unsigned tmem_slot;
-    __shared__ Plan plan;
-    __shared__ int bad_page, odd_first, odd_last;
-    __shared__ float2 handed[WIDE ? 1 : ROWS];                        // maximum and sum of the odd tiles
+    __shared__ Work queue[2];
+    __shared__ float handed[WIDE ? 1 : 2][ROWS];                      // maximum, then sum, of the even and the odd tiles
     const sapa_attention &a = p.a;
     const unsigned base = ((unsigned)__cvta_generic_to_shared(smem_dyn) + 1023u) & ~1023u;
-    const unsigned qfull = (unsigned)__cvta_generic_to_shared(bars), full = qfull + 8, empty = full + 8 * NST, sfull = empty + 8 * NST, pfull = sfull + 16;
+    const unsigned qfull = (unsigned)__cvta_generic_to_shared(bars), qempty = qfull + 8, full = qempty + 8, empty = full + 8 * NST, sfull = empty + 8 * NST, pfull = sfull + 16;
+    const unsigned posted = pfull + 16, taken = posted + 16, pair = taken + 16;
     const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
-    const int group = blockIdx.x % a.groups, tile_tok = ROWS / p.share, tok = WIDE ? 2 * tile_tok : tile_tok;
+    const int tile_tok = ROWS / p.share, tok = WIDE ? 2 * tile_tok : tile_tok;
 
     if (warp == MMA_WARP) {
         if (lane == 0) {
-            mbar_init(qfull, 1);
+            mbar_init(qfull, 1); mbar_init(qempty, 1);
             for (int i = 0; i < NST; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
-            for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 128); }
+            for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 128); mbar_init(posted + 8 * i, 1); mbar_init(taken + 8 * i, 10); }
+            for (int i = 0; i < 4; ++i) mbar_init(pair + 8 * i, 256);
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-            bad_page = 0x7fffffff; odd_first = 0x7fffffff; odd_last = -1;
         }
         __syncwarp();
         tc_alloc((unsigned)__cvta_generic_to_shared(&tmem_slot), L::TMEM_COLS);
         tc_relinquish();
     }
     begin_after_previous();
-    if (warp == 0) {
-        const Plan r = plan_at(p, blockIdx.x / a.groups, tok, lane);
-        if (lane == 0) plan = r;
-    }
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
     if (a.lse != nullptr) clear_outside(a.lse, a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = warp_uniform(*reinterpret_cast<volatile unsigned *>(&tmem_slot));
-    const Item it = plan.it;
     bool ok = true;
-    if (it.there) {
-        const Sequence s = sequence_at(a, it.b);
-        const int first = it.block * tok;                             // first token
-        // key tiles of the two accumulators: [j0, j0 + n[t]) each (WIDE), or every other one of n
-        const int j0 = (int)min((long long)it.part * plan.tiles, 0x7fffffffll / KT);
-        int n[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int last = min(first + (WIDE ? (t + 1) * tile_tok : tile_tok), s.nq) - 1;      // its last token
-            const bool some = last >= first + (WIDE ? t * tile_tok : 0);
-            const int tiles = some ? (min(sees(s, last, a.causal), s.bad) + KT - 1) / KT : 0;
-            n[t] = max(0, (int)min((long long)tiles, (long long)j0 + plan.tiles) - j0);
-        }
-        const int all = (int)warp_uniform(max(n[0], n[1]));           // the block's
-        if (!WIDE) { n[0] = (all + 1) / 2; n[1] = all / 2; }
-        const int n0 = (int)warp_uniform(n[0]), n1 = (int)warp_uniform(n[1]);
+    // the block's items one after the other: what all warps but the plans' go through
+    int turn = 0;
+    auto next_work = [&]() {                                          // nullptr behind the last one, or where a wait gave up
+        ok = ok && mbar_wait_warp(posted + 8 * (turn & 1), (turn >> 1) & 1);
+        return ok && queue[turn & 1].there ? &queue[turn & 1] : nullptr;
+    };
+    auto work_done = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(taken + 8 * (turn & 1));
+        ++turn;
+    };
 
-        if (warp == LOAD_WARP) {
-            int st = 0, ph = 0;
+    if (warp >= MMA_WARP) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(OTHER_REGS));
+        if (warp == PLAN_WARP) {
+            ForwardPlans plans(p, tok, lane);
+            for (int round = 0;; ++round) {
+                // item numbers go there and back over the grid: the work of a block's items evens out
+                const int index = round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+                Work w{};
+                if (index < most_items) {
+                    const Plan r = plans.at(index / a.groups);
+                    w.there = r.it.there;
+                    if (w.there) {
+                        w.b = r.it.b; w.parts = r.it.parts; w.group = index % a.groups; w.index = index;
+                        w.s = sequence_at(a, w.b);
+                        w.first = r.it.block * tok;
+                        // key tiles of the two accumulators: [j0, j0 + n[t]) each (WIDE), or every other one
+                        w.j0 = r.it.part * (r.it.parts > 1 ? r.tiles : 0);
+                        int n[2];
+    #pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int last = min(w.first + (WIDE ? (t + 1) * tile_tok : tile_tok), w.s.nq) - 1;      // its last token
+                            const bool some = last >= w.first + (WIDE ? t * tile_tok : 0);
+                            const int tiles = some ? tiles_of(min(sees(w.s, last, a.causal), w.s.bad), KT) : 0;
+                            n[t] = max(0, min(tiles - w.j0, r.tiles));
+                        }
+                        w.all = max(n[0], n[1]);
+                        w.n0 = WIDE ? n[0] : (w.all + 1) / 2;
+                        w.n1 = WIDE ? n[1] : w.all / 2;
+                    }
+                }
+                w.bad_page = 0x7fffffff; w.odd_first = 0x7fffffff; w.odd_last = -1;
+                ok = mbar_wait_warp(taken + 8 * (round & 1), ((round >> 1) & 1) ^ 1);
+                if (!ok) break;
+                if (lane == 0) { queue[round & 1] = w; mbar_arrive(posted + 8 * (round & 1)); }
+                __syncwarp();
+                if (!w.there) break;
+            }
+        } else if (warp == LOAD_WARP) {
+            int st = 0, ph = 0, qph = 0;
             const int boxes = PAGED ? max(1, KT / a.page) : 1, box_rows = KT / boxes;
-            if (lane == 0) {
-                mbar_expect_tx(qfull, (WIDE ? 2 : 1) * (D / 64) * 128 * p.share * tile_tok);
-                for (int t = 0; t < (WIDE ? 2 : 1); ++t)
-                    for (int b = 0; b < D / 64; ++b)
-                        tma_load_3d(base + L::Q0 + t * L::STAGE + b * BLOCK_BYTES, &qmap, qfull, 64 * b, group * p.share, s.q0 + first + t * tile_tok);
-            }
-            const int used = min(s.bad, s.nk);                        // positions that the table has pages for
-            // pages of a tile, each lane one: the page, -1 behind the keys
-            auto page_of = [&](int j) {
-                const int at = j * KT + lane * box_rows;
-                if (!PAGED || lane >= boxes || j >= j0 + all || at >= used) return -1;
-                int page = a.page_table[(long long)it.b * a.max_pages + at / a.page];
-                if ((unsigned)page >= (unsigned)a.pages) { atomicMin(&bad_page, at); page = 0; }
-                return page;
-            };
-            auto load = [&](const CUtensorMap *map, int j, int page) {
-                const unsigned there = PAGED ? __ballot_sync(0xffffffffu, page >= 0) : 1u;
-                bool can = true;
-                if (lane == 0) {
-                    can = mbar_wait_bounded(empty + 8 * st, ph ^ 1);
-                    if (can) mbar_expect_tx(full + 8 * st, __popc(there) * box_rows * (D / 64) * 128);
+            while (Work *w = next_work()) {
+                const int j0 = w->j0, all = w->all, b = w->b, group = w->group;
+                const Sequence s = w->s;
+                const int used = min(s.bad, s.nk);                        // positions that the table has pages for
+                // entries of the table for a tile, each lane one: -1 behind the keys.  Looked at only in load(), so that they are on their way till then.
+                auto page_of = [&](int j) {
+                    const int at = j * KT + lane * box_rows;
+                    return !PAGED || lane >= boxes || j >= j0 + all || at >= used ? -1 : a.page_table[(long long)b * a.max_pages + (unsigned)at / (unsigned)a.page];
+                };
+                auto load = [&](const CUtensorMap *map, int j, int page) {
+                    const int at = j * KT + lane * box_rows;
+                    const bool mine = PAGED && lane < boxes && at < used;
+                    const unsigned there = PAGED ? __ballot_sync(0xffffffffu, mine) : 1u;
+                    if (mine && (unsigned)page >= (unsigned)a.pages) { atomicMin(&w->bad_page, at); page = 0; }
+                    __syncwarp();
+                    bool can = true;
+                    if (lane == 0) {
+                        can = mbar_wait_bounded(empty + 8 * st, ph ^ 1);
+                        if (can) mbar_expect_tx(full + 8 * st, __popc(there) * box_rows * (D / 64) * 128);
+                    }
+                    ok = __shfl_sync(0xffffffffu, can, 0) != 0;
+                    if (!ok) return;
+                    const unsigned dst = base + L::KV0 + st * L::STAGE;
+                    if (PAGED) {
+                        if (mine)
+                            for (int c = 0; c < D / 64; ++c)
+                                tma_load_4d(dst + c * BLOCK_BYTES + lane * box_rows * 128, map, full + 8 * st, 64 * c, group, a.page >= KT ? (unsigned)(j * KT) % (unsigned)a.page : 0, page);
+                    } else if (lane == 0) {
+                        for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * BLOCK_BYTES, map, full + 8 * st, 64 * c, group, s.k0 + j * KT);
+                    }
+                    if (++st == NST) { st = 0; ph ^= 1; }
+                };
+                int page0 = page_of(j0), page1 = page_of(j0 + 1);
+                if (all > 0) {
+                    if (lane == 0) {
+                        ok = mbar_wait_bounded(qempty, qph ^ 1);
+                        if (ok) {
+                            mbar_expect_tx(qfull, (WIDE ? 2 : 1) * (D / 64) * 128 * p.share * tile_tok);
+                            for (int t = 0; t < (WIDE ? 2 : 1); ++t)
+                                for (int c = 0; c < D / 64; ++c)
+                                    tma_load_3d(base + L::Q0 + t * L::STAGE + c * BLOCK_BYTES, &qmap, qfull, 64 * c, group * p.share, s.q0 + w->first + t * tile_tok);
+                        }
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0) != 0;
+                    if (!ok) break;
+                    qph ^= 1;
+                    load(&kmap, j0, page0);
                 }
-                ok = __shfl_sync(0xffffffffu, can, 0) != 0;
-                if (!ok) return;
-                const unsigned dst = base + L::KV0 + st * L::STAGE;
-                if (PAGED) {
-                    if (page >= 0)
-                        for (int b = 0; b < D / 64; ++b)
-                            tma_load_4d(dst + b * BLOCK_BYTES + lane * box_rows * 128, map, full + 8 * st, 64 * b, group, a.page >= KT ? (j * KT) % a.page : 0, page);
-                } else if (lane == 0) {
-                    for (int b = 0; b < D / 64; ++b) tma_load_3d(dst + b * BLOCK_BYTES, map, full + 8 * st, 64 * b, group, s.k0 + j * KT);
-                }
-                if (++st == NST) { st = 0; ph ^= 1; }
-            };
-            if (WIDE) {
-                int page = page_of(j0);
+                // WIDE: K0, V0, K1, V1, ...; otherwise K0, K1, V0, K2, V1, ...: the scores are a tile further ahead
                 for (int j = j0; j < j0 + all && ok; ++j) {
-                    const int next = page_of(j + 1);
-                    load(&kmap, j, page);
-                    if (ok) load(&vmap, j, page);
-                    page = next;
+                    const int page2 = page_of(j + 2);
+                    if (WIDE) load(&vmap, j, page0);
+                    if (ok && j + 1 < j0 + all) load(&kmap, j + 1, page1);
+                    if (!WIDE && ok) load(&vmap, j, page0);
+                    page0 = page1; page1 = page2;
                 }
-            } else {                                                  // K0, K1, V0, K2, V1, ...
-                int before = page_of(j0), page = page_of(j0 + 1);
-                if (all > 0) load(&kmap, j0, before);
-                for (int j = j0; j < j0 + all && ok; ++j) {
-                    const int next = page_of(j + 2);
-                    if (j + 1 < j0 + all) load(&kmap, j + 1, page);
-                    if (ok) load(&vmap, j, before);
-                    before = page; page = next;
-                }
+                if (!ok) break;
+                work_done();
             }
-            if (lane == 0) ok = mbar_wait_bounded(qfull, 0) && ok;
-            if (!ok && lane == 0) (void)drain_loads<NST>(full, st, ph);
+            if (!ok && lane == 0) {                                       // none of its loads may land after it has left
+                (void)drain_loads<NST>(full, st, ph);
+                (void)mbar_wait_bounded(qfull, qph ^ 1);
+            }
         } else if (warp == MMA_WARP) {
             constexpr unsigned IDESC_S = IDESC_M128<T> | idesc_n(KT), IDESC_O = IDESC_M128<T> | (1u << 16) | idesc_n(D);
             const unsigned leader = elect_leader();
             const unsigned q_base = warp_uniform(desc_lo(base + L::Q0, 16)), k_base = warp_uniform(desc_lo(base + L::KV0, 16)), v_base = warp_uniform(desc_lo(base + L::KV0, BLOCK_BYTES));
             constexpr unsigned STEP = L::STAGE >> 4;
-            int st = 0, ph = 0;                                       // next stage to wait for
-            auto wait_full = [&]() {                                  // the stage, once it has landed
+            int st = 0, ph = 0, qph = 0, pph0 = 0, pph1 = 0;              // next stage to wait for
+            auto wait_full = [&]() {                                      // the stage, once it has landed
                 ok = ok && mbar_wait_warp(full + 8 * st, ph);
                 const int now = st;
                 if (++st == NST) { st = 0; ph ^= 1; }
@@ -238,97 +287,122 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
             };
             auto scores = [&](int t, int stage) {
                 const unsigned q = q_base + (WIDE ? t : 0) * STEP, k = k_base + stage * STEP;
-#pragma unroll
+    #pragma unroll
                 for (int c = 0; c < D / 16; ++c)
                     tc_mma<false>(leader, tmem + L::S_COL + t * KT, q + (c >> 2) * (BLOCK_BYTES >> 4) + (c & 3) * 2, k + (c >> 2) * (BLOCK_BYTES >> 4) + (c & 3) * 2, HI, IDESC_S, c > 0 ? 1u : 0u);
             };
             auto outputs = [&](int t, int stage, bool add) {
                 const unsigned v = v_base + stage * STEP;
-#pragma unroll
+    #pragma unroll
                 for (int c = 0; c < KT / 16; ++c)
                     tc_mma_ta<false>(leader, tmem + L::O_COL + t * D, tmem + L::S_COL + t * KT + c * 8, v + c * (2048 >> 4), HI, IDESC_O, add || c > 0 ? 1u : 0u);
             };
-            ok = mbar_wait_warp(qfull, 0);
-            if (WIDE) {
-                if (all > 0 && ok) {
-                    const int k = wait_full();
-                    if (ok) {
-                        tc_fence_after();
-                        if (n0 > 0) { scores(0, k); tc_commit_by(leader, sfull); }
-                        if (n1 > 0) { scores(1, k); tc_commit_by(leader, sfull + 8); }
-                        tc_commit_by(leader, empty + 8 * k);
-                    }
+            auto weights_there = [&](int t) {
+                ok = ok && mbar_wait_warp(pfull + 8 * t, t == 0 ? pph0 : pph1);
+                if (t == 0) pph0 ^= 1; else pph1 ^= 1;
+                tc_fence_after();
+            };
+            while (Work *w = next_work()) {
+                const int all = (int)warp_uniform(w->all), n0 = (int)warp_uniform(w->n0), n1 = (int)warp_uniform(w->n1);
+                if (all > 0) {
+                    ok = mbar_wait_warp(qfull, qph);
+                    qph ^= 1;
                 }
-                for (int j = 0; j < all && ok; ++j) {
-                    const int v = wait_full();
-                    int k = -1;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int nt = t == 0 ? n0 : n1;
-                        if (j >= nt || !ok) continue;
-                        ok = mbar_wait_warp(pfull + 8 * t, j & 1);
+                if (WIDE) {
+                    if (all > 0 && ok) {
+                        const int k = wait_full();
+                        if (ok) {
+                            tc_fence_after();
+                            if (n0 > 0) { scores(0, k); tc_commit_by(leader, sfull); }
+                            if (n1 > 0) { scores(1, k); tc_commit_by(leader, sfull + 8); }
+                            tc_commit_by(leader, empty + 8 * k);
+                            if (all == 1) tc_commit_by(leader, qempty);
+                        }
+                    }
+                    for (int j = 0; j < all && ok; ++j) {
+                        const int v = wait_full();
+                        int k = -1;
+    #pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int nt = t == 0 ? n0 : n1;
+                            if (j >= nt || !ok) continue;
+                            weights_there(t);
+                            if (!ok) break;
+                            outputs(t, v, j > 0);
+                            if (j + 1 < nt) {
+                                if (k < 0) k = wait_full();
+                                if (!ok) break;
+                                scores(t, k);
+                            }
+                            tc_commit_by(leader, sfull + 8 * t);
+                        }
+                        if (!ok) break;
+                        tc_commit_by(leader, empty + 8 * v);
+                        if (k >= 0) tc_commit_by(leader, empty + 8 * k);
+                        if (j + 2 == all) tc_commit_by(leader, qempty);   // the queries have been read
+                    }
+                } else {
+                    for (int t = 0; t < 2 && t < all && ok; ++t) {
+                        const int k = wait_full();
                         if (!ok) break;
                         tc_fence_after();
-                        outputs(t, v, j > 0);
-                        if (j + 1 < nt) {
-                            if (k < 0) k = wait_full();
+                        scores(t, k);
+                        tc_commit_by(leader, sfull + 8 * t);
+                        tc_commit_by(leader, empty + 8 * k);
+                        if (t + 1 == all) tc_commit_by(leader, qempty);
+                    }
+                    for (int i = 0; i < all && ok; ++i) {
+                        const int t = i & 1, v = wait_full();
+                        if (ok) weights_there(t);
+                        if (!ok) break;
+                        outputs(t, v, i > 1);
+                        tc_commit_by(leader, empty + 8 * v);
+                        if (i + 2 < all) {
+                            const int k = wait_full();
                             if (!ok) break;
                             scores(t, k);
+                            tc_commit_by(leader, empty + 8 * k);
+                            if (i + 3 == all) tc_commit_by(leader, qempty);
                         }
                         tc_commit_by(leader, sfull + 8 * t);
                     }
-                    if (!ok) break;
-                    tc_commit_by(leader, empty + 8 * v);
-                    if (k >= 0) tc_commit_by(leader, empty + 8 * k);
                 }
-            } else {
-                for (int t = 0; t < 2 && t < all && ok; ++t) {
-                    const int k = wait_full();
-                    if (!ok) break;
-                    scores(t, k);
-                    tc_commit_by(leader, sfull + 8 * t);
-                    tc_commit_by(leader, empty + 8 * k);
-                }
-                for (int i = 0; i < all && ok; ++i) {
-                    const int t = i & 1, v = wait_full();
-                    ok = ok && mbar_wait_warp(pfull + 8 * t, (i >> 1) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    outputs(t, v, i > 1);
-                    tc_commit_by(leader, empty + 8 * v);
-                    if (i + 2 < all) {
-                        const int k = wait_full();
-                        if (!ok) break;
-                        scores(t, k);
-                        tc_commit_by(leader, empty + 8 * k);
-                    }
-                    tc_commit_by(leader, sfull + 8 * t);
-                }
+                if (!ok) break;
+                work_done();
             }
-        } else {
-            const int t = warp >> 2, r = tid & 127, steps = t == 0 ? n0 : n1;
-            const unsigned quarter = (unsigned)((warp & 3) * 32) << 16;
-            const unsigned s_at = tmem + quarter + L::S_COL + t * KT, o_at = tmem + quarter + L::O_COL + t * D;
-            const int head0 = r % p.share, token = first + (WIDE ? t * tile_tok : 0) + r / p.share;      // of this thread's row
-            const int tile_first = first + (WIDE ? t * tile_tok : 0);
-            const bool mine = r < tile_tok * p.share && token < s.nq;
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(SOFTMAX_REGS));
+        const int t = warp >> 2, r = tid & 127;
+        const unsigned quarter = (unsigned)((warp & 3) * 32) << 16;
+        const unsigned s_at = tmem + quarter + L::S_COL + t * KT, o_at = tmem + quarter + L::O_COL + t * D;
+        const int head0 = r % p.share, row_token = r / p.share;
+        const bool in_tile = r < tile_tok * p.share;
+        const bool turned = p.scale_log2 <= 0.f;                      // the largest score is not the largest product
+        const float scale = turned ? 1.f : p.scale_log2;
+        int sph = 0;
+        unsigned loads = 0;                                           // stages that the items before took
+        while (Work *w = next_work()) {
+            const Sequence s = w->s;
+            const int j0 = w->j0, all = w->all, n0 = w->n0, n1 = w->n1, steps = t == 0 ? n0 : n1;
+            const int tile_first = w->first + (WIDE ? t * tile_tok : 0), token = tile_first + row_token;      // of this thread's row
+            const bool mine = in_tile && token < s.nq;
             const int lim = mine ? sees(s, token, a.causal) : 0;
-            const int least = tile_first < s.nq ? min(sees(s, tile_first, a.causal), min(s.bad, s.nk)) : 0;      // keys that all its rows see
             const int seen = min(s.nk, s.bad);                        // what lies behind is nobody's
+            const int least = tile_first < s.nq ? min(sees(s, tile_first, a.causal), seen) : 0;      // keys that all its rows see
             const bool busy = __any_sync(0xffffffffu, mine);
-            const bool turned = p.scale_log2 <= 0.f;                  // the largest score is not the largest product
-            const float scale = turned ? 1.f : p.scale_log2;
             float m = -INFINITY, sum = 0.f;
             for (int i = 0; i < steps; ++i) {
                 const int j = j0 + (WIDE ? i : 2 * i + t), k0 = j * KT;
                 const bool part = k0 + KT > least;
-                if (!mbar_wait_warp(sfull + 8 * t, i & 1)) { ok = false; break; }
+                if (!mbar_wait_warp(sfull + 8 * t, sph)) { ok = false; break; }
+                sph ^= 1;
                 tc_fence_after();
                 // the values of a tile that not every row sees; behind the scores, which came behind the last use of the stage before this one
                 if (part) {
-                    const int rel = j - j0, load = WIDE ? 2 * rel + 1 : rel == all - 1 ? 2 * all - 1 : 2 * rel + 2, stage = load % NST;
+                    const unsigned rel = j - j0, load = loads + (WIDE ? 2 * rel + 1 : rel == (unsigned)all - 1 ? 2 * all - 1 : 2 * rel + 2), stage = load % NST;
                     if (!mbar_wait_warp(full + 8 * stage, (load / NST) & 1)) { ok = false; break; }
-                    if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r) && k0 + r < seen) { atomicMin(&odd_first, k0 + r); atomicMax(&odd_last, k0 + r); }
+                    if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r) && k0 + r < seen) { atomicMin(&w->odd_first, k0 + r); atomicMax(&w->odd_last, k0 + r); }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
                 if (busy) {
@@ -373,15 +447,15 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                     for (int c = 0; c < KT; c += 32) {
-                        unsigned w[16];
+                        unsigned v[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             float2 y = fma2(make_float2(x[c + e], x[c + e + 1]), scale2, off2);
                             y.x = ex2_ftz(y.x); y.y = ex2_ftz(y.y);
                             sums[(e >> 1) & 1] = add2(sums[(e >> 1) & 1], y);
-                            w[e >> 1] = pack_pair(T(), y.x, y.y);
+                            v[e >> 1] = pack_pair(T(), y.x, y.y);
                         }
-                        tc_st16(s_at + c / 2, w);
+                        tc_st16(s_at + c / 2, v);
                     }
                     sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                     tc_wait_st();
@@ -389,65 +463,66 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 tc_fence_before();
                 mbar_arrive(pfull + 8 * t);
             }
-            if (ok && steps > 0) ok = mbar_wait_warp(sfull + 8 * t, steps & 1);      // the outputs are complete
-            tc_fence_after();
-            float *const handover = reinterpret_cast<float *>(smem_dyn + (base + L::KV0 - (unsigned)__cvta_generic_to_shared(smem_dyn)));
-            float other = 0.f, own = 1.f;                             // what the two halves' sums count
-            bool join = false;
-            if (!WIDE) {
-                asm volatile("bar.sync 1, 256;\n" ::: "memory");      // the other half's products have read the stages too
-                if (t == 1) {
-                    if (busy && steps > 0) {
-                        handed[r] = make_float2(m, sum);
-#pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            tc_ld32(o_at + c, o);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) handover[(c + e) * ROWS + r] = o[e];
-                        }
-                    }
-                    asm volatile("bar.sync 1, 256;\n" ::: "memory");
-                } else {
-                    asm volatile("bar.sync 1, 256;\n" ::: "memory");
-                    join = n1 > 0;
-                    if (join && busy) {
-                        const float2 h = handed[r];
-                        const float now = fmaxf(m, h.x), from = now == -INFINITY ? 0.f : now;
-                        own = exp2f(m - from); other = exp2f(h.x - from);
-                        sum = sum * own + h.y * other;
-                        m = now;
-                    }
-                }
+            loads += 2 * all;
+            if (ok && steps > 0) {                                    // the outputs are complete
+                ok = mbar_wait_warp(sfull + 8 * t, sph);
+                sph ^= 1;
             }
-            if ((WIDE || t == 0) && busy && ok) {
-                const int head = group * p.share + head0, from = j0 * KT;
-                const bool none = lim <= from, lost = lim > min(bad_page, s.bad);
+            tc_fence_after();
+            float own = 1.f, other = 0.f;                             // what the accumulators' sums count: this row tile's, or the even and the odd key tiles'
+            if (!WIDE) {
+                auto meet = [&](int i) {                              // of all 256 threads, bounded like every wait
+                    mbar_arrive(pair + 8 * i);
+                    ok = mbar_wait_warp(pair + 8 * i, turn & 1) && ok;
+                };
+                handed[t][r] = m;
+                tc_fence_before();
+                meet(0);                                              // both are complete
+                tc_fence_after();
+                const float even = handed[0][r], odd = n1 > 0 ? handed[1][r] : -INFINITY;
+                m = fmaxf(even, odd);
+                const float from = m == -INFINITY ? 0.f : m;
+                own = exp2f(even - from); other = n1 > 0 ? exp2f(odd - from) : 0.f;
+                meet(1);
+                handed[t][r] = sum;
+                meet(2);
+                sum = handed[0][r] * own + (n1 > 0 ? handed[1][r] * other : 0.f);
+            }
+            if (busy && ok) {
+                const int head = w->group * p.share + head0;
+                const bool none = lim <= j0 * KT, lost = lim > min(w->bad_page, s.bad), split = w->parts > 1;
                 const float nan = __int_as_float(0x7fffffff);
                 const long long row = (long long)(s.q0 + token) * a.heads + head;
-                const long long at = (long long)blockIdx.x * (tok * p.share) + (WIDE ? t * tile_tok * p.share : 0) + r;
-                const float inv = none ? 0.f : lost ? nan : it.parts > 1 && sum == 0.f ? 0.f : 1.f / sum;
-                const int odd0 = odd_first, odd1 = odd_last;
+                const long long at = (long long)w->index * (tok * p.share) + (WIDE ? t * tile_tok * p.share : 0) + r;
+                const float inv = none ? 0.f : lost ? nan : split && sum == 0.f ? 0.f : 1.f / sum;
+                const int odd0 = w->odd_first, odd1 = w->odd_last;
+                // WIDE: all channels of this tile's row; otherwise each warpgroup half of them
+                constexpr int WIDTH = WIDE ? D : D / 2;
 #pragma unroll 1
-                for (int c = 0; c < D && c < a.dim; c += 32) {
+                for (int c = WIDE ? 0 : t * WIDTH; c < (WIDE ? D : (t + 1) * WIDTH) && c < a.dim; c += 32) {
                     float o[32];
-                    if (steps > 0) {
-                        tc_ld32(o_at + c, o);
-                        tc_wait_ld();
+                    if (all > 0) tc_ld32(WIDE ? o_at + c : tmem + quarter + L::O_COL + c, o);
+                    tc_wait_ld();
+                    if (!WIDE) {
+                        if (n1 > 0) {
+                            float q[32];
+                            tc_ld32(tmem + quarter + L::O_COL + D + c, q);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = fmaf(q[e], other, o[e] * own);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] *= own;
+                        }
                     }
                     if (!mine) continue;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        o[e] = none || steps == 0 ? 0.f : o[e] * own;
-                        if (!WIDE && join && !none) o[e] = fmaf(handover[(c + e) * ROWS + r], other, o[e]);
-                        o[e] = none ? 0.f : o[e] * inv;
-                    }
+                    for (int e = 0; e < 32; ++e) o[e] = none || (WIDE ? steps : all) == 0 ? (none ? 0.f : inv) : o[e] * inv;
                     if (odd1 >= 0 && !none && sum != 0.f) {           // rare: values that are not finite and that this row sees
                         for (int k = odd0; k <= min(lim - 1, odd1); ++k) {
-                            const T *v = key_row<T>(a, s, it.b, k, a.value, a.value_strides);
+                            const T *v = key_row<T>(a, s, w->b, k, a.value, a.value_strides);
                             if (v == nullptr) continue;
-                            v += group * a.value_strides[1] + c;
+                            v += w->group * a.value_strides[1] + c;
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
                                 const float f = c + e < a.dim ? to_acc(v[e]) : 0.f;
@@ -455,7 +530,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                             }
                         }
                     }
-                    if (it.parts == 1) {
+                    if (!split) {
                         store_row(static_cast<T *>(a.out) + row * a.dim + c, o, a.dim - c);
                     } else {
                         float *to = p.part + at * a.dim + c;
@@ -464,12 +539,19 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                             if (e < a.dim - c) *reinterpret_cast<float4 *>(to + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     }
                 }
-                if (mine) {
-                    const float log = none || (it.parts > 1 && sum == 0.f) ? -INFINITY : lost || sum == 0.f ? nan : m + log2f(sum);
-                    if (it.parts > 1) p.part_lse[at] = lost ? nan : log;
+                if (mine && (WIDE || t == 0)) {
+                    const float log = none || (split && sum == 0.f) ? -INFINITY : lost || sum == 0.f ? nan : m + log2f(sum);
+                    if (split) p.part_lse[at] = lost ? nan : log;
                     else if (a.lse != nullptr) a.lse[row] = log * 0.6931471805599453f;
                 }
             }
+            tc_fence_before();
+            if (!WIDE) {
+                mbar_arrive(pair + 24);
+                ok = mbar_wait_warp(pair + 24, turn & 1) && ok;       // both accumulators, and what was handed, have been read
+            }
+            if (!ok) break;
+            work_done();
         }
     }
     if (!ok) atomicExch(&g_wait_timeout, 1);

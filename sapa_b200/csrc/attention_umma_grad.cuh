@@ -21,6 +21,8 @@ namespace umg {
 
 using namespace um;
 
+constexpr int THREADS = 10 * 32;
+
 template <int D> struct KeyLay {
     static constexpr int TILE_BYTES = D / 64 * BLOCK_BYTES, NST = D == 64 ? 3 : 2;
     static constexpr int K0 = 0, V0 = TILE_BYTES, Q0 = 2 * TILE_BYTES, O0 = Q0 + NST * TILE_BYTES, END = O0 + NST * TILE_BYTES;
@@ -61,7 +63,7 @@ template <typename T> __device__ __forceinline__ void store_packed(unsigned tadd
 }  // namespace umg
 
 template <typename T, int D>
-__global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_keys_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap omap,
+__global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_keys_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap omap,
                                                                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                                              const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     using namespace umg;
@@ -96,14 +98,14 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_keys_kernel(con
         tc_relinquish();
     }
     // rows that no copy fills: they are behind P and dS, which are 0 there
-    for (int i = tid; i < (ROWS - rows) * 8 * (D / 64) * 2 * NST; i += NT) {
+    for (int i = tid; i < (ROWS - rows) * 8 * (D / 64) * 2 * NST; i += THREADS) {
         const int tile = i / ((ROWS - rows) * 8), e = i % ((ROWS - rows) * 8);
         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(base + L::Q0 + tile * BLOCK_BYTES + (rows + e / 8) * 128 + (e % 8) * 16), "r"(0u) : "memory");
     }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     begin_after_previous();
     if (warp == 0) {
-        const Item r = block_at<false>(a, blockIdx.x / a.groups, lane, KeyBlocks{a.causal != 0, tok, KT});
+        const Item r = InOrder<false, KeyBlocks>(a, KeyBlocks{a.causal != 0, tok, KT}, lane).at(blockIdx.x / a.groups);
         if (lane == 0) item = r;
     }
     tc_fence_before();
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_keys_kernel(con
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_queries_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap omap,
+__global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_queries_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap omap,
                                                                                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                                                 const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     using namespace umg;
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_queries_kernel(
     }
     begin_after_previous();
     if (warp == 0) {
-        const Item r = block_at<true>(a, blockIdx.x / a.groups, lane, QueryBlocks{a.causal != 0, tok, KT});
+        const Item r = InOrder<true, QueryBlocks>(a, QueryBlocks{a.causal != 0, tok, KT}, lane).at(blockIdx.x / a.groups);
         if (lane == 0) item = r;
     }
     tc_fence_before();

@@ -210,6 +210,23 @@ def test_paged(new, keys, heads, groups, dim, page, layout, dtype):
         check(sapa_b200.paged_attention(q, c.key, c.value, c.table, c.lengths, offsets_of(new), causal=False, scale=0.1), want["out"], want["out_tol"])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_items_to_a_block(dim, dtype):
+    """More sequences than SMs, of one to eight tiles of keys, and few sequences whose keys are split into parts of that many: every
+    block goes through several items of every length."""
+    for new, keys, groups in (([1] * 160, [1 + 7 * i % 1000 for i in range(160)], 4), ([3 + i % 40 for i in range(90)], [60 + 11 * i % 900 for i in range(90)], 4),
+                              ([300 + 13 * i for i in range(20)], [300 + 13 * i for i in range(20)], 4), ([1], [8192], 8), ([2, 1], [6000, 800], 2), ([200], [5000], 4)):
+        q, k, v = _inputs(sum(new), sum(keys), 2 * groups, groups, dim, TYPES[dtype])
+        c = Cache(k, v, keys, 16)
+        want = oracle.packed(q, k, v, new, keys, True, dim ** -0.5)
+        for _ in range(2):
+            check(sapa_b200.paged_attention(q, c.key, c.value, c.table, c.lengths, offsets_of(new)), want["out"], want["out_tol"])
+            check(sapa_b200.packed_attention(q, k, v, offsets_of(new), offsets_of(keys)), want["out"], want["out_tol"])
+    from sapa_b200 import _lib
+    assert _lib.wait_timeout_flags("cuda") == 0
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("page", [16, 24, 128])
 def test_pages_outside_the_cache(page, dtype):
