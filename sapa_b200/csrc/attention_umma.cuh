@@ -25,11 +25,12 @@ namespace um {
 using namespace ummau;
 
 constexpr int KT = TILE, ROWS = 128, BLOCK_BYTES = 128 * 128;         // keys of a tile, rows of a tile; 128 rows of 64 channels
-constexpr int MMA_WARP = 8, LOAD_WARP = 9, PLAN_WARP = 10, NT = 12 * 32;
+constexpr int MMA_WARP = 8, LOAD_WARP = 9, PLAN_WARP = 10, VALUE_WARP = 11, NT = 12 * 32;
 // registers a thread: 168 at launch, then what the softmax needs for a row of scores and the other four warps for theirs (multiples of 8)
 constexpr int REGS = 168, SOFTMAX_REGS = 208, OTHER_REGS = 88;
 static_assert(8 * 32 * SOFTMAX_REGS + 4 * 32 * OTHER_REGS <= NT * REGS, "a block draws on what it was launched with");
 constexpr unsigned HI = (1024u >> 4) | (1u << 14) | (2u << 29);       // 8 rows of 128 bytes, descriptor version 1, 128-byte swizzle
+constexpr int BY_FMA = 1, BY_FMA_OF = 4;                              // exponentials that the FMA units take over
 constexpr float GROWTH = 8.f;                                         // powers of two
 
 // 2 row tiles: as many stages as fit beside them
@@ -38,6 +39,11 @@ template <int D, bool WIDE> struct Lay {
     static constexpr int Q0 = 0, KV0 = Q_BYTES;
     static constexpr int NEED = KV0 + NST * STAGE + 1024, SMEM = NEED < 120 * 1024 ? 120 * 1024 : NEED;      // one block an SM: tensor memory
     static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
+    // place in the order of loads of an item's tile, of `all`
+    static __device__ __forceinline__ unsigned stage_of(int tile, int all, bool keys) {
+        if (WIDE) return 2 * tile + (keys ? 0 : 1);
+        return keys ? (tile == 0 ? 0 : 2 * tile - 1) : (tile == all - 1 ? 2 * all - 1 : 2 * tile + 2);
+    }
     static_assert(SMEM <= 225 * 1024 && NST >= 3, "shared memory");      // with the 2 KB that a block holds besides
 };
 
@@ -84,6 +90,36 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// the largest of three, NaN if one of them is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x without the unit that ex2 keeps busy: x = n + f with n the nearest whole number, 2^f by a polynomial with the least relative error over [-1/2, 1/2]
+// (1.0e-4 in degree 3, a fortieth of bfloat16's half step; 2.8e-6 in degree 4 for float16) that is 1 at 0, and n added to its exponent.  0 from 2^-127 down;
+// what a NaN gives is not one, so a row with a NaN has to be found by its maximum.
+template <typename T> __device__ __forceinline__ float2 ex2_by_fma(float2 x) {
+    constexpr float ROUND = 12582912.f;                               // 1.5 * 2^23: adding it leaves whole numbers
+    x.x = fmaxf(x.x, -127.f); x.y = fmaxf(x.y, -127.f);
+    const float2 t = add2(x, make_float2(ROUND, ROUND)), n = add2(t, make_float2(-ROUND, -ROUND)), f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 y;
+    if constexpr (std::is_same<T, __half>::value) {
+        y = fma2(f, make_float2(0.009582843631505966f, 0.009582843631505966f), make_float2(0.055906426161527634f, 0.055906426161527634f));
+        y = fma2(f, y, make_float2(0.24024099111557007f, 0.24024099111557007f));
+        y = fma2(f, y, make_float2(0.6931241750717163f, 0.6931241750717163f));
+    } else {
+        y = fma2(f, make_float2(0.055008865892887115f, 0.055008865892887115f), make_float2(0.2422109693288803f, 0.2422109693288803f));
+        y = fma2(f, y, make_float2(0.693282961845398f, 0.693282961845398f));
+    }
+    y = fma2(f, y, make_float2(1.f, 1.f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap *map, unsigned bar, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
@@ -127,14 +163,14 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
     using L = um::Lay<D, WIDE>;
     constexpr int NST = L::NST;
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) unsigned long long bars[2 + 2 * NST + 4 + 4 + 4];
+    __shared__ __align__(8) unsigned long long bars[2 + 2 * NST + 6 + 4 + 4];
     __shared__ unsigned tmem_slot;
     __shared__ Work queue[2];
     __shared__ float handed[WIDE ? 1 : 2][ROWS];                      // maximum, then sum, of the even and the odd tiles
     const sapa_attention &a = p.a;
     const unsigned base = ((unsigned)__cvta_generic_to_shared(smem_dyn) + 1023u) & ~1023u;
     const unsigned qfull = (unsigned)__cvta_generic_to_shared(bars), qempty = qfull + 8, full = qempty + 8, empty = full + 8 * NST, sfull = empty + 8 * NST, pfull = sfull + 16;
-    const unsigned posted = pfull + 16, taken = posted + 16, pair = taken + 16;
+    const unsigned posted = pfull + 32, taken = posted + 16, pair = taken + 16;
     const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
     const int tile_tok = ROWS / p.share, tok = WIDE ? 2 * tile_tok : tile_tok;
 
@@ -142,7 +178,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
         if (lane == 0) {
             mbar_init(qfull, 1); mbar_init(qempty, 1);
             for (int i = 0; i < NST; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
-            for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 128); mbar_init(posted + 8 * i, 1); mbar_init(taken + 8 * i, 10); }
+            for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 16 * i, 128); mbar_init(pfull + 16 * i + 8, 128); mbar_init(posted + 8 * i, 1); mbar_init(taken + 8 * i, 11); }
             for (int i = 0; i < 4; ++i) mbar_init(pair + 8 * i, 256);
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
@@ -188,7 +224,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                         // key tiles of the two accumulators: [j0, j0 + n[t]) each (WIDE), or every other one
                         w.j0 = r.it.part * (r.it.parts > 1 ? r.tiles : 0);
                         int n[2];
-    #pragma unroll
+#pragma unroll
                         for (int t = 0; t < 2; ++t) {
                             const int last = min(w.first + (WIDE ? (t + 1) * tile_tok : tile_tok), w.s.nq) - 1;      // its last token
                             const bool some = last >= w.first + (WIDE ? t * tile_tok : 0);
@@ -207,43 +243,26 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 __syncwarp();
                 if (!w.there) break;
             }
-        } else if (warp == LOAD_WARP) {
-            int st = 0, ph = 0, qph = 0;
+        } else if (warp == LOAD_WARP || warp == VALUE_WARP) {
+            // keys (and queries) by one warp, values by the other: a box a page takes its time.  They share the ring of stages in the order in which the products
+            // take them.  WIDE: K0, V0, K1, V1, ...; otherwise K0, K1, V0, K2, V1, ...: the scores are a tile further ahead.
+            const bool keys = warp == LOAD_WARP;
+            const CUtensorMap *const map = keys ? &kmap : &vmap;
+            int qph = 0;
+            unsigned loads = 0;                                       // stages that the items before took
             const int boxes = PAGED ? max(1, KT / a.page) : 1, box_rows = KT / boxes;
+            unsigned last = 0;                                        // the last stage of this warp's, and one
             while (Work *w = next_work()) {
                 const int j0 = w->j0, all = w->all, b = w->b, group = w->group;
                 const Sequence s = w->s;
-                const int used = min(s.bad, s.nk);                        // positions that the table has pages for
-                // entries of the table for a tile, each lane one: -1 behind the keys.  Looked at only in load(), so that they are on their way till then.
+                const int used = min(s.bad, s.nk);                    // positions that the table has pages for
+                // entries of the table for a tile, each lane one.  Looked at only when they are used, so that they are on their way till then.
                 auto page_of = [&](int j) {
                     const int at = j * KT + lane * box_rows;
                     return !PAGED || lane >= boxes || j >= j0 + all || at >= used ? -1 : a.page_table[(long long)b * a.max_pages + (unsigned)at / (unsigned)a.page];
                 };
-                auto load = [&](const CUtensorMap *map, int j, int page) {
-                    const int at = j * KT + lane * box_rows;
-                    const bool mine = PAGED && lane < boxes && at < used;
-                    const unsigned there = PAGED ? __ballot_sync(0xffffffffu, mine) : 1u;
-                    if (mine && (unsigned)page >= (unsigned)a.pages) { atomicMin(&w->bad_page, at); page = 0; }
-                    __syncwarp();
-                    bool can = true;
-                    if (lane == 0) {
-                        can = mbar_wait_bounded(empty + 8 * st, ph ^ 1);
-                        if (can) mbar_expect_tx(full + 8 * st, __popc(there) * box_rows * (D / 64) * 128);
-                    }
-                    ok = __shfl_sync(0xffffffffu, can, 0) != 0;
-                    if (!ok) return;
-                    const unsigned dst = base + L::KV0 + st * L::STAGE;
-                    if (PAGED) {
-                        if (mine)
-                            for (int c = 0; c < D / 64; ++c)
-                                tma_load_4d(dst + c * BLOCK_BYTES + lane * box_rows * 128, map, full + 8 * st, 64 * c, group, a.page >= KT ? (unsigned)(j * KT) % (unsigned)a.page : 0, page);
-                    } else if (lane == 0) {
-                        for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * BLOCK_BYTES, map, full + 8 * st, 64 * c, group, s.k0 + j * KT);
-                    }
-                    if (++st == NST) { st = 0; ph ^= 1; }
-                };
-                int page0 = page_of(j0), page1 = page_of(j0 + 1);
-                if (all > 0) {
+                int page = page_of(j0), next = page_of(j0 + 1);
+                if (keys && all > 0) {
                     if (lane == 0) {
                         ok = mbar_wait_bounded(qempty, qph ^ 1);
                         if (ok) {
@@ -256,22 +275,37 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     ok = __shfl_sync(0xffffffffu, ok, 0) != 0;
                     if (!ok) break;
                     qph ^= 1;
-                    load(&kmap, j0, page0);
                 }
-                // WIDE: K0, V0, K1, V1, ...; otherwise K0, K1, V0, K2, V1, ...: the scores are a tile further ahead
                 for (int j = j0; j < j0 + all && ok; ++j) {
-                    const int page2 = page_of(j + 2);
-                    if (WIDE) load(&vmap, j, page0);
-                    if (ok && j + 1 < j0 + all) load(&kmap, j + 1, page1);
-                    if (!WIDE && ok) load(&vmap, j, page0);
-                    page0 = page1; page1 = page2;
+                    const int behind = page_of(j + 2), at = j * KT + lane * box_rows, rel = j - j0;
+                    const unsigned load = loads + L::stage_of(rel, all, keys), st = load % NST, dst = base + L::KV0 + st * L::STAGE;
+                    const bool mine = PAGED && lane < boxes && at < used;
+                    const unsigned there = PAGED ? __ballot_sync(0xffffffffu, mine) : 1u;
+                    if (mine && (unsigned)page >= (unsigned)a.pages) { atomicMin(&w->bad_page, at); page = 0; }
+                    __syncwarp();
+                    if (lane == 0) {
+                        ok = mbar_wait_bounded(empty + 8 * st, ((load / NST) & 1) ^ 1);
+                        if (ok) mbar_expect_tx(full + 8 * st, __popc(there) * box_rows * (D / 64) * 128);
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0) != 0;
+                    if (!ok) break;
+                    if (PAGED) {
+                        if (mine)
+                            for (int c = 0; c < D / 64; ++c)
+                                tma_load_4d(dst + c * BLOCK_BYTES + lane * box_rows * 128, map, full + 8 * st, 64 * c, group, a.page >= KT ? (unsigned)(j * KT) % (unsigned)a.page : 0, page);
+                    } else if (lane == 0) {
+                        for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * BLOCK_BYTES, map, full + 8 * st, 64 * c, group, s.k0 + j * KT);
+                    }
+                    last = load + 1;
+                    page = next; next = behind;
                 }
                 if (!ok) break;
+                loads += 2 * all;
                 work_done();
             }
-            if (!ok && lane == 0) {                                       // none of its loads may land after it has left
-                (void)drain_loads<NST>(full, st, ph);
-                (void)mbar_wait_bounded(qfull, qph ^ 1);
+            if (!ok && lane == 0) {                                   // none of its loads may land after it has left: each, while its stage is waited for again
+                for (unsigned load = last > NST ? last - NST : 0; load < last; ++load) (void)mbar_wait_bounded(full + 8 * (load % NST), (load / NST) & 1);
+                if (keys) (void)mbar_wait_bounded(qfull, qph ^ 1);
             }
         } else if (warp == MMA_WARP) {
             constexpr unsigned IDESC_S = IDESC_M128<T> | idesc_n(KT), IDESC_O = IDESC_M128<T> | (1u << 16) | idesc_n(D);
@@ -287,20 +321,22 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
             };
             auto scores = [&](int t, int stage) {
                 const unsigned q = q_base + (WIDE ? t : 0) * STEP, k = k_base + stage * STEP;
-    #pragma unroll
+#pragma unroll
                 for (int c = 0; c < D / 16; ++c)
                     tc_mma<false>(leader, tmem + L::S_COL + t * KT, q + (c >> 2) * (BLOCK_BYTES >> 4) + (c & 3) * 2, k + (c >> 2) * (BLOCK_BYTES >> 4) + (c & 3) * 2, HI, IDESC_S, c > 0 ? 1u : 0u);
             };
-            auto outputs = [&](int t, int stage, bool add) {
-                const unsigned v = v_base + stage * STEP;
-    #pragma unroll
-                for (int c = 0; c < KT / 16; ++c)
+            auto outputs = [&](int t, int stage, bool add) {              // as its weights come, half a tile at a time
+                const unsigned v = v_base + stage * STEP, parity = t == 0 ? pph0 : pph1;
+#pragma unroll
+                for (int c = 0; c < KT / 16; ++c) {
+                    if (c % (KT / 32) == 0) {
+                        ok = ok && mbar_wait_warp(pfull + 16 * t + 8 * (c / (KT / 32)), parity);
+                        if (!ok) return;
+                        tc_fence_after();
+                    }
                     tc_mma_ta<false>(leader, tmem + L::O_COL + t * D, tmem + L::S_COL + t * KT + c * 8, v + c * (2048 >> 4), HI, IDESC_O, add || c > 0 ? 1u : 0u);
-            };
-            auto weights_there = [&](int t) {
-                ok = ok && mbar_wait_warp(pfull + 8 * t, t == 0 ? pph0 : pph1);
+                }
                 if (t == 0) pph0 ^= 1; else pph1 ^= 1;
-                tc_fence_after();
             };
             while (Work *w = next_work()) {
                 const int all = (int)warp_uniform(w->all), n0 = (int)warp_uniform(w->n0), n1 = (int)warp_uniform(w->n1);
@@ -322,13 +358,12 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     for (int j = 0; j < all && ok; ++j) {
                         const int v = wait_full();
                         int k = -1;
-    #pragma unroll
+#pragma unroll
                         for (int t = 0; t < 2; ++t) {
                             const int nt = t == 0 ? n0 : n1;
                             if (j >= nt || !ok) continue;
-                            weights_there(t);
-                            if (!ok) break;
                             outputs(t, v, j > 0);
+                            if (!ok) break;
                             if (j + 1 < nt) {
                                 if (k < 0) k = wait_full();
                                 if (!ok) break;
@@ -353,9 +388,8 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     }
                     for (int i = 0; i < all && ok; ++i) {
                         const int t = i & 1, v = wait_full();
-                        if (ok) weights_there(t);
+                        if (ok) outputs(t, v, i > 1);
                         if (!ok) break;
-                        outputs(t, v, i > 1);
                         tc_commit_by(leader, empty + 8 * v);
                         if (i + 2 < all) {
                             const int k = wait_full();
@@ -400,7 +434,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 tc_fence_after();
                 // the values of a tile that not every row sees; behind the scores, which came behind the last use of the stage before this one
                 if (part) {
-                    const unsigned rel = j - j0, load = loads + (WIDE ? 2 * rel + 1 : rel == (unsigned)all - 1 ? 2 * all - 1 : 2 * rel + 2), stage = load % NST;
+                    const unsigned load = loads + L::stage_of(j - j0, all, false), stage = load % NST;
                     if (!mbar_wait_warp(full + 8 * stage, (load / NST) & 1)) { ok = false; break; }
                     if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r) && k0 + r < seen) { atomicMin(&w->odd_first, k0 + r); atomicMax(&w->odd_last, k0 + r); }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -421,11 +455,14 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     }
                     float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                    for (int c = 4; c < KT; c += 4)
+                    for (int c = 4; c + 8 <= KT; c += 8)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[c + e]);
-                    const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale);
-                    const bool grown = mine && now > m + GROWTH;      // each row by itself: its bits do not depend on its neighbours
+                        for (int e = 0; e < 4; ++e) top[e] = max3(top[e], x[c + e], x[c + 4 + e]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = max2(top[e], x[KT - 4 + e]);
+                    const float now = max2(m, max2(max2(top[0], top[1]), max2(top[2], top[3])) * scale);
+                    // each row by itself: its bits do not depend on its neighbours.  A NaN goes on into all its weights.
+                    const bool grown = mine && !(now <= m + GROWTH);
                     if (i == 0) {
                         m = now;
                     } else if (__any_sync(0xffffffffu, grown)) {
@@ -451,17 +488,25 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             float2 y = fma2(make_float2(x[c + e], x[c + e + 1]), scale2, off2);
-                            y.x = ex2_ftz(y.x); y.y = ex2_ftz(y.y);
+                            if ((e >> 1) % BY_FMA_OF < BY_FMA) y = ex2_by_fma<T>(y);
+                            else y = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
                             sums[(e >> 1) & 1] = add2(sums[(e >> 1) & 1], y);
                             v[e >> 1] = pack_pair(T(), y.x, y.y);
                         }
                         tc_st16(s_at + c / 2, v);
+                        if (c == KT / 2 - 32) {                       // the second product can begin with the first half
+                            tc_wait_st();
+                            tc_fence_before();
+                            mbar_arrive(pfull + 16 * t);
+                        }
                     }
                     sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                     tc_wait_st();
+                } else {
+                    mbar_arrive(pfull + 16 * t);
                 }
                 tc_fence_before();
-                mbar_arrive(pfull + 8 * t);
+                mbar_arrive(pfull + 16 * t + 8);
             }
             loads += 2 * all;
             if (ok && steps > 0) {                                    // the outputs are complete
@@ -469,6 +514,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 sph ^= 1;
             }
             tc_fence_after();
+            if (!(m < INFINITY)) sum = __int_as_float(0x7fffffff);    // infinity less infinity, or a NaN
             float own = 1.f, other = 0.f;                             // what the accumulators' sums count: this row tile's, or the even and the odd key tiles'
             if (!WIDE) {
                 auto meet = [&](int i) {                              // of all 256 threads, bounded like every wait
