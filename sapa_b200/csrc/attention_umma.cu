@@ -94,17 +94,14 @@ int umma_forward(const Args &p, bool wide, long long items, int dtype, cudaStrea
 
 namespace umg {
 
-template <typename T, int D>
-static int launch(const Args &p, const Grads &g, const CUtensorMap &q, const CUtensorMap &o, const CUtensorMap &k, const CUtensorMap &v, long long key_blocks,
-                  long long query_blocks, cudaStream_t st) {
+template <typename T, int D, bool KEYS>
+static int launch(const Args &p, const Grads &g, const CUtensorMap &own0, const CUtensorMap &own1, const CUtensorMap &over0, const CUtensorMap &over1, long long items,
+                  cudaStream_t st) {
     int sms = 0;
-    constexpr int KEYS = KeyLay<D>::SMEM, QUERIES = QueryLay<D>::SMEM;
-    if (int e = prepare_launch((const void *)sapa_attention_umma_keys_kernel<T, D>, KEYS, "sapa_attention_umma_keys_kernel", sms)) return e;
-    if (int e = prepare_launch((const void *)sapa_attention_umma_queries_kernel<T, D>, QUERIES, "sapa_attention_umma_queries_kernel", sms)) return e;
-    launch_next(sapa_attention_umma_keys_kernel<T, D>, dim3((unsigned)key_blocks), dim3(umg::THREADS), KEYS, st, q, o, k, v, p, g);
-    if (int e = check_launch("sapa_attention_umma_keys_kernel")) return e;
-    launch_next(sapa_attention_umma_queries_kernel<T, D>, dim3((unsigned)query_blocks), dim3(umg::THREADS), QUERIES, st, q, o, k, v, p, g);
-    return check_launch("sapa_attention_umma_queries_kernel");
+    constexpr int SMEM = umg::Lay<D>::SMEM;
+    if (int e = prepare_launch((const void *)sapa_attention_umma_grad_kernel<T, D, KEYS>, SMEM, "sapa_attention_umma_grad_kernel", sms)) return e;
+    launch_next(sapa_attention_umma_grad_kernel<T, D, KEYS>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), SMEM, st, own0, own1, over0, over1, p, g, (int)items);
+    return check_launch(KEYS ? "sapa_attention_umma_grad_kernel<keys>" : "sapa_attention_umma_grad_kernel<queries>");
 }
 
 }  // namespace umg
@@ -113,19 +110,31 @@ int umma_backward(const Args &p, const Grads &g, int dtype, cudaStream_t st) {
     using namespace um;
     const sapa_attention &a = p.a;
     const bool half = dtype == SAPA_F16;
-    CUtensorMap q, o, k, v;
-    const int tok = ROWS / p.share, qb[2] = {p.share, tok}, kb[2] = {1, KT};
+    const int tok = ROWS / p.share, at_once = p.share < umg::N ? p.share : umg::N, few = umg::N / at_once;
     const long long qd[2] = {a.heads, a.tokens}, qs[2] = {a.query_strides[1], a.query_strides[0]}, os[2] = {g.go_strides[1], g.go_strides[0]};
     const long long kd[2] = {a.groups, a.keys}, ks[2] = {a.key_strides[1], a.key_strides[0]}, vs[2] = {a.value_strides[1], a.value_strides[0]};
-    const bool good = encode(&q, a.query, a.dim, 2, qd, qs, qb, half) && encode(&o, g.go, a.dim, 2, qd, os, qb, half) &&
-                      encode(&k, a.key, a.dim, 2, kd, ks, kb, half) && encode(&v, a.value, a.dim, 2, kd, vs, kb, half);
+    const long long key_items = most_blocks(a, a.keys, KT) * a.groups, query_items = most_blocks(a, a.tokens, tok) * a.groups;
+    SAPA_REQUIRE(key_items < 0x3fffffffll && query_items < 0x3fffffffll, SAPA_ERR_UNSUPPORTED, "sapa_attention_backward: too many blocks");
+    if (key_items == 0 || query_items == 0) return SAPA_OK;           // no sequence
+    // the operands as an item holds them (128 rows) and as another goes over them (64)
+    CUtensorMap q[2], o[2], k[2], v[2];
+    bool good = true;
+    for (int i = 0; i < 2; ++i) {
+        const int qb[2] = {i == 0 ? p.share : at_once, i == 0 ? tok : few}, kb[2] = {1, i == 0 ? KT : umg::N};
+        good = good && encode(&q[i], a.query, a.dim, 2, qd, qs, qb, half) && encode(&o[i], g.go, a.dim, 2, qd, os, qb, half) &&
+               encode(&k[i], a.key, a.dim, 2, kd, ks, kb, half) && encode(&v[i], a.value, a.dim, 2, kd, vs, kb, half);
+    }
     SAPA_REQUIRE(good, SAPA_ERR_LAUNCH, "sapa_attention_backward: cuTensorMapEncodeTiled failed (%d)", last_encode_result());
-    const long long key_blocks = most_blocks(a, a.keys, KT) * a.groups, query_blocks = most_blocks(a, a.tokens, tok) * a.groups;
-    SAPA_REQUIRE(key_blocks < 0x7fffffffll && query_blocks < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "sapa_attention_backward: too many blocks");
-    if (key_blocks == 0 || query_blocks == 0) return SAPA_OK;         // no sequence
-    if (half) return a.dim <= 64 ? umg::launch<__half, 64>(p, g, q, o, k, v, key_blocks, query_blocks, st) : umg::launch<__half, 128>(p, g, q, o, k, v, key_blocks, query_blocks, st);
-    return a.dim <= 64 ? umg::launch<__nv_bfloat16, 64>(p, g, q, o, k, v, key_blocks, query_blocks, st)
-                       : umg::launch<__nv_bfloat16, 128>(p, g, q, o, k, v, key_blocks, query_blocks, st);
+    auto run = [&](auto t, auto d) -> int {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value;
+        if (int e = umg::launch<T, D, true>(p, g, k[0], v[0], q[1], o[1], key_items, st)) return e;
+        return umg::launch<T, D, false>(p, g, q[0], o[0], k[1], v[1], query_items, st);
+    };
+    using Narrow = std::integral_constant<int, 64>;
+    using Wide = std::integral_constant<int, 128>;
+    if (half) return a.dim <= 64 ? run(__half(), Narrow()) : run(__half(), Wide());
+    return a.dim <= 64 ? run(__nv_bfloat16(), Narrow()) : run(__nv_bfloat16(), Wide());
 }
 
 // Flag of this family's bounded waits on the current device, cleared when it was raised; -1: it cannot be read.

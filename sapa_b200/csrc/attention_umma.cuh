@@ -124,25 +124,28 @@ __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-// Replaces what is not finite in a row of a landed tile (128 rows of D channels) with 0; whether there was any.
+// Replaces what is not finite in 128 bytes of a row of a landed tile with 0; whether there was any.
+template <typename T> __device__ __forceinline__ bool clean_line(unsigned line, int row) {
+    bool any = false;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {                                     // in another order in every row: no two on the same banks
+        const unsigned at = line + ((c ^ (row & 7)) << 4);
+        unsigned v[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+        if (!finite::all_finite<T, 4>(v)) {
+            any = true;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = finite::or_zero<T>(v[e]);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+        }
+    }
+    return any;
+}
+// The same for a row of a tile of 128 rows
 template <typename T, int D> __device__ __forceinline__ bool clean_row(unsigned tile, int row) {
     bool any = false;
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) {
-        const unsigned line = tile + b * BLOCK_BYTES + row * 128;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {                                 // in another order in every row: no two on the same banks
-            const unsigned at = line + ((c ^ (row & 7)) << 4);
-            unsigned v[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
-            if (!finite::all_finite<T, 4>(v)) {
-                any = true;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = finite::or_zero<T>(v[e]);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-            }
-        }
-    }
+    for (int b = 0; b < D / 64; ++b) any = clean_line<T>(tile + b * BLOCK_BYTES + row * 128, row) || any;
     return any;
 }
 // 32 channels of a row of the output from float32, those below `left`
