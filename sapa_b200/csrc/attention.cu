@@ -36,6 +36,18 @@ template <> __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
     const uint2 u = *reinterpret_cast<const uint2 *>(p);
     return widen(*reinterpret_cast<const __nv_bfloat162 *>(&u.x), *reinterpret_cast<const __nv_bfloat162 *>(&u.y));
 }
+// 8 elements, 0 where they are not `there`
+__device__ __forceinline__ void load8(const float *p, bool there, float4 (&v)[2]) {
+    v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (there) { v[0] = load4(p); v[1] = load4(p + 4); }
+}
+template <typename T> __device__ __forceinline__ void load8(const T *p, bool there, float4 (&v)[2]) {
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (there) raw = *reinterpret_cast<const uint4 *>(p);
+    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    v[0] = widen(*reinterpret_cast<const P *>(&raw.x), *reinterpret_cast<const P *>(&raw.y));
+    v[1] = widen(*reinterpret_cast<const P *>(&raw.z), *reinterpret_cast<const P *>(&raw.w));
+}
 __device__ __forceinline__ void store4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
 __device__ __forceinline__ bool finite4(float4 v) { return isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w); }
 __device__ __forceinline__ float at(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -96,26 +108,51 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
                       (long long)(group * p.share + r % p.share) * a.query_strides[1] + c);
         store4(sm + L::Q0 + r * L::QS + c, v);
     }
+    // a tile's keys and values, by way of registers: all pages first, then all rows; of narrow blocks while the tile before is at work
+    constexpr int EACH = KT * (DP / 4) / NT;
+    constexpr bool AHEAD = RI == 1;
+    float4 kr[EACH], vr[EACH];
+    auto fetch = [&](int k0) {
+        const int n = min(KT, (int)upto - k0);
+        long long key_at[EACH], value_at[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int e = tid + i * NT, r = e / (DP / 4), position = k0 + r;
+            key_at[i] = -1;
+            if (r >= n || e % (DP / 4) * 4 >= D) continue;
+            long long row = s.k0 + position, page = 0;
+            if (a.page_table != nullptr) {
+                const unsigned at = (unsigned)position / (unsigned)a.page;
+                page = a.page_table[(long long)it.b * a.max_pages + at];
+                row = position - (int)(at * a.page);
+                if ((unsigned long long)page >= (unsigned)a.pages) { atomicMin(&bad_page, position); continue; }
+            }
+            key_at[i] = row * a.key_strides[0] + page * a.key_strides[2];
+            value_at[i] = row * a.value_strides[0] + page * a.value_strides[2];
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            kr[i] = vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (key_at[i] < 0) continue;
+            const int c = (tid + i * NT) % (DP / 4) * 4;
+            kr[i] = load4(static_cast<const T *>(a.key) + key_at[i] + group * a.key_strides[1] + c);
+            vr[i] = load4(static_cast<const T *>(a.value) + value_at[i] + group * a.value_strides[1] + c);
+        }
+    };
+    if (AHEAD && from < upto) fetch((int)from);
     for (int k0 = (int)from; k0 < upto; k0 += KT) {
         const int n = min(KT, (int)upto - k0);
         bool odd = false;
+        if (!AHEAD) fetch(k0);
         __syncthreads();
-        for (int e = tid; e < KT * (DP / 4); e += NT) {
-            const int r = e / (DP / 4), c = e % (DP / 4) * 4;
-            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-            if (r < n && c < D) {
-                const T *kp = key_row<T>(a, s, it.b, k0 + r, a.key, a.key_strides), *vp = key_row<T>(a, s, it.b, k0 + r, a.value, a.value_strides);
-                if (kp == nullptr) {
-                    atomicMin(&bad_page, k0 + r);
-                } else {
-                    k = load4(kp + group * a.key_strides[1] + c);
-                    v = load4(vp + group * a.value_strides[1] + c);
-                }
-            }
-            odd = odd || !finite4(v);
-            store4(sm + L::K0 + r * L::QS + c, k);
-            store4(sm + L::V0 + r * DP + c, v);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int e = tid + i * NT, r = e / (DP / 4), c = e % (DP / 4) * 4;
+            odd = odd || !finite4(vr[i]);
+            store4(sm + L::K0 + r * L::QS + c, kr[i]);
+            store4(sm + L::V0 + r * DP + c, vr[i]);
         }
+        if (AHEAD && k0 + KT < upto) fetch(k0 + KT);
         // a value that a row does not see must not reach it, not even as 0 * infinity
         const bool careful = __syncthreads_or(odd && k0 + KT > least);
         float sc[RI][4];
@@ -277,35 +314,46 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------------------------- backward
-// delta, and what lies outside the sequences: 16 lanes per token and head, 8 channels each.  Reads grad_out and out once, which bounds it.
+// delta, and what lies outside the sequences: 16 lanes per token and head, 8 channels each, two rows on their way at once.  Reads grad_out and out once, which
+// bounds it.
 template <typename T>
 __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     const sapa_attention &a = p.a;
+    constexpr int AT_ONCE = 2;
     const int lane = threadIdx.x & 15, c = 8 * lane, D = a.dim;
     begin_after_previous();
-    const long long n = (long long)a.tokens * a.heads, all = (long long)gridDim.x * 16;
-    for (long long row0 = (long long)blockIdx.x * 16; row0 < n; row0 += all) {
-        const long long row = row0 + (threadIdx.x >> 4);
-        const long long t = row / a.heads;
-        const int h = (int)(row % a.heads);
-        float sum = 0.f;
-        if (row < n && c < D) {
-            const T *o = static_cast<const T *>(a.out) + row * D + c, *y = static_cast<const T *>(g.go) + t * g.go_strides[0] + h * g.go_strides[1] + c;
+    const long long n = (long long)a.tokens * a.heads;
+    for (long long base = (long long)blockIdx.x * (16 * AT_ONCE); base < n; base += (long long)gridDim.x * (16 * AT_ONCE)) {
+        const long long row0 = base + (threadIdx.x >> 4);
+        float4 u[AT_ONCE][2], v[AT_ONCE][2];
+        unsigned t[AT_ONCE], h[AT_ONCE];
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const float4 u = rows::load4(o + e), v = rows::load4(y + e);
-                sum = fmaf(u.w, v.w, fmaf(u.z, v.z, fmaf(u.y, v.y, fmaf(u.x, v.x, sum))));
-            }
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const long long row = row0 + 16 * i;
+            t[i] = n <= 0x7fffffff ? (unsigned)row / (unsigned)a.heads : (unsigned)(row / a.heads);
+            h[i] = (unsigned)(row - (long long)t[i] * a.heads);
+            const bool there = row < n && c < D;
+            const T *o = static_cast<const T *>(a.out) + row * D + c, *y = static_cast<const T *>(g.go) + t[i] * g.go_strides[0] + h[i] * g.go_strides[1] + c;
+            rows::load8(o, there, u[i]);
+            rows::load8(y, there, v[i]);
         }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane != 0 || row >= n) continue;
-        if (g.nlse != nullptr) {
-            const long long at = ((long long)(h / p.share) * a.tokens + t) * p.share + h % p.share;
-            g.delta[at] = sum;
-            g.nlse[at] = -1.4426950408889634f * a.lse[row];
-        } else {
-            g.delta[row] = sum;
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const long long row = row0 + 16 * i;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                sum = fmaf(u[i][e].w, v[i][e].w, fmaf(u[i][e].z, v[i][e].z, fmaf(u[i][e].y, v[i][e].y, fmaf(u[i][e].x, v[i][e].x, sum))));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane != 0 || row >= n) continue;
+            if (g.nlse != nullptr) {
+                const long long at = ((long long)(h[i] / p.share) * a.tokens + t[i]) * p.share + h[i] % p.share;
+                g.delta[at] = sum;
+                g.nlse[at] = -1.4426950408889634f * a.lse[row];
+            } else {
+                g.delta[row] = sum;
+            }
         }
     }
     clear_outside(static_cast<T *>(g.gq), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
@@ -315,18 +363,21 @@ __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_
 
 namespace grad {
 using namespace rows;
-constexpr int N = 64, WS = N + 4;             // rows and keys of a tile
+constexpr int OWN = 32, OVER = 64, THREADS = 128, WS = OWN + 4;      // rows or keys of a block, of a tile that it goes over
 template <int DP> struct Lay {
     static constexpr int XS = DP + 4;
-    static constexpr int Q0 = 0, O0 = N * XS, K0 = 2 * N * XS, V0 = 3 * N * XS, P0 = 4 * N * XS, S0 = P0 + N * WS, L0 = S0 + N * WS, END = L0 + 2 * N;
+    static constexpr int A0 = 0, A1 = OWN * XS, B0 = 2 * OWN * XS, B1 = B0 + OVER * XS, P0 = B1 + OVER * XS, S0 = P0 + OVER * WS, L0 = S0 + OVER * WS, END = L0 + 2 * OVER;
     static constexpr size_t SMEM = (size_t)END * sizeof(float);
 };
 }  // namespace grad
 
-// float32.  KEYS: gradients of 64 keys and values, over the rows that see them; otherwise those of 64 query rows, over the keys that they see.  P and dS of
-// a tile are formed again from the scores, lse and delta: P = 2^(s - lse), dS = P (dP - delta); no atomics.
+// float32.  KEYS: gradients of 32 keys and values, over the rows (token x head of a key head) that see them; otherwise those of 32 query rows, over the keys
+// that they see.  P and dS of a tile are formed again from the scores, lse and delta: P = 2^(s - lse), dS = P (dP - delta); no atomics.  128 threads as 8 x 16:
+// of S and dP the rows ty + 8 i and the columns tx + 16 j, of the sums the rows 4 ty + i and the channels 4 tx + 64 j.  Blocks of 32, so that
+// small problems have one for every SM (256 threads on 64 rows: 1342 tokens, 8 heads of 64 channels, 209 us for the keys and 92 for the queries).
+// What bounds it: the FP32 pipe.
 template <int DP, bool KEYS>
-__global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
+__global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     using namespace grad;
     using T = float;
     using L = grad::Lay<DP>;
@@ -334,62 +385,63 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(cons
     __shared__ Item item;
     const sapa_attention &a = p.a;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.dim;
-    const int share = p.share, heads_at_once = min(share, N), tok = N / heads_at_once;       // of a row tile; more heads than rows: in turns
-    const int turns = KEYS ? (share + N - 1) / N : 1;
-    const int slots = KEYS ? a.groups : a.groups * ((share + N - 1) / N);
-    const int slot = blockIdx.x % slots, group = KEYS ? slot : slot % a.groups;
+    constexpr int ROWS = KEYS ? OVER : OWN;                                                   // of a tile of rows
+    const int share = p.share, at_once = min(share, ROWS), tok = ROWS / at_once, turns = (share + at_once - 1) / at_once;      // more heads than rows: in turns
+    const int slots = KEYS ? a.groups : a.groups * turns, slot = blockIdx.x % slots, group = slot % a.groups;
     begin_after_previous();
     if (tid < 32) {
-        const Item r = KEYS ? InOrder<false, KeyBlocks>(a, KeyBlocks{a.causal != 0, tok, N}, tid).at(blockIdx.x / slots)
-                            : InOrder<true, QueryBlocks>(a, QueryBlocks{a.causal != 0, tok, N}, tid).at(blockIdx.x / slots);
+        const Item r = KEYS ? InOrder<false, KeyBlocks>(a, KeyBlocks{a.causal != 0, tok, OWN}, tid).at(blockIdx.x / slots)
+                            : InOrder<true, QueryBlocks>(a, QueryBlocks{a.causal != 0, tok, OVER}, tid).at(blockIdx.x / slots);
         if (tid == 0) item = r;
     }
     __syncthreads();
     if (!item.there) return;
-    const int b = item.b, block = item.block;
-    const Sequence s = sequence_at(a, b);
+    const Sequence s = sequence_at(a, item.b);
 
-    auto load_keys = [&](int k0) {             // returns whether something is not finite among the keys
+    // rows of tokens from i0, heads from h0: r -> token i0 + r / at_once, head h0 + r % at_once
+    auto load = [&](int to0, int to1, int rows, bool keys, int k0, int i0, int h0, int used) {      // returns whether something is not finite
         bool odd = false;
-        for (int e = tid; e < N * (DP / 4); e += NT) {
-            const int r = e / (DP / 4), c = e % (DP / 4) * 4;
-            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-            if (k0 + r < s.nk && c < D) {
-                k = load4(static_cast<const T *>(a.key) + (long long)(s.k0 + k0 + r) * a.key_strides[0] + group * a.key_strides[1] + c);
-                v = load4(static_cast<const T *>(a.value) + (long long)(s.k0 + k0 + r) * a.value_strides[0] + group * a.value_strides[1] + c);
-            }
-            odd = odd || !finite4(k);
-            store4(sm + L::K0 + r * L::XS + c, k);
-            store4(sm + L::V0 + r * L::XS + c, v);
-        }
-        return odd;
-    };
-    auto load_queries = [&](int i0, int h0, int used) {
-        bool odd = false;
-        for (int e = tid; e < N * (DP / 4); e += NT) {
-            const int r = e / (DP / 4), c = e % (DP / 4) * 4;
-            float4 q = make_float4(0.f, 0.f, 0.f, 0.f), o = q;
-            if (r < used) {
-                const long long t = s.q0 + i0 + r / heads_at_once, h = group * share + h0 + r % heads_at_once;
-                if (c < D && h0 + r % heads_at_once < share) {
-                    q = load4(static_cast<const T *>(a.query) + t * a.query_strides[0] + h * a.query_strides[1] + c);
-                    o = load4(static_cast<const T *>(g.go) + t * g.go_strides[0] + h * g.go_strides[1] + c);
+        constexpr int MOST = OVER * (DP / 4) / THREADS;
+        float4 u[MOST / 2], v[MOST / 2];
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {                        // of the tile, each with all its loads on their way at once
+            const int from = half * rows / 2;
+#pragma unroll
+            for (int i = 0; i < MOST / 2; ++i) {
+                const int e = tid + i * THREADS, r = from + e / (DP / 4), c = e % (DP / 4) * 4;
+                u[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r >= from + rows / 2 || c >= D) continue;
+                if (keys) {
+                    if (k0 + r >= s.nk) continue;
+                    u[i] = load4(static_cast<const T *>(a.key) + (long long)(s.k0 + k0 + r) * a.key_strides[0] + group * a.key_strides[1] + c);
+                    v[i] = load4(static_cast<const T *>(a.value) + (long long)(s.k0 + k0 + r) * a.value_strides[0] + group * a.value_strides[1] + c);
+                } else {
+                    if (r >= used || h0 + r % at_once >= share) continue;
+                    const long long t = s.q0 + i0 + r / at_once, h = group * share + h0 + r % at_once;
+                    u[i] = load4(static_cast<const T *>(a.query) + t * a.query_strides[0] + h * a.query_strides[1] + c);
+                    v[i] = load4(static_cast<const T *>(g.go) + t * g.go_strides[0] + h * g.go_strides[1] + c);
                 }
             }
-            odd = odd || !finite4(q) || !finite4(o);
-            store4(sm + L::Q0 + r * L::XS + c, q);
-            store4(sm + L::O0 + r * L::XS + c, o);
-        }
-        for (int r = tid; r < N; r += NT) {
-            float e = 0.f, d = 0.f;
-            if (r < used && h0 + r % heads_at_once < share) {
-                const long long at = (long long)(s.q0 + i0 + r / heads_at_once) * a.heads + group * share + h0 + r % heads_at_once;
-                e = a.lse[at] * 1.4426950408889634f;
-                d = g.delta[at];
+#pragma unroll
+            for (int i = 0; i < MOST / 2; ++i) {
+                const int e = tid + i * THREADS, r = from + e / (DP / 4), c = e % (DP / 4) * 4;
+                if (r >= from + rows / 2) continue;
+                odd = odd || !finite4(u[i]) || (!keys && !finite4(v[i]));
+                store4(sm + to0 + r * L::XS + c, u[i]);
+                store4(sm + to1 + r * L::XS + c, v[i]);
             }
-            sm[L::L0 + r] = e;
-            sm[L::L0 + N + r] = d;
         }
+        if (!keys)
+            for (int r = tid; r < rows; r += THREADS) {
+                float e = 0.f, d = 0.f;
+                if (r < used && h0 + r % at_once < share) {
+                    const long long at = (long long)(s.q0 + i0 + r / at_once) * a.heads + group * share + h0 + r % at_once;
+                    e = a.lse[at] * 1.4426950408889634f;
+                    d = g.delta[at];
+                }
+                sm[L::L0 + r] = e;
+                sm[L::L0 + OVER + r] = d;
+            }
         return odd;
     };
     float x[4][DP / 16], y[4][DP / 16];        // KEYS: of values, of keys; otherwise y: of queries
@@ -400,66 +452,55 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(cons
 
     // a tile: rows of tokens from i0, heads from h0; keys from k0
     auto tile = [&](int i0, int h0, int used, int k0, bool odd) {
-        int lim[4];
-        bool whole = true;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = ty + 16 * i;
-            lim[i] = r < used && h0 + r % heads_at_once < share ? sees(s, i0 + r / heads_at_once, a.causal) : 0;
-            whole = whole && (lim[i] >= k0 + N);
-        }
+        auto limit = [&](int r) { return r < used && h0 + r % at_once < share ? sees(s, i0 + r / at_once, a.causal) - k0 : 0; };      // keys of the tile that a row sees
         const bool careful = __syncthreads_or(odd);
         float sc[4][4], dp[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) sc[i][j] = dp[i][j] = 0.f;
-#pragma unroll 1
+#pragma unroll 2
         for (int c = 0; c < DP; c += 4) {
-            float4 k[4], v[4];
+            float4 u[4], v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                k[j] = *reinterpret_cast<const float4 *>(sm + L::K0 + (tx + 16 * j) * L::XS + c);
-                v[j] = *reinterpret_cast<const float4 *>(sm + L::V0 + (tx + 16 * j) * L::XS + c);
+                u[j] = *reinterpret_cast<const float4 *>(sm + L::B0 + (tx + 16 * j) * L::XS + c);
+                v[j] = *reinterpret_cast<const float4 *>(sm + L::B1 + (tx + 16 * j) * L::XS + c);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float4 q = *reinterpret_cast<const float4 *>(sm + L::Q0 + (ty + 16 * i) * L::XS + c);
-                const float4 o = *reinterpret_cast<const float4 *>(sm + L::O0 + (ty + 16 * i) * L::XS + c);
+                const float4 m = *reinterpret_cast<const float4 *>(sm + L::A0 + (ty + 8 * i) * L::XS + c);
+                const float4 n = *reinterpret_cast<const float4 *>(sm + L::A1 + (ty + 8 * i) * L::XS + c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    sc[i][j] = fmaf(q.w, k[j].w, fmaf(q.z, k[j].z, fmaf(q.y, k[j].y, fmaf(q.x, k[j].x, sc[i][j]))));
-                    dp[i][j] = fmaf(o.w, v[j].w, fmaf(o.z, v[j].z, fmaf(o.y, v[j].y, fmaf(o.x, v[j].x, dp[i][j]))));
+                    sc[i][j] = fmaf(m.w, u[j].w, fmaf(m.z, u[j].z, fmaf(m.y, u[j].y, fmaf(m.x, u[j].x, sc[i][j]))));
+                    dp[i][j] = fmaf(n.w, v[j].w, fmaf(n.z, v[j].z, fmaf(n.y, v[j].y, fmaf(n.x, v[j].x, dp[i][j]))));
                 }
             }
         }
+        int lim[4];                            // of the rows that this thread has
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = ty + 16 * i;
-            const float lse = sm[L::L0 + r], delta = sm[L::L0 + N + r];
+        for (int i = 0; i < 4; ++i) lim[i] = limit(KEYS ? tx + 16 * i : ty + 8 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int k = tx + 16 * j;
-                const float w = k0 + k < lim[i] ? exp2f(fmaf(sc[i][j], p.scale_log2, -lse)) : 0.f;
-                const float ds = k0 + k < lim[i] ? w * (dp[i][j] - delta) : 0.f;
-                if (KEYS) {
-                    sm[L::P0 + r * WS + k] = w;
-                    sm[L::S0 + r * WS + k] = ds;
-                } else {
-                    sm[L::S0 + k * WS + r] = ds;
-                }
+                const int own = ty + 8 * i, over = tx + 16 * j, r = KEYS ? over : own, k = KEYS ? own : over;
+                const bool seen = k < lim[KEYS ? j : i];
+                const float w = seen ? exp2f(fmaf(sc[i][j], p.scale_log2, -sm[L::L0 + r])) : 0.f;
+                if (KEYS) sm[L::P0 + over * WS + own] = w;
+                sm[L::S0 + over * WS + own] = seen ? w * (dp[i][j] - sm[L::L0 + OVER + r]) : 0.f;
             }
-        }
         __syncthreads();
         if (!careful) {
 #pragma unroll 2
-            for (int n = 0; n < N; ++n) {      // rows (KEYS) or keys
+            for (int n = 0; n < OVER; ++n) {
                 const float4 w = KEYS ? *reinterpret_cast<const float4 *>(sm + L::P0 + n * WS + 4 * ty) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const float4 ds = *reinterpret_cast<const float4 *>(sm + L::S0 + n * WS + 4 * ty);
 #pragma unroll
                 for (int j = 0; j < DP / 64; ++j) {
-                    const float4 f = *reinterpret_cast<const float4 *>(sm + (KEYS ? L::Q0 : L::K0) + n * L::XS + 4 * tx + 64 * j);
-                    const float4 o = KEYS ? *reinterpret_cast<const float4 *>(sm + L::O0 + n * L::XS + 4 * tx + 64 * j) : f;
+                    const float4 f = *reinterpret_cast<const float4 *>(sm + L::B0 + n * L::XS + 4 * tx + 64 * j);
+                    const float4 o = KEYS ? *reinterpret_cast<const float4 *>(sm + L::B1 + n * L::XS + 4 * tx + 64 * j) : f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -470,40 +511,39 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(cons
                 }
             }
         } else {                               // what is not seen must not reach a gradient, not even as 0 * infinity
-            for (int n = 0; n < N; ++n)
+            for (int n = 0; n < OVER; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = KEYS ? n : 4 * ty + i, k = KEYS ? 4 * ty + i : n;
-                    if (r >= used || h0 + r % heads_at_once >= share || k0 + k >= sees(s, i0 + r / heads_at_once, a.causal)) continue;
+                    if ((KEYS ? 4 * ty + i : n) >= limit(KEYS ? n : 4 * ty + i)) continue;
 #pragma unroll
                     for (int c = 0; c < DP / 16; ++c) {
                         const int col = 4 * tx + 64 * (c >> 2) + (c & 3);
-                        if (KEYS) x[i][c] = fmaf(sm[L::P0 + n * WS + 4 * ty + i], sm[L::O0 + n * L::XS + col], x[i][c]);
-                        y[i][c] = fmaf(sm[L::S0 + n * WS + 4 * ty + i], sm[(KEYS ? L::Q0 : L::K0) + n * L::XS + col], y[i][c]);
+                        if (KEYS) x[i][c] = fmaf(sm[L::P0 + n * WS + 4 * ty + i], sm[L::B1 + n * L::XS + col], x[i][c]);
+                        y[i][c] = fmaf(sm[L::S0 + n * WS + 4 * ty + i], sm[L::B0 + n * L::XS + col], y[i][c]);
                     }
                 }
         }
     };
 
+    const int first = item.block * (KEYS ? OWN : tok);                // key or token
     if (KEYS) {
-        const int k0 = block * N;
-        load_keys(k0);
-        const int from = a.causal ? (int)max(0ll, (long long)k0 - s.nk + s.nq) : 0;      // the first token that sees one of them
+        load(L::A0, L::A1, OWN, true, first, 0, 0, 0);
+        const int from = a.causal ? (int)max(0ll, (long long)first - s.nk + s.nq) : 0;      // the first token that sees one of them
         for (int i0 = from; i0 < s.nq; i0 += tok)
             for (int turn = 0; turn < turns; ++turn) {
-                const int used = min(tok, s.nq - i0) * heads_at_once;
+                const int used = min(tok, s.nq - i0) * at_once;
                 __syncthreads();
-                const bool odd = load_queries(i0, turn * N, used);
-                tile(i0, turn * N, used, k0, odd);
+                const bool odd = load(L::B0, L::B1, OVER, false, 0, i0, turn * at_once, used);
+                tile(i0, turn * at_once, used, first, odd);
             }
     } else {
-        const int i0 = block * tok, h0 = slot / a.groups * N, used = min(tok, s.nq - i0) * heads_at_once;
-        const int most = sees(s, i0 + used / heads_at_once - 1, a.causal);
-        load_queries(i0, h0, used);
-        for (int k0 = 0; k0 < most; k0 += N) {
+        const int h0 = slot / a.groups * at_once, used = min(tok, s.nq - first) * at_once;
+        const int most = sees(s, first + used / at_once - 1, a.causal);
+        load(L::A0, L::A1, OWN, false, 0, first, h0, used);
+        for (int k0 = 0; k0 < most; k0 += OVER) {
             __syncthreads();
-            const bool odd = load_keys(k0);
-            tile(i0, h0, used, k0, odd);
+            const bool odd = load(L::B0, L::B1, OVER, true, k0, 0, 0, 0);
+            tile(first, h0, used, k0, odd);
         }
     }
     // the scores' scale is in the gradients of queries and keys
@@ -512,12 +552,12 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_grad_kernel(cons
         const int n = 4 * ty + i;
         long long row;
         if (KEYS) {
-            if (block * N + n >= s.nk) continue;
-            row = (long long)(s.k0 + block * N + n) * a.groups + group;
+            if (first + n >= s.nk) continue;
+            row = (long long)(s.k0 + first + n) * a.groups + group;
         } else {
-            const int i0 = block * tok, h = slot / a.groups * N + n % heads_at_once;
-            if (n >= min(tok, s.nq - i0) * heads_at_once || h >= share) continue;
-            row = (long long)(s.q0 + i0 + n / heads_at_once) * a.heads + group * share + h;
+            const int h = slot / a.groups * at_once + n % at_once;
+            if (n >= min(tok, s.nq - first) * at_once || h >= share) continue;
+            row = (long long)(s.q0 + first + n / at_once) * a.heads + group * share + h;
         }
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
@@ -617,6 +657,8 @@ static Shape shape_of(const Args &p, int dtype, int sms) {
         // single tokens and short chunks: 16 rows a block, as long as an average sequence has no more
         s.narrow = p.share <= 16 && (long long)a.tokens * p.share <= 16ll * a.B;
         s.bm = s.narrow ? 16 : 128;
+        // few blocks of 128 rows: of 32, before keys are split (1342 tokens of 515-token sequences, 8 heads of 64 channels, float32: 80 us with 128 and split keys)
+        if (!s.narrow && p.share <= 32 && most_blocks(a, a.tokens, 128 / p.share) * a.groups < 2ll * sms) s.bm = 32;
         s.tok = s.bm / p.share;
     }
     s.blocks = most_blocks(a, a.tokens, s.tok) * a.groups;
@@ -649,7 +691,7 @@ template <int DP, bool KEYS> static int run_grad(const Args &p, const Grads &g, 
     int sms = 0;
     if (blocks == 0) return SAPA_OK;
     if (int e = tmau::prepare_launch((const void *)sapa_attention_rows_grad_kernel<DP, KEYS>, (int)L::SMEM, "sapa_attention_rows_grad_kernel", sms)) return e;
-    launch_next(sapa_attention_rows_grad_kernel<DP, KEYS>, dim3((unsigned)blocks), dim3(rows::NT), L::SMEM, st, p, g);
+    launch_next(sapa_attention_rows_grad_kernel<DP, KEYS>, dim3((unsigned)blocks), dim3(grad::THREADS), L::SMEM, st, p, g);
     return check_launch(KEYS ? "sapa_attention_rows_grad_kernel<keys>" : "sapa_attention_rows_grad_kernel<queries>");
 }
 
@@ -681,7 +723,7 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
         SAPA_REQUIRE(workspace != nullptr && workspace_bytes >= s.bytes, SAPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, s.bytes, workspace_bytes);
         SAPA_REQUIRE(aligned16(workspace), SAPA_ERR_ALIGNMENT, "%s: the workspace must be 256-byte aligned", fn);
         p.split = s.split;
-        p.least = 2;
+        p.least = s.umma ? 2 : 1;
         p.part = static_cast<float *>(workspace);
         p.part_lse = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.part);
     }
@@ -689,6 +731,7 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
         int e;
         if (s.umma) e = umma_forward(p, !s.narrow, s.grid, dtype, st);
         else if (s.narrow) e = a->dim <= 64 ? run_rows<scalar_t, 1, 64>(p, s, st) : run_rows<scalar_t, 1, 128>(p, s, st);
+        else if (s.bm == 32) e = a->dim <= 64 ? run_rows<scalar_t, 2, 64>(p, s, st) : run_rows<scalar_t, 2, 128>(p, s, st);
         else e = a->dim <= 64 ? run_rows<scalar_t, 8, 64>(p, s, st) : run_rows<scalar_t, 8, 128>(p, s, st);
         if (e != SAPA_OK || s.split == 0) return e;
         launch_next(sapa_attention_join_kernel<scalar_t>, dim3((unsigned)s.blocks, (unsigned)ceil_div(s.rows, 16)), dim3(256), 0, st, p, s.bm, s.tok);
@@ -731,9 +774,9 @@ extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad
             umma ? reinterpret_cast<float *>(static_cast<char *>(workspace) + need / 2) : nullptr};
     int sms = 0;
     if (int e = sm_count(fn, sms)) return e;
-    const long long rows16 = ((long long)a->tokens * a->heads + 15) / 16, delta_grid = rows16 < 16ll * sms ? (rows16 > 0 ? rows16 : 1) : 16ll * sms;
-    const int slots = (p.share + grad::N - 1) / grad::N, tok = grad::N / (p.share < grad::N ? p.share : grad::N);
-    const long long key_blocks = most_blocks(*a, a->keys, grad::N) * a->groups, query_blocks = most_blocks(*a, a->tokens, tok) * a->groups * slots;
+    const long long rows32 = ((long long)a->tokens * a->heads + 31) / 32, delta_grid = rows32 < (1ll << 20) ? rows32 : 1ll << 20;
+    const int at_once = p.share < grad::OWN ? p.share : grad::OWN, slots = (p.share + at_once - 1) / at_once, tok = grad::OWN / at_once;
+    const long long key_blocks = most_blocks(*a, a->keys, grad::OWN) * a->groups, query_blocks = most_blocks(*a, a->tokens, tok) * a->groups * slots;
     SAPA_REQUIRE(key_blocks < 0x7fffffffll && query_blocks < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
     return SAPA_DISPATCH_FAST(dtype, [&]() -> int {
         launch_next(sapa_attention_delta_kernel<scalar_t>, dim3((unsigned)delta_grid), dim3(256), 0, st, p, g);

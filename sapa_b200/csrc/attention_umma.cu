@@ -43,16 +43,22 @@ static bool encode(CUtensorMap *map, const void *base, int dim, int rank, const 
     return r == CUDA_SUCCESS;
 }
 
+// The warps take registers from one another by numbers that go by those at launch: with others they would wait for ever.
+template <auto *KERNEL> static int check_registers(const char *name) {
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, (const void *)KERNEL) == cudaSuccess ? f.numRegs : -1;
+    }();
+    SAPA_REQUIRE(regs == REGS, SAPA_ERR_LAUNCH, "%s: built with %d registers a thread, not %d", name, regs, REGS);
+    return SAPA_OK;
+}
+
 template <typename T, int D, bool WIDE, bool PAGED>
 static int launch(const Args &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, long long items, cudaStream_t st) {
     using L = um::Lay<D, WIDE>;
     int sms = 0;
     if (int e = prepare_launch((const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED>, L::SMEM, "sapa_attention_umma_kernel", sms)) return e;
-    static const int regs = [] {
-        cudaFuncAttributes f;
-        return cudaFuncGetAttributes(&f, (const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED>) == cudaSuccess ? f.numRegs : -1;
-    }();
-    SAPA_REQUIRE(regs == um::REGS, SAPA_ERR_LAUNCH, "sapa_attention_umma_kernel: built with %d registers, its warps would wait for %d", regs, um::REGS);
+    if (int e = check_registers<sapa_attention_umma_kernel<T, D, WIDE, PAGED>>("sapa_attention_umma_kernel")) return e;
     launch_next(sapa_attention_umma_kernel<T, D, WIDE, PAGED>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), L::SMEM, st, q, k, v, p, (int)items);
     return check_launch(WIDE ? "sapa_attention_umma_kernel<wide>" : "sapa_attention_umma_kernel<narrow>");
 }
@@ -98,8 +104,9 @@ template <typename T, int D, bool KEYS>
 static int launch(const Args &p, const Grads &g, const CUtensorMap &own0, const CUtensorMap &own1, const CUtensorMap &over0, const CUtensorMap &over1, long long items,
                   cudaStream_t st) {
     int sms = 0;
-    constexpr int SMEM = umg::Lay<D>::SMEM;
+    constexpr int SMEM = umg::Lay<D, KEYS>::SMEM;
     if (int e = prepare_launch((const void *)sapa_attention_umma_grad_kernel<T, D, KEYS>, SMEM, "sapa_attention_umma_grad_kernel", sms)) return e;
+    if (int e = um::check_registers<sapa_attention_umma_grad_kernel<T, D, KEYS>>("sapa_attention_umma_grad_kernel")) return e;
     launch_next(sapa_attention_umma_grad_kernel<T, D, KEYS>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), SMEM, st, own0, own1, over0, over1, p, g, (int)items);
     return check_launch(KEYS ? "sapa_attention_umma_grad_kernel<keys>" : "sapa_attention_umma_grad_kernel<queries>");
 }
@@ -110,17 +117,18 @@ int umma_backward(const Args &p, const Grads &g, int dtype, cudaStream_t st) {
     using namespace um;
     const sapa_attention &a = p.a;
     const bool half = dtype == SAPA_F16;
-    const int tok = ROWS / p.share, at_once = p.share < umg::N ? p.share : umg::N, few = umg::N / at_once;
+    const int tok = ROWS / p.share, over_rows = a.dim <= 64 ? umg::Lay<64, true>::TN : umg::Lay<128, true>::TN;      // that keys' items go over
+    const int at_once = p.share < over_rows ? p.share : over_rows, few = over_rows / at_once;
     const long long qd[2] = {a.heads, a.tokens}, qs[2] = {a.query_strides[1], a.query_strides[0]}, os[2] = {g.go_strides[1], g.go_strides[0]};
     const long long kd[2] = {a.groups, a.keys}, ks[2] = {a.key_strides[1], a.key_strides[0]}, vs[2] = {a.value_strides[1], a.value_strides[0]};
     const long long key_items = most_blocks(a, a.keys, KT) * a.groups, query_items = most_blocks(a, a.tokens, tok) * a.groups;
     SAPA_REQUIRE(key_items < 0x3fffffffll && query_items < 0x3fffffffll, SAPA_ERR_UNSUPPORTED, "sapa_attention_backward: too many blocks");
     if (key_items == 0 || query_items == 0) return SAPA_OK;           // no sequence
-    // the operands as an item holds them (128 rows) and as another goes over them (64)
+    // the operands as an item holds them (128 rows) and as another goes over them
     CUtensorMap q[2], o[2], k[2], v[2];
     bool good = true;
     for (int i = 0; i < 2; ++i) {
-        const int qb[2] = {i == 0 ? p.share : at_once, i == 0 ? tok : few}, kb[2] = {1, i == 0 ? KT : umg::N};
+        const int qb[2] = {i == 0 ? p.share : at_once, i == 0 ? tok : few}, kb[2] = {1, i == 0 ? KT : umg::Lay<64, false>::TN};
         good = good && encode(&q[i], a.query, a.dim, 2, qd, qs, qb, half) && encode(&o[i], g.go, a.dim, 2, qd, os, qb, half) &&
                encode(&k[i], a.key, a.dim, 2, kd, ks, kb, half) && encode(&v[i], a.value, a.dim, 2, kd, vs, kb, half);
     }

@@ -102,11 +102,11 @@ __device__ __forceinline__ float max2(float a, float b) {
     return d;
 }
 // 2^x without the unit that ex2 keeps busy: x = n + f with n the nearest whole number, 2^f by a polynomial with the least relative error over [-1/2, 1/2]
-// (1.0e-4 in degree 3, a fortieth of bfloat16's half step; 2.8e-6 in degree 4 for float16) that is 1 at 0, and n added to its exponent.  0 from 2^-127 down;
-// what a NaN gives is not one, so a row with a NaN has to be found by its maximum.
-template <typename T> __device__ __forceinline__ float2 ex2_by_fma(float2 x) {
+// (1.0e-4 in degree 3, a fortieth of bfloat16's half step; 2.8e-6 in degree 4 for float16) that is 1 at 0, and n added to its exponent.  0 from 2^-127 down.
+// KEEP: NaN for a NaN, at the price of a product by 2^n; otherwise it gives a number, and a row with a NaN has to be found by its maximum.
+template <typename T, bool KEEP = false> __device__ __forceinline__ float2 ex2_by_fma(float2 x) {
     constexpr float ROUND = 12582912.f;                               // 1.5 * 2^23: adding it leaves whole numbers
-    x.x = fmaxf(x.x, -127.f); x.y = fmaxf(x.y, -127.f);
+    x.x = KEEP ? max2(x.x, -127.f) : fmaxf(x.x, -127.f); x.y = KEEP ? max2(x.y, -127.f) : fmaxf(x.y, -127.f);
     const float2 t = add2(x, make_float2(ROUND, ROUND)), n = add2(t, make_float2(-ROUND, -ROUND)), f = fma2(n, make_float2(-1.f, -1.f), x);
     float2 y;
     if constexpr (std::is_same<T, __half>::value) {
@@ -118,28 +118,26 @@ template <typename T> __device__ __forceinline__ float2 ex2_by_fma(float2 x) {
         y = fma2(f, y, make_float2(0.693282961845398f, 0.693282961845398f));
     }
     y = fma2(f, y, make_float2(1.f, 1.f));
+    if (KEEP) return mul2(y, make_float2(__int_as_float(0x3f800000 + (__float_as_int(t.x) << 23)), __int_as_float(0x3f800000 + (__float_as_int(t.y) << 23))));
     return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap *map, unsigned bar, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-// Replaces what is not finite in 128 bytes of a row of a landed tile with 0; whether there was any.
+// Replaces what is not finite in 128 bytes of a row of a landed tile with 0; whether there was any.  All are read before they are looked at.
 template <typename T> __device__ __forceinline__ bool clean_line(unsigned line, int row) {
-    bool any = false;
+    unsigned v[32];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {                                     // in another order in every row: no two on the same banks
-        const unsigned at = line + ((c ^ (row & 7)) << 4);
-        unsigned v[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
-        if (!finite::all_finite<T, 4>(v)) {
-            any = true;
+    for (int c = 0; c < 8; ++c)                                       // in another order in every row: no two on the same banks
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[4 * c]), "=r"(v[4 * c + 1]), "=r"(v[4 * c + 2]), "=r"(v[4 * c + 3])
+                     : "r"(line + ((c ^ (row & 7)) << 4)) : "memory");
+    if (finite::all_finite<T, 32>(v)) return false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = finite::or_zero<T>(v[e]);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-        }
-    }
-    return any;
+    for (int c = 0; c < 8; ++c)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(line + ((c ^ (row & 7)) << 4)), "r"(finite::or_zero<T>(v[4 * c])),
+                     "r"(finite::or_zero<T>(v[4 * c + 1])), "r"(finite::or_zero<T>(v[4 * c + 2])), "r"(finite::or_zero<T>(v[4 * c + 3])) : "memory");
+    return true;
 }
 // The same for a row of a tile of 128 rows
 template <typename T, int D> __device__ __forceinline__ bool clean_row(unsigned tile, int row) {
@@ -192,9 +190,12 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
     begin_after_previous();
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
     if (a.lse != nullptr) clear_outside(a.lse, a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    auto meet = [&]() {
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    };
+    if (warp != PLAN_WARP) meet();                                    // that one looks for the first item meanwhile
     const unsigned tmem = warp_uniform(*reinterpret_cast<volatile unsigned *>(&tmem_slot));
     bool ok = true;
     // the block's items one after the other: what all warps but the plans' go through
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     }
                 }
                 w.bad_page = 0x7fffffff; w.odd_first = 0x7fffffff; w.odd_last = -1;
+                if (round == 0) meet();
                 ok = mbar_wait_warp(taken + 8 * (round & 1), ((round >> 1) & 1) ^ 1);
                 if (!ok) break;
                 if (lane == 0) { queue[round & 1] = w; mbar_arrive(posted + 8 * (round & 1)); }
