@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
     }
     // a tile's keys and values, by way of registers: all pages first, then all rows; of narrow blocks while the tile before is at work
     constexpr int EACH = KT * (DP / 4) / NT;
-    constexpr bool AHEAD = RI == 1;
+    constexpr bool AHEAD = RI <= 2;
     float4 kr[EACH], vr[EACH];
     auto fetch = [&](int k0) {
         const int n = min(KT, (int)upto - k0);
@@ -258,21 +258,18 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
 }
 
 // Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(lse_p - max lse).  Grid: a block and group, 16 of its rows; a warp per row, whose
-// lanes first weigh the parts and then take 4 channels each.  Bound by the latency of its few loads; four parts are on their way at once.
+// lanes first weigh the parts and then take 4 channels each, of every part or (up to 64 channels) of every other one.  Bound by the latency of its few
+// loads: eight parts are on their way at once, and the rows' places are found before the forward has ended.
 template <typename T>
 __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_constant__ Args p, int bm, int tok) {
     const sapa_attention &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x % a.groups, D = a.dim;
-    __shared__ Plan shared_plan;
+    const int ways = D <= 64 ? 2 : 1, way = D <= 64 ? lane >> 4 : 0, c = 4 * (D <= 64 ? lane & 15 : lane);
+    // what it reads here came before the forward, which began behind it
+    const Plan plan = split_at<false>(p, blockIdx.x / a.groups, tok, part_tiles(p, tok, lane), lane);
+    const Sequence s = sequence_at(a, plan.it.there ? plan.it.b : 0);
     begin_after_previous();
-    if (warp == 0) {
-        const Plan r = split_at<false>(p, blockIdx.x / a.groups, tok, part_tiles(p, tok, lane), lane);
-        if (lane == 0) shared_plan = r;
-    }
-    __syncthreads();
-    const Plan plan = shared_plan;
     if (!plan.it.there || plan.it.parts == 1) return;
-    const Sequence s = sequence_at(a, plan.it.b);
     const int first = plan.it.block * tok, used = min(tok, s.nq - first) * p.share, parts = plan.it.parts;
     const long long step = (long long)a.groups * bm;                                  // from a part to the next
     for (int r = blockIdx.y * 16 + warp; r < min(used, (int)blockIdx.y * 16 + 16); r += 8) {
@@ -286,29 +283,36 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
         lost = __any_sync(0xffffffffu, lost) || (lim > 0 && top == -INFINITY);
         float sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float *from = p.part + at * D + 4 * lane;
+        const float *from = p.part + at * D + c;
         for (int q0 = 0; q0 < parts; q0 += 32) {
             const float e = q0 + lane < parts ? p.part_lse[at + (q0 + lane) * step] : -INFINITY;
             const float mine = e == -INFINITY ? 0.f : exp2f(e - top);
             const int n = min(32, parts - q0);
-            for (int q = 0; q < n; q += 4) {
-                float4 v[4];
-                float w[4];
+            for (int q = 0; q < n; q += 8 * ways) {
+                float4 v[8];
+                float w[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {                                         // a part that a row sees nothing of counts 0, and holds 0
-                    w[i] = __shfl_sync(0xffffffffu, mine, q + i);
-                    v[i] = q + i < n && 4 * lane < D ? *reinterpret_cast<const float4 *>(from + (q0 + q + i) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < 8; ++i) {                                         // a part that a row sees nothing of counts 0, and holds 0
+                    const int k = q + i * ways + way;
+                    w[i] = __shfl_sync(0xffffffffu, mine, k & 31);
+                    if (k >= n) w[i] = 0.f;
+                    v[i] = k < n && c < D ? *reinterpret_cast<const float4 *>(from + (q0 + k) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     sum += w[i];
                     acc.x = fmaf(w[i], v[i].x, acc.x); acc.y = fmaf(w[i], v[i].y, acc.y); acc.z = fmaf(w[i], v[i].z, acc.z); acc.w = fmaf(w[i], v[i].w, acc.w);
                 }
             }
         }
+        if (ways == 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16); acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
+            acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
+        }
         const float inv = lost ? __int_as_float(0x7fffffff) : lim <= 0 ? 0.f : 1.f / sum;
         const long long row = (long long)(s.q0 + first + r / p.share) * a.heads + group * p.share + r % p.share;
-        if (4 * lane < D) rows::put4(static_cast<T *>(a.out) + row * D + 4 * lane, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (c < D && way == 0) rows::put4(static_cast<T *>(a.out) + row * D + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
         if (a.lse != nullptr && lane == 0) a.lse[row] = lost ? __int_as_float(0x7fffffff) : lim <= 0 ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
     }
 }
@@ -571,13 +575,15 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
 }
 
 // ---------------------------------------------------------------------------------- writing into a paged cache
-// A thread moves 16 bytes of a token's key row and of its value row.  What bounds it: reading and writing them once; for single tokens the launch.
+// A warp takes 2 KB of a token's keys and of its values, all on their way at once: where they go is found once for them.  What bounds it: reading and writing
+// them once; for single tokens the launch.
 __global__ void __launch_bounds__(256) sapa_paged_write_kernel(const __grid_constant__ sapa_paged_rows a, int esize) {
+    constexpr int EACH = 4;
     begin_after_previous();
-    const int chunks = a.dim * esize / 16, per_row = a.groups * chunks;
-    const long long n = (long long)a.tokens * per_row;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const int t = (int)(i / per_row), rest = (int)(i % per_row), group = rest / chunks, c = rest % chunks;
+    const int chunks = a.dim * esize / 16, per_row = a.groups * chunks, lane = threadIdx.x & 31, parts = (per_row + 32 * EACH - 1) / (32 * EACH);
+    const long long n = (long long)a.tokens * parts;
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (long long)gridDim.x * 8) {
+        const int t = (int)(i / parts), part = (int)(i % parts);
         // the first sequence whose end lies behind the token
         int lo = 0, hi = a.B;
         while (lo < hi) {
@@ -589,13 +595,27 @@ __global__ void __launch_bounds__(256) sapa_paged_write_kernel(const __grid_cons
         if (at < 0 || at >= (long long)a.max_pages * a.page) continue;
         const int page = a.page_table[(long long)lo * a.max_pages + at / a.page], slot = (int)(at % a.page);
         if ((unsigned)page >= (unsigned)a.pages) continue;
-        auto move = [&](const void *from, const long long (&fs)[2], void *to, const long long (&ts)[3]) {
-            const char *src = static_cast<const char *>(from) + ((long long)t * fs[0] + group * fs[1]) * esize + 16 * c;
-            char *dst = static_cast<char *>(to) + (page * ts[2] + slot * ts[0] + group * ts[1]) * esize + 16 * c;
-            *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+        auto from = [&](const void *x, const long long (&st)[2], int group, int c) {
+            return reinterpret_cast<const uint4 *>(static_cast<const char *>(x) + ((long long)t * st[0] + group * st[1]) * esize + 16 * c);
         };
-        move(a.key, a.key_strides, a.key_pages, a.key_page_strides);
-        move(a.value, a.value_strides, a.value_pages, a.value_page_strides);
+        auto to = [&](void *x, const long long (&st)[3], int group, int c) {
+            return reinterpret_cast<uint4 *>(static_cast<char *>(x) + (page * st[2] + slot * st[0] + group * st[1]) * esize + 16 * c);
+        };
+        uint4 k[EACH], v[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int x = (part * EACH + e) * 32 + lane, group = x / chunks, c = x - group * chunks;
+            if (x >= per_row) continue;
+            k[e] = *from(a.key, a.key_strides, group, c);
+            v[e] = *from(a.value, a.value_strides, group, c);
+        }
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int x = (part * EACH + e) * 32 + lane, group = x / chunks, c = x - group * chunks;
+            if (x >= per_row) continue;
+            *to(a.key_pages, a.key_page_strides, group, c) = k[e];
+            *to(a.value_pages, a.value_page_strides, group, c) = v[e];
+        }
     }
 }
 
@@ -666,7 +686,7 @@ static Shape shape_of(const Args &p, int dtype, int sms) {
     s.grid = s.blocks;
     // few blocks: their keys are split so that every SM has items
     const long long keys = a.page_table != nullptr ? (long long)a.max_pages * a.page : a.keys;
-    if (s.blocks < 2ll * sms && keys > 2 * TILE) {
+    if (s.blocks < 2ll * sms && keys > (s.umma ? 8 : 2) * TILE) {
         s.split = (s.umma ? 3 : 4) * sms;
         s.grid = s.blocks + s.split;
         s.part = (size_t)s.grid * s.bm * a.dim * sizeof(float);
@@ -723,7 +743,7 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
         SAPA_REQUIRE(workspace != nullptr && workspace_bytes >= s.bytes, SAPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, s.bytes, workspace_bytes);
         SAPA_REQUIRE(aligned16(workspace), SAPA_ERR_ALIGNMENT, "%s: the workspace must be 256-byte aligned", fn);
         p.split = s.split;
-        p.least = s.umma ? 2 : 1;
+        p.least = s.umma ? 4 : 1;
         p.part = static_cast<float *>(workspace);
         p.part_lse = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.part);
     }
@@ -808,7 +828,7 @@ extern "C" int sapa_paged_write(const sapa_paged_rows *a, int dtype, void *strea
     SAPA_REQUIRE(all_aligned16(a->key, a->value, a->key_pages, a->value_pages), SAPA_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", fn);
     int sms = 0;
     if (int e = sm_count(fn, sms)) return e;
-    const long long blocks = ((long long)a->tokens * a->groups * (a->dim * esize / 16) + 255) / 256;
+    const long long warps = (long long)a->tokens * ((a->groups * (a->dim * esize / 16) + 127) / 128), blocks = (warps + 7) / 8;
     launch_next(sapa_paged_write_kernel, dim3((unsigned)(blocks < 16ll * sms ? blocks : 16ll * sms)), dim3(256), 0, static_cast<cudaStream_t>(stream), *a, (int)esize);
     return check_launch("sapa_paged_write_kernel");
 }

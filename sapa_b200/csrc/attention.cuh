@@ -40,7 +40,7 @@ __device__ __forceinline__ Sequence sequence_at(const sapa_attention &a, int b) 
 }
 // keys that token i of the sequence sees
 __device__ __forceinline__ int sees(const Sequence &s, int i, bool causal) {
-    return causal ? (int)min((long long)s.nk, max(0ll, (long long)s.nk - s.nq + i + 1)) : s.nk;
+    return causal ? max(0, s.nk - s.nq + i + 1) : s.nk;      // i < nq
 }
 
 // A block's work: `rows` rows (tokens x query heads of one key head, the heads of a token next to each other) of a sequence.

@@ -464,6 +464,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
             T *const to = KEYS ? static_cast<T *>(values ? g.gv : g.gk) + ((long long)(s.k0 + key) * a.groups + w->group) * a.dim
                                : static_cast<T *>(g.gq) + ((long long)(s.q0 + token) * a.heads + w->group * p.share + r % p.share) * a.dim;
             const int odd0 = w->odd_first, odd1 = w->odd_last;
+            const bool whole = whole_rows(KEYS ? (values ? g.gv : g.gk) : g.gq, a.dim);
 #pragma unroll 1
             for (int c = KEYS ? 0 : t * (D / 2); c < (KEYS ? D : (t + 1) * (D / 2)) && c < a.dim && ok; c += 32) {
                 float o[32];
@@ -471,10 +472,9 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                     tc_ld32(at + c, o);
                     tc_wait_ld();
                 }
-                if (!mine) continue;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = n > 0 && (KEYS || lim > 0) ? o[e] * factor : 0.f;
-                if (odd1 >= 0 && (values || !KEYS)) {                 // rare: what is not finite and was taken out of the products
+                if (odd1 >= 0 && mine && (values || !KEYS)) {         // rare: what is not finite and was taken out of the products
                     for (int i = odd0; i <= odd1; ++i)
                         for (int k = 0; k < (KEYS ? rows : 1); ++k) {
                             const T *v;
@@ -493,7 +493,8 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                             }
                         }
                 }
-                store_row(to + c, o, a.dim - c);
+                __syncwarp();
+                store_rows(to + c, mine, o, a.dim - c, whole);
             }
             tc_fence_before();
             mbar_arrive(accfree);
