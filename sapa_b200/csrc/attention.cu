@@ -367,19 +367,27 @@ __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_
 
 namespace grad {
 using namespace rows;
-constexpr int OWN = 32, OVER = 64, THREADS = 128, WS = OWN + 4;      // rows or keys of a block, of a tile that it goes over
+constexpr int OWN = 32, OVER = 32, TEAM = 128, TEAMS = 4, THREADS = TEAM * TEAMS, WS = OWN + 4;      // rows or keys of a block, of a tile that it goes over
 template <int DP> struct Lay {
     static constexpr int XS = DP + 4;
-    static constexpr int A0 = 0, A1 = OWN * XS, B0 = 2 * OWN * XS, B1 = B0 + OVER * XS, P0 = B1 + OVER * XS, S0 = P0 + OVER * WS, L0 = S0 + OVER * WS, END = L0 + 2 * OVER;
-    static constexpr size_t SMEM = (size_t)END * sizeof(float);
+    static constexpr int A0 = 0, A1 = OWN * XS, LA = 2 * OWN * XS, TEAM0 = LA + 2 * OWN;
+    static constexpr int B0 = 0, B1 = OVER * XS, P0 = 2 * OVER * XS, S0 = P0 + OVER * WS, LB = S0 + OVER * WS, EACH = LB + 2 * OVER;      // of a team
+    static constexpr size_t SMEM = (size_t)(TEAM0 + TEAMS * EACH) * sizeof(float);
+    static_assert(EACH >= 2 * 4 * (DP / 16) * TEAM, "a team's sums are handed over in its tile");
 };
+__device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + team) : "memory"); }
+__device__ __forceinline__ bool team_or(int team, bool v) {
+    unsigned any;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"(1 + team), "r"((unsigned)v) : "memory");
+    return any != 0;
+}
 }  // namespace grad
 
 // float32.  KEYS: gradients of 32 keys and values, over the rows (token x head of a key head) that see them; otherwise those of 32 query rows, over the keys
-// that they see.  P and dS of a tile are formed again from the scores, lse and delta: P = 2^(s - lse), dS = P (dP - delta); no atomics.  128 threads as 8 x 16:
-// of S and dP the rows ty + 8 i and the columns tx + 16 j, of the sums the rows 4 ty + i and the channels 4 tx + 64 j.  Blocks of 32, so that
-// small problems have one for every SM (256 threads on 64 rows: 1342 tokens, 8 heads of 64 channels, 209 us for the keys and 92 for the queries).
-// What bounds it: the FP32 pipe.
+// that they see.  P and dS of a tile of 32 are formed again from the scores, lse and delta: P = 2^(s - lse), dS = P (dP - delta); no atomics.  Four teams of
+// 128 threads take the tiles in turn and add up at the end: a team by itself waits most of the time (1342 tokens, 8 heads of 64 channels: keys 164 us).
+// Threads of a team as 8 x 16: of S and dP the rows ty + 8 i and the columns tx + 16 j, of the sums the rows 4 ty + i and the channels 4 tx + 64 j.
+// What bounds it: the FP32 pipe, in small problems the longest block.
 template <int DP, bool KEYS>
 __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     using namespace grad;
@@ -388,12 +396,13 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
     extern __shared__ __align__(16) float sm[];
     __shared__ Item item;
     const sapa_attention &a = p.a;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.dim;
+    const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, tx = tid & 15, ty = tid >> 4, D = a.dim;
+    float *const mine = sm + L::TEAM0 + team * L::EACH;               // this team's tile
     constexpr int ROWS = KEYS ? OVER : OWN;                                                   // of a tile of rows
     const int share = p.share, at_once = min(share, ROWS), tok = ROWS / at_once, turns = (share + at_once - 1) / at_once;      // more heads than rows: in turns
     const int slots = KEYS ? a.groups : a.groups * turns, slot = blockIdx.x % slots, group = slot % a.groups;
     begin_after_previous();
-    if (tid < 32) {
+    if (threadIdx.x < 32) {
         const Item r = KEYS ? InOrder<false, KeyBlocks>(a, KeyBlocks{a.causal != 0, tok, OWN}, tid).at(blockIdx.x / slots)
                             : InOrder<true, QueryBlocks>(a, QueryBlocks{a.causal != 0, tok, OVER}, tid).at(blockIdx.x / slots);
         if (tid == 0) item = r;
@@ -403,18 +412,17 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
     const Sequence s = sequence_at(a, item.b);
 
     // rows of tokens from i0, heads from h0: r -> token i0 + r / at_once, head h0 + r % at_once
-    auto load = [&](int to0, int to1, int rows, bool keys, int k0, int i0, int h0, int used) {      // returns whether something is not finite
+    auto load = [&](float *to0, float *to1, float *lse, int rows, int me, int threads, bool keys, int k0, int i0, int h0, int used) {      // returns whether something is not finite
         bool odd = false;
-        constexpr int MOST = OVER * (DP / 4) / THREADS;
-        float4 u[MOST / 2], v[MOST / 2];
+        constexpr int AT_ONCE = 4;
+        float4 u[AT_ONCE], v[AT_ONCE];
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {                        // of the tile, each with all its loads on their way at once
-            const int from = half * rows / 2;
+        for (int e0 = 0; e0 < rows * (DP / 4); e0 += AT_ONCE * threads) {
 #pragma unroll
-            for (int i = 0; i < MOST / 2; ++i) {
-                const int e = tid + i * THREADS, r = from + e / (DP / 4), c = e % (DP / 4) * 4;
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int e = e0 + me + i * threads, r = e / (DP / 4), c = e % (DP / 4) * 4;
                 u[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r >= from + rows / 2 || c >= D) continue;
+                if (r >= rows || c >= D) continue;
                 if (keys) {
                     if (k0 + r >= s.nk) continue;
                     u[i] = load4(static_cast<const T *>(a.key) + (long long)(s.k0 + k0 + r) * a.key_strides[0] + group * a.key_strides[1] + c);
@@ -427,24 +435,24 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
                 }
             }
 #pragma unroll
-            for (int i = 0; i < MOST / 2; ++i) {
-                const int e = tid + i * THREADS, r = from + e / (DP / 4), c = e % (DP / 4) * 4;
-                if (r >= from + rows / 2) continue;
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int e = e0 + me + i * threads, r = e / (DP / 4), c = e % (DP / 4) * 4;
+                if (r >= rows) continue;
                 odd = odd || !finite4(u[i]) || (!keys && !finite4(v[i]));
-                store4(sm + to0 + r * L::XS + c, u[i]);
-                store4(sm + to1 + r * L::XS + c, v[i]);
+                store4(to0 + r * L::XS + c, u[i]);
+                store4(to1 + r * L::XS + c, v[i]);
             }
         }
         if (!keys)
-            for (int r = tid; r < rows; r += THREADS) {
+            for (int r = me; r < rows; r += threads) {
                 float e = 0.f, d = 0.f;
                 if (r < used && h0 + r % at_once < share) {
                     const long long at = (long long)(s.q0 + i0 + r / at_once) * a.heads + group * share + h0 + r % at_once;
                     e = a.lse[at] * 1.4426950408889634f;
                     d = g.delta[at];
                 }
-                sm[L::L0 + r] = e;
-                sm[L::L0 + OVER + r] = d;
+                lse[r] = e;
+                lse[rows + r] = d;
             }
         return odd;
     };
@@ -457,54 +465,56 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
     // a tile: rows of tokens from i0, heads from h0; keys from k0
     auto tile = [&](int i0, int h0, int used, int k0, bool odd) {
         auto limit = [&](int r) { return r < used && h0 + r % at_once < share ? sees(s, i0 + r / at_once, a.causal) - k0 : 0; };      // keys of the tile that a row sees
-        const bool careful = __syncthreads_or(odd);
-        float sc[4][4], dp[4][4];
+        const bool careful = team_or(team, odd);
+        float sc[4][2], dp[4][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sc[i][j] = dp[i][j] = 0.f;
+            for (int j = 0; j < 2; ++j) sc[i][j] = dp[i][j] = 0.f;
 #pragma unroll 2
         for (int c = 0; c < DP; c += 4) {
-            float4 u[4], v[4];
+            float4 u[2], v[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u[j] = *reinterpret_cast<const float4 *>(sm + L::B0 + (tx + 16 * j) * L::XS + c);
-                v[j] = *reinterpret_cast<const float4 *>(sm + L::B1 + (tx + 16 * j) * L::XS + c);
+            for (int j = 0; j < 2; ++j) {
+                u[j] = *reinterpret_cast<const float4 *>(mine + L::B0 + (tx + 16 * j) * L::XS + c);
+                v[j] = *reinterpret_cast<const float4 *>(mine + L::B1 + (tx + 16 * j) * L::XS + c);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float4 m = *reinterpret_cast<const float4 *>(sm + L::A0 + (ty + 8 * i) * L::XS + c);
                 const float4 n = *reinterpret_cast<const float4 *>(sm + L::A1 + (ty + 8 * i) * L::XS + c);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 2; ++j) {
                     sc[i][j] = fmaf(m.w, u[j].w, fmaf(m.z, u[j].z, fmaf(m.y, u[j].y, fmaf(m.x, u[j].x, sc[i][j]))));
                     dp[i][j] = fmaf(n.w, v[j].w, fmaf(n.z, v[j].z, fmaf(n.y, v[j].y, fmaf(n.x, v[j].x, dp[i][j]))));
                 }
             }
         }
-        int lim[4];                            // of the rows that this thread has
+        constexpr int HAS = KEYS ? 2 : 4;      // rows that this thread has
+        int lim[HAS];
+        const float *const lse = KEYS ? mine + L::LB : sm + L::LA;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lim[i] = limit(KEYS ? tx + 16 * i : ty + 8 * i);
+        for (int i = 0; i < HAS; ++i) lim[i] = limit(KEYS ? tx + 16 * i : ty + 8 * i);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 const int own = ty + 8 * i, over = tx + 16 * j, r = KEYS ? over : own, k = KEYS ? own : over;
                 const bool seen = k < lim[KEYS ? j : i];
-                const float w = seen ? exp2f(fmaf(sc[i][j], p.scale_log2, -sm[L::L0 + r])) : 0.f;
-                if (KEYS) sm[L::P0 + over * WS + own] = w;
-                sm[L::S0 + over * WS + own] = seen ? w * (dp[i][j] - sm[L::L0 + OVER + r]) : 0.f;
+                const float w = seen ? exp2f(fmaf(sc[i][j], p.scale_log2, -lse[r])) : 0.f;
+                if (KEYS) mine[L::P0 + over * WS + own] = w;
+                mine[L::S0 + over * WS + own] = seen ? w * (dp[i][j] - lse[ROWS + r]) : 0.f;
             }
-        __syncthreads();
+        team_sync(team);
         if (!careful) {
-#pragma unroll 2
+#pragma unroll 4
             for (int n = 0; n < OVER; ++n) {
-                const float4 w = KEYS ? *reinterpret_cast<const float4 *>(sm + L::P0 + n * WS + 4 * ty) : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float4 ds = *reinterpret_cast<const float4 *>(sm + L::S0 + n * WS + 4 * ty);
+                const float4 w = KEYS ? *reinterpret_cast<const float4 *>(mine + L::P0 + n * WS + 4 * ty) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 ds = *reinterpret_cast<const float4 *>(mine + L::S0 + n * WS + 4 * ty);
 #pragma unroll
                 for (int j = 0; j < DP / 64; ++j) {
-                    const float4 f = *reinterpret_cast<const float4 *>(sm + L::B0 + n * L::XS + 4 * tx + 64 * j);
-                    const float4 o = KEYS ? *reinterpret_cast<const float4 *>(sm + L::B1 + n * L::XS + 4 * tx + 64 * j) : f;
+                    const float4 f = *reinterpret_cast<const float4 *>(mine + L::B0 + n * L::XS + 4 * tx + 64 * j);
+                    const float4 o = KEYS ? *reinterpret_cast<const float4 *>(mine + L::B1 + n * L::XS + 4 * tx + 64 * j) : f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -522,8 +532,8 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
 #pragma unroll
                     for (int c = 0; c < DP / 16; ++c) {
                         const int col = 4 * tx + 64 * (c >> 2) + (c & 3);
-                        if (KEYS) x[i][c] = fmaf(sm[L::P0 + n * WS + 4 * ty + i], sm[L::B1 + n * L::XS + col], x[i][c]);
-                        y[i][c] = fmaf(sm[L::S0 + n * WS + 4 * ty + i], sm[L::B0 + n * L::XS + col], y[i][c]);
+                        if (KEYS) x[i][c] = fmaf(mine[L::P0 + n * WS + 4 * ty + i], mine[L::B1 + n * L::XS + col], x[i][c]);
+                        y[i][c] = fmaf(mine[L::S0 + n * WS + 4 * ty + i], mine[L::B0 + n * L::XS + col], y[i][c]);
                     }
                 }
         }
@@ -531,24 +541,49 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
 
     const int first = item.block * (KEYS ? OWN : tok);                // key or token
     if (KEYS) {
-        load(L::A0, L::A1, OWN, true, first, 0, 0, 0);
+        load(sm + L::A0, sm + L::A1, nullptr, OWN, threadIdx.x, THREADS, true, first, 0, 0, 0);
+        __syncthreads();
         const int from = a.causal ? (int)max(0ll, (long long)first - s.nk + s.nq) : 0;      // the first token that sees one of them
-        for (int i0 = from; i0 < s.nq; i0 += tok)
-            for (int turn = 0; turn < turns; ++turn) {
-                const int used = min(tok, s.nq - i0) * at_once;
-                __syncthreads();
-                const bool odd = load(L::B0, L::B1, OVER, false, 0, i0, turn * at_once, used);
-                tile(i0, turn * at_once, used, first, odd);
-            }
+        const int tiles = from < s.nq ? tiles_of(s.nq - from, tok) * turns : 0;
+        for (int i = team; i < tiles; i += TEAMS) {
+            const int i0 = from + i / turns * tok, h0 = i % turns * at_once, used = min(tok, s.nq - i0) * at_once;
+            team_sync(team);
+            const bool odd = load(mine + L::B0, mine + L::B1, mine + L::LB, OVER, tid, TEAM, false, 0, i0, h0, used);
+            tile(i0, h0, used, first, odd);
+        }
     } else {
         const int h0 = slot / a.groups * at_once, used = min(tok, s.nq - first) * at_once;
-        const int most = sees(s, first + used / at_once - 1, a.causal);
-        load(L::A0, L::A1, OWN, false, 0, first, h0, used);
-        for (int k0 = 0; k0 < most; k0 += OVER) {
-            __syncthreads();
-            const bool odd = load(L::B0, L::B1, OVER, true, k0, 0, 0, 0);
-            tile(first, h0, used, k0, odd);
+        const int tiles = tiles_of(sees(s, first + used / at_once - 1, a.causal), OVER);
+        load(sm + L::A0, sm + L::A1, sm + L::LA, OWN, threadIdx.x, THREADS, false, 0, first, h0, used);
+        __syncthreads();
+        for (int i = team; i < tiles; i += TEAMS) {
+            team_sync(team);
+            const bool odd = load(mine + L::B0, mine + L::B1, nullptr, OVER, tid, TEAM, true, i * OVER, 0, 0, 0);
+            tile(first, h0, used, i * OVER, odd);
         }
+    }
+    // the teams' sums, in their order, through their tiles
+    team_sync(team);
+    if (team != 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                mine[(i * (DP / 16) + c) * TEAM + tid] = y[i][c];
+                if (KEYS) mine[(4 * (DP / 16) + i * (DP / 16) + c) * TEAM + tid] = x[i][c];
+            }
+    __syncthreads();
+    if (team != 0) return;
+#pragma unroll 1
+    for (int q = 1; q < TEAMS; ++q) {
+        const float *const other = sm + L::TEAM0 + q * L::EACH;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                y[i][c] += other[(i * (DP / 16) + c) * TEAM + tid];
+                if (KEYS) x[i][c] += other[(4 * (DP / 16) + i * (DP / 16) + c) * TEAM + tid];
+            }
     }
     // the scores' scale is in the gradients of queries and keys
 #pragma unroll
