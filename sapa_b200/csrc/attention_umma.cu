@@ -44,12 +44,12 @@ static bool encode(CUtensorMap *map, const void *base, int dim, int rank, const 
 }
 
 // The warps take registers from one another by numbers that go by those at launch: with others they would wait for ever.
-template <auto *KERNEL> static int check_registers(const char *name) {
+template <auto *KERNEL, int REGISTERS> static int check_registers(const char *name) {
     static const int regs = [] {
         cudaFuncAttributes f;
         return cudaFuncGetAttributes(&f, (const void *)KERNEL) == cudaSuccess ? f.numRegs : -1;
     }();
-    SAPA_REQUIRE(regs == REGS, SAPA_ERR_LAUNCH, "%s: built with %d registers a thread, not %d", name, regs, REGS);
+    SAPA_REQUIRE(regs == REGISTERS, SAPA_ERR_LAUNCH, "%s: built with %d registers a thread, not %d", name, regs, REGISTERS);
     return SAPA_OK;
 }
 
@@ -58,7 +58,7 @@ static int launch(const Args &p, const CUtensorMap &q, const CUtensorMap &k, con
     using L = um::Lay<D, WIDE>;
     int sms = 0;
     if (int e = prepare_launch((const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED>, L::SMEM, "sapa_attention_umma_kernel", sms)) return e;
-    if (int e = check_registers<sapa_attention_umma_kernel<T, D, WIDE, PAGED>>("sapa_attention_umma_kernel")) return e;
+    if (int e = check_registers<sapa_attention_umma_kernel<T, D, WIDE, PAGED>, REGS>("sapa_attention_umma_kernel")) return e;
     launch_next(sapa_attention_umma_kernel<T, D, WIDE, PAGED>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), L::SMEM, st, q, k, v, p, (int)items);
     return check_launch(WIDE ? "sapa_attention_umma_kernel<wide>" : "sapa_attention_umma_kernel<narrow>");
 }
@@ -106,8 +106,8 @@ static int launch(const Args &p, const Grads &g, const CUtensorMap &own0, const 
     int sms = 0;
     constexpr int SMEM = umg::Lay<D, KEYS>::SMEM;
     if (int e = prepare_launch((const void *)sapa_attention_umma_grad_kernel<T, D, KEYS>, SMEM, "sapa_attention_umma_grad_kernel", sms)) return e;
-    if (int e = um::check_registers<sapa_attention_umma_grad_kernel<T, D, KEYS>>("sapa_attention_umma_grad_kernel")) return e;
-    launch_next(sapa_attention_umma_grad_kernel<T, D, KEYS>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), SMEM, st, own0, own1, over0, over1, p, g, (int)items);
+    if (int e = um::check_registers<sapa_attention_umma_grad_kernel<T, D, KEYS>, umg::GRAD_REGS>("sapa_attention_umma_grad_kernel")) return e;
+    launch_next(sapa_attention_umma_grad_kernel<T, D, KEYS>, dim3((unsigned)(items < sms ? items : sms)), dim3(umg::THREADS), SMEM, st, own0, own1, over0, over1, p, g, (int)items);
     return check_launch(KEYS ? "sapa_attention_umma_grad_kernel<keys>" : "sapa_attention_umma_grad_kernel<queries>");
 }
 

@@ -106,10 +106,10 @@ __device__ __forceinline__ float max2(float a, float b) {
 }
 // 2^x without the unit that ex2 keeps busy: x = n + f with n the nearest whole number, 2^f by a polynomial with the least relative error over [-1/2, 1/2]
 // (1.0e-4 in degree 3, a fortieth of bfloat16's half step; 2.8e-6 in degree 4 for float16) that is 1 at 0, and n added to its exponent.  0 from 2^-127 down.
-// KEEP: NaN for a NaN, at the price of a product by 2^n; otherwise it gives a number, and a row with a NaN has to be found by its maximum.
-template <typename T, bool KEEP = false> __device__ __forceinline__ float2 ex2_by_fma(float2 x) {
+// What a NaN gives is a number: a row with a NaN has to be found by its maximum.
+template <typename T> __device__ __forceinline__ float2 ex2_by_fma(float2 x) {
     constexpr float ROUND = 12582912.f;                               // 1.5 * 2^23: adding it leaves whole numbers
-    x.x = KEEP ? max2(x.x, -127.f) : fmaxf(x.x, -127.f); x.y = KEEP ? max2(x.y, -127.f) : fmaxf(x.y, -127.f);
+    x.x = fmaxf(x.x, -127.f); x.y = fmaxf(x.y, -127.f);
     const float2 t = add2(x, make_float2(ROUND, ROUND)), n = add2(t, make_float2(-ROUND, -ROUND)), f = fma2(n, make_float2(-1.f, -1.f), x);
     float2 y;
     if constexpr (std::is_same<T, __half>::value) {
@@ -121,9 +121,9 @@ template <typename T, bool KEEP = false> __device__ __forceinline__ float2 ex2_b
         y = fma2(f, y, make_float2(0.693282961845398f, 0.693282961845398f));
     }
     y = fma2(f, y, make_float2(1.f, 1.f));
-    if (KEEP) return mul2(y, make_float2(__int_as_float(0x3f800000 + (__float_as_int(t.x) << 23)), __int_as_float(0x3f800000 + (__float_as_int(t.y) << 23))));
     return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap *map, unsigned bar, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
         tc_alloc((unsigned)__cvta_generic_to_shared(&tmem_slot), L::TMEM_COLS);
         tc_relinquish();
     }
+    if (warp == LOAD_WARP && lane < 3) prefetch_map(lane == 0 ? &qmap : lane == 1 ? &kmap : &vmap);
     begin_after_previous();
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
     if (a.lse != nullptr) clear_outside(a.lse, a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);

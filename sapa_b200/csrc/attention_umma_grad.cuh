@@ -24,23 +24,22 @@ namespace umg {
 
 using namespace um;
 
-constexpr int N = 64;                                                 // columns of a thread
-constexpr int GRAD_BY_FMA = 1, GRAD_BY_FMA_OF = 4;
-constexpr int ROW_WARP = VALUE_WARP;                                  // loads lse and delta
+constexpr int N = 32, GROUPS = 4;                                     // columns of a thread; warpgroups that form P and dS
+constexpr int MMA = 4 * GROUPS, LOAD = MMA + 1, PLANS = MMA + 2, ROW = MMA + 3, THREADS = (4 * GROUPS + 4) * 32;      // warps; ROW loads lse and delta
+// registers a thread: 96 at launch
+constexpr int GRAD_REGS = 96, FORM_REGS = 104, REST_REGS = 64;
+static_assert(GROUPS * 128 * FORM_REGS + 128 * REST_REGS <= THREADS * GRAD_REGS, "a block draws on what it was launched with");
 
 template <int D, bool KEYS> struct Lay {
     static constexpr bool BOTH = KEYS && D == 128;
-    static constexpr int TN = BOTH ? 128 : 64, SLOTS = BOTH ? 1 : 2, THREADS = 256 / SLOTS;      // rows of a tile that is gone over, tiles at once, threads that take one
+    static constexpr int TN = BOTH ? 128 : 64, SLOTS = BOTH ? 1 : 2, FORM = GROUPS * 128 / SLOTS;      // rows of a tile that is gone over, tiles at once, threads that take one
     static constexpr int OWN = D / 64 * BLOCK_BYTES, BOX = TN * 128, HALF = D / 64 * BOX, NST = BOTH ? 2 : D == 64 ? 8 : 4;      // stages of each operand
     static constexpr int OWN0 = 0, ST0 = 2 * OWN, NEED = ST0 + 2 * NST * HALF + 1024, SMEM = NEED < 120 * 1024 ? 120 * 1024 : NEED;
     // S and dP of what is at work, dV and dK or dQ, and where there is room the item's own two operands
-    static constexpr int S_COL = 0, P_COL = 2 * N, ACC_COL = 4 * N, OWN_COL = ACC_COL + (KEYS ? 2 : 1) * D, TMEM_COLS = 512;
+    static constexpr int S_COL = 0, P_COL = 128, ACC_COL = 256, OWN_COL = ACC_COL + (KEYS ? 2 : 1) * D, TMEM_COLS = 512;
     static constexpr bool IN_TMEM = OWN_COL + D <= TMEM_COLS;
     static_assert(SMEM <= 222 * 1024 && OWN_COL <= TMEM_COLS, "shared memory, with lse and delta; tensor memory");
 };
-// which of a thread's 64 columns have their exponentials on the FMA units
-__device__ __forceinline__ constexpr bool by_fma(int column) { return (column >> 1) % GRAD_BY_FMA_OF < GRAD_BY_FMA; }
-
 // An item of a block
 struct Work {
     bool there;
@@ -61,20 +60,17 @@ template <typename T, int D, int TN, bool IN_TMEM> __device__ __forceinline__ vo
         else tc_mma<false>(leader, d, a + (c >> 2) * (BLOCK_BYTES >> 4) + (c & 3) * 2, at, HI, IDESC, c > 0 ? 1u : 0u);
     }
 }
-// acc[128 x D] (+)= A[128 x TN] B: A in tensor memory, the 32 words of a thread's 64 columns in 64, B MN-major
+// acc[128 x D] (+)= A[128 x TN] B: A in tensor memory, the 16 words of a thread's 32 columns in 32, B MN-major
 template <typename T, int D, int TN> __device__ __forceinline__ void mma_columns(unsigned leader, unsigned d, unsigned a, unsigned b, bool add) {
     constexpr unsigned IDESC = IDESC_M128<T> | (1u << 16) | idesc_n(D);
 #pragma unroll
-    for (int c = 0; c < TN / 16; ++c) tc_mma_ta<false>(leader, d, a + (c >> 2) * N + (c & 3) * 8, b + c * (2048 >> 4), HI, IDESC, add || c > 0 ? 1u : 0u);
+    for (int c = 0; c < TN / 16; ++c) tc_mma_ta<false>(leader, d, a + (c >> 1) * N + (c & 1) * 8, b + c * (2048 >> 4), HI, IDESC, add || c > 0 ? 1u : 0u);
 }
 template <typename T> __device__ __forceinline__ void store_packed(unsigned taddr, const float *v) {
+    unsigned w[16];
 #pragma unroll
-    for (int c = 0; c < N; c += 32) {
-        unsigned w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack_pair(T(), v[c + 2 * e], v[c + 2 * e + 1]);
-        tc_st16(taddr + c / 2, w);
-    }
+    for (int e = 0; e < 16; ++e) w[e] = pack_pair(T(), v[2 * e], v[2 * e + 1]);
+    tc_st16(taddr, w);
 }
 // Replaces what is not finite in a row of a tile of TN rows; whether there was any.
 template <typename T, int D, int TN> __device__ __forceinline__ bool clean_box(unsigned tile, int row) {
@@ -87,7 +83,7 @@ template <typename T, int D, int TN> __device__ __forceinline__ bool clean_box(u
 }  // namespace umg
 
 template <typename T, int D, bool KEYS>
-__global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(const __grid_constant__ CUtensorMap own0, const __grid_constant__ CUtensorMap own1,
+__global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kernel(const __grid_constant__ CUtensorMap own0, const __grid_constant__ CUtensorMap own1,
                                                                              const __grid_constant__ CUtensorMap over0, const __grid_constant__ CUtensorMap over1,
                                                                              const __grid_constant__ Args p, const __grid_constant__ Grads g, const int most_items) {
     using namespace umg;
@@ -95,7 +91,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
     using Work = umg::Work;
     constexpr int NST = L::NST, TN = L::TN, SLOTS = L::SLOTS;
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(16) float row_lse[KEYS ? NST : 1][TN], row_delta[KEYS ? NST : 1][TN];
+    __shared__ __align__(16) float row_lse[KEYS ? NST : 1][TN], row_delta[KEYS ? NST : 1][TN];      // as nlse, -delta
     __shared__ __align__(8) unsigned long long bars[2 + 4 * NST + 8 + 4 + 3];
     __shared__ unsigned tmem_slot;
     __shared__ bool row_odd[NST];                                     // KEYS: whether a row of the stage may hold something not finite
@@ -108,13 +104,13 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
     // KEYS: rows of a tile are `tok` tokens x `at_once` heads of a key head, which take `turns` tiles if they are more; otherwise an item is `tok` tokens
     const int at_once = KEYS ? min(p.share, TN) : p.share, tok = (KEYS ? TN : ROWS) / at_once, rows = tok * at_once;
 
-    if (warp == MMA_WARP) {
+    if (warp == MMA) {
         if (lane == 0) {
-            mbar_init(ownfull, 1); mbar_init(ownempty, L::IN_TMEM ? 256 : 1); mbar_init(done, 1); mbar_init(accfree, 256); mbar_init(ownready, 256);
+            mbar_init(ownfull, 1); mbar_init(ownempty, L::IN_TMEM ? GROUPS * 128 : 1); mbar_init(done, 1); mbar_init(accfree, GROUPS * 128); mbar_init(ownready, GROUPS * 128);
             for (int i = 0; i < NST; ++i) { mbar_init(full + 8 * i, KEYS ? 33 : 1); mbar_init(empty + 8 * i, 1); mbar_init(full1 + 8 * i, 1); mbar_init(empty1 + 8 * i, 1); }
             for (int i = 0; i < 2; ++i) {
-                mbar_init(sfull + 8 * i, 1); mbar_init(dpfull + 8 * i, 1); mbar_init(pfull + 8 * i, L::THREADS); mbar_init(dsfull + 8 * i, L::THREADS);
-                mbar_init(posted + 8 * i, 1); mbar_init(taken + 8 * i, KEYS ? 11 : 10);
+                mbar_init(sfull + 8 * i, 1); mbar_init(dpfull + 8 * i, 1); mbar_init(pfull + 8 * i, L::FORM); mbar_init(dsfull + 8 * i, L::FORM);
+                mbar_init(posted + 8 * i, 1); mbar_init(taken + 8 * i, 4 * GROUPS + (KEYS ? 3 : 2));
             }
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
@@ -123,18 +119,19 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
         tc_relinquish();
     }
     if (KEYS)                                                         // rows that no copy fills: they are behind P and dS, which are 0 there
-        for (int i = tid; i < (TN - rows) * 8 * (D / 64) * 2 * NST; i += NT) {
+        for (int i = tid; i < (TN - rows) * 8 * (D / 64) * 2 * NST; i += umg::THREADS) {
             const int tile = i / ((TN - rows) * 8), e = i % ((TN - rows) * 8);
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(base + L::ST0 + tile * L::BOX + (rows + e / 8) * 128 + (e % 8) * 16), "r"(0u) : "memory");
         }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    if (warp == LOAD && lane < 4) prefetch_map(lane == 0 ? &own0 : lane == 1 ? &own1 : lane == 2 ? &over0 : &over1);
     begin_after_previous();
     auto meet = [&]() {
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
     };
-    if (warp != PLAN_WARP) meet();                                    // that one looks for the first item meanwhile
+    if (warp != PLANS) meet();                                    // that one looks for the first item meanwhile
     const unsigned tmem = warp_uniform(*reinterpret_cast<volatile unsigned *>(&tmem_slot));
     bool ok = true;
     int turn = 0;
@@ -148,9 +145,9 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
         ++turn;
     };
 
-    if (warp >= MMA_WARP) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(OTHER_REGS));
-        if (warp == PLAN_WARP) {
+    if (warp >= MMA) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REST_REGS));
+        if (warp == PLANS) {
             typename std::conditional<KEYS, InOrder<false, KeyBlocks>, InOrder<true, QueryBlocks>>::type order(a, {a.causal != 0, tok, KT}, lane);
             for (int round = 0;; ++round) {
                 const int index = round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
@@ -180,7 +177,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                 __syncwarp();
                 if (!w.there) break;
             }
-        } else if (warp == LOAD_WARP) {
+        } else if (warp == LOAD) {
             int st = 0, ph = 0, own_ph = 0;
             while (Work *w = next_work()) {
                 const int n = w->n, first = w->first, group = w->group;
@@ -226,7 +223,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                 (void)drain_loads<NST>(full1, st, ph);
                 (void)mbar_wait_bounded(ownfull, own_ph ^ 1);
             }
-        } else if (warp == ROW_WARP) {
+        } else if (warp == ROW) {
             if (KEYS) {                                                   // lse and delta of a tile's rows, read a tile ahead
                 int st = 0, ph = 0;
                 while (Work *w = next_work()) {
@@ -250,7 +247,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                         ok = mbar_wait_warp(empty + 8 * st, ph ^ 1);
                         if (!ok) break;
 #pragma unroll
-                        for (int r = 0; r < TN / 32; ++r) { row_lse[st][lane + 32 * r] = e[r]; row_delta[st][lane + 32 * r] = d[r]; }
+                        for (int r = 0; r < TN / 32; ++r) { row_lse[st][lane + 32 * r] = e[r]; row_delta[st][lane + 32 * r] = -d[r]; }
                         // what is not finite in a row of dO is in its delta, and in a row of Q in its lse, if it sees a key at all
                         bool odd = false;
 #pragma unroll
@@ -265,7 +262,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                     work_done();
                 }
             }
-        } else if (warp == MMA_WARP) {
+        } else if (warp == MMA) {
             const unsigned leader = elect_leader();
             const unsigned a0 = L::IN_TMEM ? tmem + L::OWN_COL : warp_uniform(desc_lo(base + L::OWN0, 16));
             const unsigned a1 = L::IN_TMEM ? tmem + L::OWN_COL + D / 2 : warp_uniform(desc_lo(base + L::OWN0 + L::OWN, 16));
@@ -275,13 +272,13 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
             auto scores = [&](int t) {
                 ok = ok && mbar_wait_warp(full + 8 * st, ph);
                 if (!ok) return;
-                mma_rows<T, D, TN, L::IN_TMEM>(leader, tmem + L::S_COL + t * N, a0, b_rows + st * STEP);
+                mma_rows<T, D, TN, L::IN_TMEM>(leader, tmem + L::S_COL + t * 64, a0, b_rows + st * STEP);
                 tc_commit_by(leader, sfull + 8 * t);
             };
             auto products = [&](int t) {                              // dP, of the stage that scores() has waited for
                 ok = ok && mbar_wait_warp(full1 + 8 * st, ph);
                 if (!ok) return;
-                mma_rows<T, D, TN, L::IN_TMEM>(leader, tmem + L::P_COL + t * N, a1, b_rows + st * STEP + SECOND);
+                mma_rows<T, D, TN, L::IN_TMEM>(leader, tmem + L::P_COL + t * 64, a1, b_rows + st * STEP + SECOND);
                 tc_commit_by(leader, dpfull + 8 * t);
                 if (!KEYS) tc_commit_by(leader, empty1 + 8 * st);
                 if (++st == NST) { st = 0; ph ^= 1; }
@@ -306,14 +303,14 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                     if (!ok) break;
                     tc_fence_after();
                     if (KEYS) {
-                        mma_columns<T, D, TN>(leader, tmem + L::ACC_COL, tmem + L::S_COL + t * N, b_cols + now * STEP + SECOND, i > 0);
+                        mma_columns<T, D, TN>(leader, tmem + L::ACC_COL, tmem + L::S_COL + t * 64, b_cols + now * STEP + SECOND, i > 0);
                         tc_commit_by(leader, empty1 + 8 * now);
                     }
                     if (i + SLOTS < n) scores(t);
                     ok = ok && mbar_wait_warp(dsfull + 8 * t, t == 0 ? tph0 : tph1);
                     if (!ok) break;
                     tc_fence_after();
-                    mma_columns<T, D, TN>(leader, tmem + L::ACC_COL + (KEYS ? D : 0), tmem + L::P_COL + t * N, b_cols + now * STEP, i > 0);
+                    mma_columns<T, D, TN>(leader, tmem + L::ACC_COL + (KEYS ? D : 0), tmem + L::P_COL + t * 64, b_cols + now * STEP, i > 0);
                     tc_commit_by(leader, empty + 8 * now);
                     if (++now == NST) now = 0;
                     if (i + SLOTS < n) {
@@ -328,12 +325,12 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(SOFTMAX_REGS));
-        const int t = warp >> 2, r = tid & 127;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(FORM_REGS));
+        // warpgroup, the tile that it takes (BOTH: all take every tile, otherwise two each every other one), its part of the columns
+        const int wg = warp >> 2, t = L::BOTH ? 0 : wg >> 1, part_of = L::BOTH ? wg : wg & 1, r = tid & 127, bar = 8 * t, col0 = N * part_of;
         const unsigned quarter = (unsigned)((warp & 3) * 32) << 16;
-        const unsigned s_at = tmem + quarter + L::S_COL + t * N, d_at = tmem + quarter + L::P_COL + t * N;
+        const unsigned s_at = tmem + quarter + L::S_COL + wg * N, d_at = tmem + quarter + L::P_COL + wg * N;
         const float2 scale = make_float2(p.scale_log2, p.scale_log2);
-        const int bar = L::BOTH ? 0 : 8 * t, col0 = L::BOTH ? N * t : 0;      // BOTH: columns 64 t .. of every tile; otherwise every other tile
         const int row_token = r / p.share;
         int sph = 0, own_ph = 0;
         unsigned loads = 0;                                           // stages that the items before took
@@ -348,19 +345,20 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                 const long long row = ((long long)w->group * a.tokens + s.q0 + first) * p.share + r;
                 nlse = g.nlse[row]; delta = g.delta[row];
             }
-            if (L::IN_TMEM && n > 0) {                                // the item's own operands, one by each warpgroup; what was there has been used: `done`
+            if (L::IN_TMEM && n > 0) {                                // the item's own operands, half of one by each warpgroup; what was there has been used: `done`
                 if (!mbar_wait_warp(ownfull, own_ph)) { ok = false; break; }
                 own_ph ^= 1;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-                    unsigned v[32];
+                for (int h = 0; h < D / 64; ++h) {
+                    unsigned v[16];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
+                    for (int e = 0; e < 4; ++e) {
+                        const int chunk = (wg & 1) * (D / 16) + 4 * h + e;
                         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[4 * e]), "=r"(v[4 * e + 1]), "=r"(v[4 * e + 2]), "=r"(v[4 * e + 3])
-                                     : "r"(base + L::OWN0 + t * L::OWN + c * BLOCK_BYTES + r * 128 + ((e ^ (r & 7)) << 4)) : "memory");
-                    tc_st16(tmem + quarter + L::OWN_COL + t * (D / 2) + 32 * c, v);
-                    tc_st16(tmem + quarter + L::OWN_COL + t * (D / 2) + 32 * c + 16, v + 16);
+                                     : "r"(base + L::OWN0 + (wg >> 1) * L::OWN + (chunk >> 3) * BLOCK_BYTES + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) : "memory");
+                    }
+                    tc_st16(tmem + quarter + L::OWN_COL + (wg >> 1) * (D / 2) + (wg & 1) * (D / 4) + 16 * h, v);
                 }
                 mbar_arrive(ownempty);
                 tc_wait_st();
@@ -392,7 +390,6 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                 if (!mbar_wait_warp(sfull + bar, sph)) { ok = false; break; }
                 tc_fence_after();
                 tc_ld32(s_at, x);
-                tc_ld32(s_at + 32, x + 32);
                 tc_wait_ld();
                 if (!KEYS) {                                          // the next scores may come
                     tc_fence_before();
@@ -400,9 +397,8 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                 }
 #pragma unroll
                 for (int c = 0; c < N; c += 2) {
-                    float2 u = fma2(make_float2(x[c], x[c + 1]), scale, KEYS ? make_float2(y[c], y[c + 1]) : make_float2(nlse, nlse));
-                    u = by_fma(c) ? ex2_by_fma<T, true>(u) : make_float2(ex2_ftz(u.x), ex2_ftz(u.y));
-                    x[c] = u.x; x[c + 1] = u.y;
+                    const float2 u = fma2(make_float2(x[c], x[c + 1]), scale, KEYS ? make_float2(y[c], y[c + 1]) : make_float2(nlse, nlse));
+                    x[c] = ex2_ftz(u.x); x[c + 1] = ex2_ftz(u.y);
                 }
                 if (KEYS) {
                     if (part) {
@@ -413,13 +409,12 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                 }
                 if (part && (!KEYS || row_odd[st])) {                 // behind the products that take the tiles as they are
                     if (!mbar_wait_warp(dpfull + bar, sph)) { ok = false; break; }
-                    // a row of dO or of Q each; of K
-                    const int row = L::BOTH ? r : r & 63;
-                    const bool second = L::BOTH ? t == 0 : r >= 64;
-                    if (KEYS) {
-                        const bool odd = clean_box<T, D, TN>(stage + (second ? NST * L::HALF : 0), row);
-                        if (odd && second && row < hi) { atomicMin(&w->odd_first, i); atomicMax(&w->odd_last, i); }
-                    } else if (r < TN) {
+                    if (KEYS) {                                       // rows of dO by the first warpgroup of the tile's, of Q by the second
+                        if (part_of < 2 && r < TN) {
+                            const bool odd = clean_box<T, D, TN>(stage + (part_of == 0 ? NST * L::HALF : 0), r);
+                            if (odd && part_of == 0 && r < hi) { atomicMin(&w->odd_first, i); atomicMax(&w->odd_last, i); }
+                        }
+                    } else if (part_of == 0 && r < TN) {
                         if (clean_box<T, D, TN>(stage, r) && i * TN + r < s.nk) { atomicMin(&w->odd_first, i * TN + r); atomicMax(&w->odd_last, i * TN + r); }
                     }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -429,21 +424,17 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
                     tc_fence_before();
                     mbar_arrive(pfull + bar);
                 }
-                float d[KEYS ? N : 1];
-                if (KEYS) {
-#pragma unroll
-                    for (int c = 0; c < N; c += 4) *reinterpret_cast<float4 *>(&d[KEYS ? c : 0]) = *reinterpret_cast<const float4 *>(&row_delta[KEYS ? st : 0][col0 + c]);
-                }
                 if (!mbar_wait_warp(dpfull + bar, sph)) { ok = false; break; }
                 sph ^= 1;
                 tc_fence_after();
                 tc_ld32(d_at, y);
-                tc_ld32(d_at + 32, y + 32);
                 tc_wait_ld();
 #pragma unroll
-                for (int c = 0; c < N; c += 2) {
-                    const float2 u = mul2(make_float2(x[c], x[c + 1]), add2(make_float2(y[c], y[c + 1]), KEYS ? make_float2(-d[KEYS ? c : 0], -d[KEYS ? c + 1 : 0]) : make_float2(-delta, -delta)));
-                    y[c] = u.x; y[c + 1] = u.y;
+                for (int c = 0; c < N; c += 4) {
+                    const float4 d = KEYS ? *reinterpret_cast<const float4 *>(&row_delta[KEYS ? st : 0][col0 + c]) : make_float4(-delta, -delta, -delta, -delta);
+                    const float2 u = mul2(make_float2(x[c], x[c + 1]), add2(make_float2(y[c], y[c + 1]), make_float2(d.x, d.y)));
+                    const float2 v = mul2(make_float2(x[c + 2], x[c + 3]), add2(make_float2(y[c + 2], y[c + 3]), make_float2(d.z, d.w)));
+                    y[c] = u.x; y[c + 1] = u.y; y[c + 2] = v.x; y[c + 3] = v.y;
                 }
                 if (part) {
 #pragma unroll
@@ -457,16 +448,18 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
             loads += n;
             ok = ok && mbar_wait_warp(done, turn & 1);
             tc_fence_after();
-            // KEYS: the first warpgroup stores the gradients of the values, the second those of the keys; otherwise each half of the channels
-            const bool values = KEYS && t == 0;
-            const unsigned at = tmem + quarter + L::ACC_COL + (KEYS ? t * D : 0);
-            const float factor = values ? 1.f : a.scale;
-            T *const to = KEYS ? static_cast<T *>(values ? g.gv : g.gk) + ((long long)(s.k0 + key) * a.groups + w->group) * a.dim
-                               : static_cast<T *>(g.gq) + ((long long)(s.q0 + token) * a.heads + w->group * p.share + r % p.share) * a.dim;
+            // 32 channels a warpgroup at a time: of the gradients of values, of keys; or of queries
             const int odd0 = w->odd_first, odd1 = w->odd_last;
-            const bool whole = whole_rows(KEYS ? (values ? g.gv : g.gk) : g.gq, a.dim);
+            const bool whole = whole_rows(KEYS ? g.gk : g.gq, a.dim) && (!KEYS || whole_rows(g.gv, a.dim));
 #pragma unroll 1
-            for (int c = KEYS ? 0 : t * (D / 2); c < (KEYS ? D : (t + 1) * (D / 2)) && c < a.dim && ok; c += 32) {
+            for (int unit = wg; unit < (KEYS ? 2 : 1) * (D / 32) && ok; unit += GROUPS) {
+                const bool values = KEYS && unit < D / 32;
+                const int c = unit % (D / 32) * 32;
+                if (c >= a.dim) continue;
+                const unsigned at = tmem + quarter + L::ACC_COL + unit * 32 - c;
+                const float factor = values ? 1.f : a.scale;
+                T *const to = KEYS ? static_cast<T *>(values ? g.gv : g.gk) + ((long long)(s.k0 + key) * a.groups + w->group) * a.dim
+                                   : static_cast<T *>(g.gq) + ((long long)(s.q0 + token) * a.heads + w->group * p.share + r % p.share) * a.dim;
                 float o[32];
                 if (n > 0) {
                     tc_ld32(at + c, o);
@@ -506,7 +499,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_grad_kernel(con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == MMA_WARP) tc_dealloc(tmem, L::TMEM_COLS);
+    if (warp == MMA) tc_dealloc(tmem, L::TMEM_COLS);
 }
 
 }  // namespace attn
