@@ -722,7 +722,7 @@ static Shape shape_of(const Args &p, int dtype, int sms) {
     // few blocks: their keys are split so that every SM has items
     const long long keys = a.page_table != nullptr ? (long long)a.max_pages * a.page : a.keys;
     if (s.blocks < 2ll * sms && keys > (s.umma ? 8 : 2) * TILE) {
-        s.split = (s.umma ? 3 : 4) * sms;
+        s.split = (s.umma ? (s.narrow ? 2 : 3) : 4) * sms;
         s.grid = s.blocks + s.split;
         s.part = (size_t)s.grid * s.bm * a.dim * sizeof(float);
         s.lse = (size_t)s.grid * s.bm * sizeof(float);
@@ -773,7 +773,7 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
     Args p = args_of(a);
     Shape s = shape_of(p, dtype, sms);
     if (s.grid == 0) s.grid = 1;                     // no sequence: every row is cleared
-    SAPA_REQUIRE(s.grid < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
+    SAPA_REQUIRE(s.grid < 0x3fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
     if (s.split > 0) {
         SAPA_REQUIRE(workspace != nullptr && workspace_bytes >= s.bytes, SAPA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, s.bytes, workspace_bytes);
         SAPA_REQUIRE(aligned16(workspace), SAPA_ERR_ALIGNMENT, "%s: the workspace must be 256-byte aligned", fn);

@@ -66,23 +66,26 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {      // inclusive
 // `Blocks::at_least(s, w)`: blocks of a sequence with at least w units of work, all for w = 0; `units(s)`: the most that one of its blocks has.  LAST: a
 // sequence's blocks have the more work the later they come (a causal token sees the more keys), otherwise the less.  The amount of work is searched
 // for by halving, each time adding up the sequences' counts; each lane keeps the first of its sequences in registers.  A block of the grid asks for
-// growing indices, so the search goes on from the last one's: mostly nothing is added up again.
+// growing indices, so the search goes on from the last one's: mostly nothing is added up again, and no sequence is looked at twice.
+// Of more than SORTED sequences the order is theirs: adding up so many again and again would take longer than it gains.
 template <bool LAST, typename Blocks> struct InOrder {
     const sapa_attention &a;
     const Blocks kind;
     const int lane;
     Sequence own;
+    static constexpr int SORTED = 512;
     int total, lo, hi, upto, behind;                    // all(lo) = upto > index >= behind = all(hi)
+    int chunk, passed;                                  // sequences below `chunk` have their blocks of just lo units among the first `passed` ones
     __device__ __forceinline__ InOrder(const sapa_attention &args, const Blocks &k, int l, bool wanted = true)
-        : a(args), kind(k), lane(l), own{0, 0, 0, 0, 0}, total(0), lo(0), hi(0), upto(0), behind(0) {
+        : a(args), kind(k), lane(l), own{0, 0, 0, 0, 0}, total(0), lo(0), hi(0), upto(0), behind(0), chunk(0), passed(0) {
         if (!wanted) return;
         if (lane < a.B) own = sequence_at(a, lane);
         int most = kind.units(own);
         for (int b = lane + 32; b < a.B; b += 32) most = max(most, kind.units(sequence_at(a, b)));
         total = all(0);
         hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) + 1;
-        lo = hi;
-        upto = behind = 0;
+        lo = a.B > SORTED ? 0 : hi;
+        upto = a.B > SORTED ? total : 0;
     }
     __device__ __forceinline__ int all(int w) const {
         int n = kind.at_least(own, w);
@@ -101,12 +104,14 @@ template <bool LAST, typename Blocks> struct InOrder {
                 const int mid = lo + (hi - lo) / 2, n = all(mid);
                 if (n > index) { lo = mid; upto = n; } else { hi = mid; behind = n; }
             }
+            chunk = 0;
+            passed = behind;
         }
-        int left = index - behind;                      // among the blocks with just lo units
-        for (int b0 = 0; b0 < a.B; b0 += 32) {
+        for (int b0 = chunk; b0 < a.B; b0 += 32) {      // among the blocks with just lo units
             const int b = b0 + lane;
             const Sequence s = b0 == 0 ? own : b < a.B ? sequence_at(a, b) : Sequence{0, 0, 0, 0, 0};
             const int more = kind.at_least(s, hi), here = kind.at_least(s, lo) - more, end = warp_scan(here, lane);
+            const int left = index - passed;
             const unsigned hit = __ballot_sync(0xffffffffu, left < end);
             if (hit != 0u) {
                 const int from = __ffs(hit) - 1, before = more + left - (end - here);      // blocks of the sequence with no less work in front of it
@@ -115,7 +120,8 @@ template <bool LAST, typename Blocks> struct InOrder {
                 it.there = true;
                 return it;
             }
-            left -= __shfl_sync(0xffffffffu, end, 31);
+            passed += __shfl_sync(0xffffffffu, end, 31);
+            chunk = b0 + 32;
         }
         return it;
     }

@@ -302,6 +302,55 @@ def test_prompt_then_tokens(dtype):
         lo, hi = hi, [min(n, h + 1) for n, h in zip(total, hi)]
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_sequences_than_are_sorted(dtype):
+    """Hundreds of sequences, some empty, forward, backward and over a cache."""
+    lengths = [(7 * i) % 23 for i in range(700)]
+    T = sum(lengths)
+    q, k, v = (x.requires_grad_() for x in _inputs(T, T, 4, 2, 32, TYPES[dtype]))
+    go = _made((T, 4, 32), TYPES[dtype], 9)
+    want = oracle.packed(q.detach(), k.detach(), v.detach(), lengths, lengths, True, 32 ** -0.5, go)
+    out = sapa_b200.packed_attention(q, k, v, offsets_of(lengths))
+    check(out.detach(), want["out"], want["out_tol"])
+    for name, g in zip(("gq", "gk", "gv"), torch.autograd.grad(out, (q, k, v), go)):
+        check(g, want[name], want[name + "_tol"])
+    c = Cache(k.detach(), v.detach(), lengths, 16)
+    with torch.no_grad():
+        check(sapa_b200.paged_attention(q, c.key, c.value, c.table, c.lengths, offsets_of(lengths)), want["out"], want["out_tol"])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_scale_of_zero_is_the_mean(dtype):
+    q, k, v = _inputs(300, 300, 4, 2, 64, TYPES[dtype])
+    want = oracle.packed(q, k, v, [300], [300], True, 0.0)
+    check(sapa_b200.packed_attention(q, k, v, offsets_of([300]), scale=0.0), want["out"], want["out_tol"])
+    k[100, 0, 0] = math.inf                              # 0 * infinity is not a number
+    assert bool(sapa_b200.packed_attention(q, k, v, offsets_of([300]), scale=0.0)[100:, :2].isnan().all())
+
+
+def test_which_kernels_serve():
+    from sapa_b200 import _lib
+    q, k, v = (x.requires_grad_() for x in _inputs(4000, 4000, 8, 2, 64, torch.bfloat16))
+    off = offsets_of([4000])
+    out = sapa_b200.packed_attention(q, k, v, off)
+    assert _lib.last_kernels()[0] == "sapa_attention_umma_kernel<wide>"
+    torch.autograd.grad(out.sum(), (q, k, v))
+    assert _lib.last_kernels() == ["sapa_attention_delta_kernel", "sapa_attention_umma_grad_kernel<keys>", "sapa_attention_umma_grad_kernel<queries>"]
+    with torch.no_grad():
+        for page, kernel in ((16, "sapa_attention_umma_kernel<narrow>"), (256, "sapa_attention_umma_kernel<narrow>"), (24, "sapa_attention_rows_kernel"),
+                             (4, "sapa_attention_rows_kernel")):
+            c = Cache(k, v, [4000], page)
+            sapa_b200.paged_attention(q[:1], c.key, c.value, c.table, c.lengths, offsets_of([1]))
+            assert _lib.last_kernels() == [kernel, "sapa_attention_join_kernel"]
+            sapa_b200.paged_write(k[:3], v[:3], c.key, c.value, c.table, c.lengths, offsets_of([3]))
+            assert _lib.last_kernels() == ["sapa_paged_write_kernel"]
+    f = [x.detach().float().requires_grad_() for x in (q, k, v)]
+    out = sapa_b200.packed_attention(*f, off)
+    assert _lib.last_kernels()[0] == "sapa_attention_rows_kernel"
+    torch.autograd.grad(out.sum(), f)
+    assert _lib.last_kernels() == ["sapa_attention_delta_kernel", "sapa_attention_rows_grad_kernel<keys>", "sapa_attention_rows_grad_kernel<queries>"]
+
+
 def test_captured_and_replayed_with_other_lengths():
     q, k, v = _inputs(64, 600, 8, 2, 64, torch.bfloat16)
     off, koff = offsets_of([1] * 4), offsets_of([100, 20, 5, 300])
