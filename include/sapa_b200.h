@@ -413,6 +413,7 @@ typedef struct sapa_attention {
     const void *query, *key, *value;
     void *out;
     float *lse;                     /* log of the sum of exp(scale * <q, k>), for the backward pass; may be NULL; -inf: no key seen */
+    void *low;                      /* what rounding left out, for the backward pass, or NULL: of `out` (16-bit types, like `out`), of `lse` (float32) */
     const int *offsets;             /* [B + 1] */
     const int *key_offsets;         /* [B + 1], packed */
     const int *page_table;          /* [B, max_pages], paged */
@@ -429,7 +430,7 @@ typedef struct sapa_attention {
 /* Forward.  Workspace: sapa_attention_workspace() bytes (may be 0), 256-byte aligned.  Deterministic. */
 size_t sapa_attention_workspace(const sapa_attention *a, int dtype);
 int sapa_attention_forward(const sapa_attention *a, void *workspace, size_t workspace_bytes, int dtype, void *stream);
-/* Gradients of the packed form from grad_out (its strides: of a token, of a head); a->out and a->lse are the forward's.  Deterministic.
+/* Gradients of the packed form from grad_out (its strides: of a token, of a head); a->out, a->lse and a->low are the forward's.  Deterministic.
  * Workspace: sapa_attention_backward_workspace() bytes, 256-byte aligned. */
 size_t sapa_attention_backward_workspace(const sapa_attention *a, int dtype);
 int sapa_attention_backward(const sapa_attention *a, const void *grad_out, long long grad_token_stride, long long grad_head_stride,

@@ -34,9 +34,9 @@ class PackedAttentionFunction(Function):
 
     @staticmethod
     def forward(ctx, query, key, value, offsets, key_offsets, causal, scale):
-        out, lse, scale = _lib.load_host().packed_attention_forward(query, key, value, offsets, key_offsets, causal, scale)
+        out, lse, low, scale = _lib.load_host().packed_attention_forward(query, key, value, offsets, key_offsets, causal, scale)
         ctx.config = (causal, scale)
-        ctx.save_for_backward(query, key, value, out, lse, offsets, offsets if key_offsets is None else key_offsets)
+        ctx.save_for_backward(query, key, value, out, lse, low, offsets, offsets if key_offsets is None else key_offsets)
         return out
 
     @staticmethod

@@ -58,6 +58,19 @@ template <typename T> __device__ __forceinline__ void put4(T *p, float4 v) {
     *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(e);
 }
 
+// scale * s - base in base 2.  The product is not rounded by itself, nor the scale: with scores of 20 either would put a weight 1e-6 off.
+__device__ __forceinline__ float exponent(const Args &p, float s, float base) {
+    const float x = fmaf(s, p.scale_log2, -base);
+    return isfinite(x) ? fmaf(s, p.scale_rest, x) : x;
+}
+// lse of a row from the maximum and the sum of its softmax in base 2, and in float32 what its rounding leaves out
+__device__ __forceinline__ void put_lse(const sapa_attention &a, long long row, bool none, bool lost, float m, float sum, bool rest = true) {
+    const double lse = ((double)m + (double)log2f(sum)) * 0.6931471805599453;
+    const float high = none ? -INFINITY : lost ? __int_as_float(0x7fffffff) : (float)lse;
+    a.lse[row] = high;
+    if (rest && a.low != nullptr) static_cast<float *>(a.low)[row] = isfinite(high) ? (float)(lse - high) : 0.f;
+}
+
 }  // namespace rows
 
 // RI: rows of a thread (a block has 16 of them across), DP: channels in shared memory.  256 threads as 16 x 16: rows ty + 16 i, of the scores
@@ -80,6 +93,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
     }
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, tid, NT);
     if (a.lse != nullptr) clear_outside(a.lse, a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);
+    if (a.low != nullptr && std::is_same<T, float>::value) clear_outside(static_cast<float *>(a.low), a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);
     __syncthreads();
     const Item it = plan.it;
     if (!it.there) return;
@@ -177,8 +191,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                sc[i][j] = k0 + tx + 16 * j < lim[i] && tx + 16 * j < n ? sc[i][j] * p.scale_log2 : -INFINITY;
-                top = fmaxf(top, sc[i][j]);
+                if (k0 + tx + 16 * j < lim[i] && tx + 16 * j < n) top = fmaxf(top, sc[i][j] * p.scale_log2);
             }
 #pragma unroll
             for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -189,7 +202,8 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
             for (int c = 0; c < DP / 16; ++c) o[i][c] *= old;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float w = exp2f(sc[i][j] - base);
+                const bool seen = k0 + tx + 16 * j < lim[i] && tx + 16 * j < n;
+                const float w = seen ? exp2f(exponent(p, sc[i][j], base)) : 0.f;
                 l[i] += w;
                 sm[L::P0 + (ty + 16 * i) * L::PS + tx + 16 * j] = w;
             }
@@ -244,7 +258,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
             for (int j = 0; j < DP / 64; ++j)
                 if (4 * tx + 64 * j < D)
                     put4(out + 4 * tx + 64 * j, none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv));
-            if (a.lse != nullptr && tx == 0) a.lse[row] = none ? -INFINITY : lost || sum == 0.f ? nan : (m[i] + log2f(sum)) * 0.6931471805599453f;
+            if (a.lse != nullptr && tx == 0) put_lse(a, row, none, lost || sum == 0.f, m[i], sum, std::is_same<T, float>::value);
         } else {
             const float inv = sum == 0.f ? 0.f : lost ? nan : 1.f / sum;
             const long long at = ((long long)blockIdx.x * L::BM + r);
@@ -312,24 +326,30 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
         }
         const float inv = lost ? __int_as_float(0x7fffffff) : lim <= 0 ? 0.f : 1.f / sum;
         const long long row = (long long)(s.q0 + first + r / p.share) * a.heads + group * p.share + r % p.share;
-        if (c < D && way == 0) rows::put4(static_cast<T *>(a.out) + row * D + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-        if (a.lse != nullptr && lane == 0) a.lse[row] = lost ? __int_as_float(0x7fffffff) : lim <= 0 ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+        if (c < D && way == 0) {
+            const float4 v = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            rows::put4(static_cast<T *>(a.out) + row * D + c, v);
+            if (a.low != nullptr && !std::is_same<T, float>::value)
+                rows::put4(static_cast<T *>(a.low) + row * D + c, make_float4(left_out<T>(v.x), left_out<T>(v.y), left_out<T>(v.z), left_out<T>(v.w)));
+        }
+        if (a.lse != nullptr && lane == 0) rows::put_lse(a, row, lim <= 0, lost, top, sum, std::is_same<T, float>::value);
     }
 }
 
 // ---------------------------------------------------------------------------------- backward
-// delta, and what lies outside the sequences: 16 lanes per token and head, 8 channels each, two rows on their way at once.  Reads grad_out and out once, which
-// bounds it.
+// delta, and what lies outside the sequences: 16 lanes per token and head, 8 channels each, two rows on their way at once.  Reads grad_out, out and
+// what its rounding left out once, which bounds it.
 template <typename T>
 __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     const sapa_attention &a = p.a;
     constexpr int AT_ONCE = 2;
+    constexpr bool RESTS = !std::is_same<T, float>::value;            // `out` before its rounding: by itself that would make the gradients a third less exact
     const int lane = threadIdx.x & 15, c = 8 * lane, D = a.dim;
     begin_after_previous();
     const long long n = (long long)a.tokens * a.heads;
     for (long long base = (long long)blockIdx.x * (16 * AT_ONCE); base < n; base += (long long)gridDim.x * (16 * AT_ONCE)) {
         const long long row0 = base + (threadIdx.x >> 4);
-        float4 u[AT_ONCE][2], v[AT_ONCE][2];
+        float4 u[AT_ONCE][2], v[AT_ONCE][2], low[AT_ONCE][2];
         unsigned t[AT_ONCE], h[AT_ONCE];
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
@@ -340,6 +360,7 @@ __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_
             const T *o = static_cast<const T *>(a.out) + row * D + c, *y = static_cast<const T *>(g.go) + t[i] * g.go_strides[0] + h[i] * g.go_strides[1] + c;
             rows::load8(o, there, u[i]);
             rows::load8(y, there, v[i]);
+            rows::load8(static_cast<const T *>(a.low) + row * D + c, there && RESTS, low[i]);
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
@@ -347,7 +368,7 @@ __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                sum = fmaf(u[i][e].w, v[i][e].w, fmaf(u[i][e].z, v[i][e].z, fmaf(u[i][e].y, v[i][e].y, fmaf(u[i][e].x, v[i][e].x, sum))));
+                sum = fmaf(u[i][e].w + low[i][e].w, v[i][e].w, fmaf(u[i][e].z + low[i][e].z, v[i][e].z, fmaf(u[i][e].y + low[i][e].y, v[i][e].y, fmaf(u[i][e].x + low[i][e].x, v[i][e].x, sum))));
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (lane != 0 || row >= n) continue;
@@ -370,8 +391,8 @@ using namespace rows;
 constexpr int OWN = 32, OVER = 32, TEAM = 128, TEAMS = 4, THREADS = TEAM * TEAMS, WS = OWN + 4;      // rows or keys of a block, of a tile that it goes over
 template <int DP> struct Lay {
     static constexpr int XS = DP + 4;
-    static constexpr int A0 = 0, A1 = OWN * XS, LA = 2 * OWN * XS, TEAM0 = LA + 2 * OWN;
-    static constexpr int B0 = 0, B1 = OVER * XS, P0 = 2 * OVER * XS, S0 = P0 + OVER * WS, LB = S0 + OVER * WS, EACH = LB + 2 * OVER;      // of a team
+    static constexpr int A0 = 0, A1 = OWN * XS, LA = 2 * OWN * XS, TEAM0 = LA + 3 * OWN;
+    static constexpr int B0 = 0, B1 = OVER * XS, P0 = 2 * OVER * XS, S0 = P0 + OVER * WS, LB = S0 + OVER * WS, EACH = LB + 3 * OVER;      // of a team
     static constexpr size_t SMEM = (size_t)(TEAM0 + TEAMS * EACH) * sizeof(float);
     static_assert(EACH >= 2 * 4 * (DP / 16) * TEAM, "a team's sums are handed over in its tile");
 };
@@ -445,14 +466,17 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
         }
         if (!keys)
             for (int r = me; r < rows; r += threads) {
-                float e = 0.f, d = 0.f;
+                float e = 0.f, rest = 0.f, d = 0.f;
                 if (r < used && h0 + r % at_once < share) {
                     const long long at = (long long)(s.q0 + i0 + r / at_once) * a.heads + group * share + h0 + r % at_once;
-                    e = a.lse[at] * 1.4426950408889634f;
+                    const double both = ((double)a.lse[at] + static_cast<const float *>(a.low)[at]) * 1.4426950408889634;
+                    e = (float)both;
+                    rest = isfinite(e) ? (float)(both - e) : 0.f;
                     d = g.delta[at];
                 }
                 lse[r] = e;
                 lse[rows + r] = d;
+                lse[2 * rows + r] = rest;
             }
         return odd;
     };
@@ -501,7 +525,7 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
             for (int j = 0; j < 2; ++j) {
                 const int own = ty + 8 * i, over = tx + 16 * j, r = KEYS ? over : own, k = KEYS ? own : over;
                 const bool seen = k < lim[KEYS ? j : i];
-                const float w = seen ? exp2f(fmaf(sc[i][j], p.scale_log2, -lse[r])) : 0.f;
+                const float w = seen ? exp2f(exponent(p, sc[i][j], lse[r]) - lse[2 * ROWS + r]) : 0.f;
                 if (KEYS) mine[L::P0 + over * WS + own] = w;
                 mine[L::S0 + over * WS + own] = seen ? w * (dp[i][j] - lse[ROWS + r]) : 0.f;
             }
@@ -680,14 +704,16 @@ static int check(const sapa_attention *a, int dtype, const char *fn) {
     if (a->tokens == 0) return SAPA_OK;
     SAPA_REQUIRE(a->query != nullptr && a->out != nullptr, SAPA_ERR_ARGUMENT, "%s: query or out is NULL", fn);
     SAPA_REQUIRE(a->keys == 0 || (a->key != nullptr && a->value != nullptr), SAPA_ERR_ARGUMENT, "%s: key or value is NULL", fn);
-    SAPA_REQUIRE(all_aligned16(a->query, a->key, a->value, a->out), SAPA_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", fn);
+    SAPA_REQUIRE(all_aligned16(a->query, a->key, a->value, a->out, a->low), SAPA_ERR_ALIGNMENT, "%s: tensors must be 16-byte aligned", fn);
     return SAPA_OK;
 }
 
 static Args args_of(const sapa_attention *a) {
     Args p{};
     p.a = *a;
-    p.scale_log2 = a->scale * 1.4426950408889634f;
+    const double scale = (double)a->scale * 1.4426950408889634;
+    p.scale_log2 = (float)scale;
+    p.scale_rest = (float)(scale - p.scale_log2);
     p.share = a->heads / a->groups;
     return p;
 }
@@ -809,7 +835,8 @@ extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad
     SAPA_REQUIRE(a->page_table == nullptr, SAPA_ERR_UNSUPPORTED, "%s: the paged form has no gradients", fn);
     if (a->tokens == 0 && a->keys == 0) return SAPA_OK;
     const long long quantum = 16 / (long long)dtype_size(dtype);
-    SAPA_REQUIRE(a->tokens == 0 || (grad_out != nullptr && grad_query != nullptr && a->lse != nullptr), SAPA_ERR_ARGUMENT, "%s: grad_out, grad_query or lse is NULL", fn);
+    SAPA_REQUIRE(a->tokens == 0 || (grad_out != nullptr && grad_query != nullptr && a->lse != nullptr && a->low != nullptr), SAPA_ERR_ARGUMENT,
+                 "%s: grad_out, grad_query, lse or low is NULL", fn);
     SAPA_REQUIRE(a->keys == 0 || (grad_key != nullptr && grad_value != nullptr), SAPA_ERR_ARGUMENT, "%s: grad_key or grad_value is NULL", fn);
     SAPA_REQUIRE(all_aligned16(grad_out, grad_query, grad_key, grad_value, workspace) && grad_token_stride >= 0 && grad_head_stride >= 0 &&
                      grad_token_stride % quantum == 0 && grad_head_stride % quantum == 0,

@@ -9,7 +9,7 @@ namespace attn {
 
 struct Args {
     sapa_attention a;
-    float scale_log2;              // scale * log2(e): the softmax runs in base 2
+    float scale_log2, scale_rest;  // scale * log2(e): the softmax runs in base 2; what its rounding left out
     int share;                     // query heads of a key head
     int split, least;              // > 0: items that the keys of all sequences are spread over, and tiles of an item at least, see Plan
     float *part, *part_lse;        // outputs of the parts of split sequences, float32
@@ -220,6 +220,9 @@ struct ForwardPlans {
         return Plan{order.at(index), 0x7fffffff / TILE, 0};
     }
 };
+
+// what rounding to T leaves out of a finite number
+template <typename T> __device__ __forceinline__ float left_out(float v) { return isfinite(v) ? v - to_acc(from_acc<T>(v)) : 0.f; }
 
 // Of a backward pass
 struct Grads {

@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
     begin_after_previous();
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
     if (a.lse != nullptr) clear_outside(a.lse, a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);
+    if (a.low != nullptr) clear_outside(static_cast<T *>(a.low), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
     auto meet = [&]() {
         tc_fence_before();
         __syncthreads();
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 const long long at = (long long)w->index * (tok * p.share) + (WIDE ? t * tile_tok * p.share : 0) + r;
                 const float inv = none ? 0.f : lost ? nan : split && sum == 0.f ? 0.f : 1.f / sum;
                 const int odd0 = w->odd_first, odd1 = w->odd_last;
-                const bool whole = whole_rows(a.out, a.dim);
+                const bool whole = whole_rows(a.out, a.dim) && whole_rows(a.low, a.dim);
                 // WIDE: all channels of this tile's row; otherwise each warpgroup half of them
                 constexpr int WIDTH = WIDE ? D : D / 2;
 #pragma unroll 1
@@ -623,6 +624,11 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     __syncwarp();
                     if (!split) {
                         store_rows(static_cast<T *>(a.out) + row * a.dim + c, mine, o, a.dim - c, whole);
+                        if (a.low != nullptr) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = left_out<T>(o[e]);
+                            store_rows(static_cast<T *>(a.low) + row * a.dim + c, mine, o, a.dim - c, whole);
+                        }
                     } else if (mine) {
                         float *to = p.part + at * a.dim + c;
 #pragma unroll

@@ -70,14 +70,14 @@ def test_sizes_and_types_without_a_kernel(call):
 
 # ---------------------------------------------------------------------------------- the C ABI
 class _Attention(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("query", "key", "value", "out", "lse", "offsets", "key_offsets", "page_table", "key_lengths")] +
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("query", "key", "value", "out", "lse", "low", "offsets", "key_offsets", "page_table", "key_lengths")] +
                 [("query_strides", ctypes.c_longlong * 2), ("key_strides", ctypes.c_longlong * 3), ("value_strides", ctypes.c_longlong * 3)] +
                 [(n, ctypes.c_int) for n in ("B", "tokens", "keys", "pages", "page", "max_pages", "heads", "groups", "dim", "causal")] +
                 [("scale", ctypes.c_float)])
 
 
 def _arguments(**kw):
-    a = _Attention(query=4096, key=4096, value=4096, out=4096, lse=4096, offsets=4096, key_offsets=4096, B=1, tokens=4, keys=4, heads=4, groups=2, dim=16, causal=1,
+    a = _Attention(query=4096, key=4096, value=4096, out=4096, lse=4096, low=4096, offsets=4096, key_offsets=4096, B=1, tokens=4, keys=4, heads=4, groups=2, dim=16, causal=1,
                    scale=1.0)
     a.query_strides[:] = (64, 16)
     a.key_strides[:] = a.value_strides[:] = (32, 16, 0)
@@ -114,7 +114,7 @@ def test_c_backward_refuses():
     def call(a, go=4096, stride=64, gq=4096, gk=4096, ws=4096, size=1 << 20):
         return h.sapa_attention_backward(ctypes.byref(a), go, stride, 16, gq, gk, 4096, ws, size, 0, None)
     assert call(_arguments(page_table=4096, key_lengths=4096, pages=1, page=1, max_pages=1)) == -5
-    assert call(_arguments(lse=0)) == -1 and call(_arguments(), go=0) == -1 and call(_arguments(), gq=0) == -1 and call(_arguments(), gk=0) == -1
+    assert call(_arguments(lse=0)) == -1 and call(_arguments(low=0)) == -1 and call(_arguments(), go=0) == -1 and call(_arguments(), gq=0) == -1 and call(_arguments(), gk=0) == -1
     assert call(_arguments(), stride=66) == -3 and call(_arguments(), go=4100) == -3
     assert call(_arguments(), size=8) == -6 and call(_arguments(), ws=0) == -6
     assert h.sapa_attention_forward(None, None, 0, 0, None) == -1

@@ -328,6 +328,28 @@ def test_scale_of_zero_is_the_mean(dtype):
     assert bool(sapa_b200.packed_attention(q, k, v, offsets_of([300]), scale=0.0)[100:, :2].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_infinite_scores(dtype):
+    """A score of -infinity has no weight, one of +infinity, or nothing but -infinity, makes a row NaN, as the formula does; gradients of the rest stay finite."""
+    q, k, v = (x.abs() for x in _inputs(200, 200, 2, 1, 64, TYPES[dtype]))
+    k = k.clone()
+    k[50, 0, 5] = -math.inf
+    out = sapa_b200.packed_attention(q, k, v, offsets_of([200]))
+    keep = [j for j in range(200) if j != 50]
+    assert bool(out.isfinite().all())
+    without = oracle.packed(q[150:], k[keep], v[keep], [50], [199], True, 0.125)      # rows from 150 on see all of the 199 up to their own
+    check(out[150:], without["out"], without["out_tol"])
+    qq, kk, vv = (x.clone().requires_grad_() for x in (q, k, v))
+    gq, gk, gv = torch.autograd.grad(sapa_b200.packed_attention(qq, kk, vv, offsets_of([200])).sum(), (qq, kk, vv))
+    assert bool(gq[:50].isfinite().all()) and bool(gk.isfinite().all()) and bool(gv.isfinite().all())
+    assert bool(gq[50:, :, 5].isnan().all()) and bool(gq[50:, :, 6].isfinite().all())      # 0 * infinity
+    k[50, 0, 5] = math.inf
+    out = sapa_b200.packed_attention(q, k, v, offsets_of([200]))
+    assert bool(out[:50].isfinite().all()) and bool(out[50:].isnan().all())
+    k[:, 0, 5] = -math.inf
+    assert bool(sapa_b200.packed_attention(q, k, v, offsets_of([200])).isnan().all())
+
+
 def test_which_kernels_serve():
     from sapa_b200 import _lib
     q, k, v = (x.requires_grad_() for x in _inputs(4000, 4000, 8, 2, 64, torch.bfloat16))
