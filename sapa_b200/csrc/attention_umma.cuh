@@ -26,9 +26,7 @@ using namespace ummau;
 
 constexpr int KT = TILE, ROWS = 128, BLOCK_BYTES = 128 * 128;         // keys of a tile, rows of a tile; 128 rows of 64 channels
 constexpr int MMA_WARP = 8, LOAD_WARP = 9, PLAN_WARP = 10, VALUE_WARP = 11, NT = 12 * 32;
-// registers a thread: 168 at launch, then what the softmax needs for a row of scores and the other four warps for theirs (multiples of 8)
-constexpr int REGS = 168, SOFTMAX_REGS = 208, OTHER_REGS = 88;
-static_assert(8 * 32 * SOFTMAX_REGS + 4 * 32 * OTHER_REGS <= NT * REGS, "a block draws on what it was launched with");
+constexpr int REGS = 168;                                             // a thread's at launch
 constexpr unsigned HI = (1024u >> 4) | (1u << 14) | (2u << 29);       // 8 rows of 128 bytes, descriptor version 1, 128-byte swizzle
 constexpr int BY_FMA = 1, BY_FMA_OF = 4;                              // exponentials that the FMA units take over
 constexpr float GROWTH = 8.f;                                         // powers of two
@@ -39,6 +37,10 @@ template <int D, bool WIDE> struct Lay {
     static constexpr int Q0 = 0, KV0 = Q_BYTES;
     static constexpr int NEED = KV0 + NST * STAGE + 1024, SMEM = NEED < 120 * 1024 ? 120 * 1024 : NEED;      // one block an SM: tensor memory
     static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
+    // registers a thread: what the softmax needs for a row of scores (with 208 narrow blocks keep 500 bytes of it in memory: single tokens over 209 thousand keys
+    // 157 us, 150 with 224; four prompts of up to 100 tokens, in wide blocks, 8.8 us with 208, 9.5 with 224), the rest for the other four warps; multiples of 8
+    static constexpr int SOFTMAX_REGS = WIDE ? 208 : 224, OTHER_REGS = WIDE ? 88 : 56;
+    static_assert(8 * 32 * SOFTMAX_REGS + 4 * 32 * OTHER_REGS <= NT * REGS, "a block draws on what it was launched with");
     // whether the second product begins with half of a tile's weights.  In 64 channels it is short, and waiting for the stores twice costs more than that
     // gains: one prompt of 8192 tokens, 32 heads, bfloat16: 64 channels 358 us with halves, 330 without; 128 channels 410 and 428.
     static constexpr bool HALVES = D == 128;
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
     };
 
     if (warp >= MMA_WARP) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(OTHER_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::OTHER_REGS));
         if (warp == PLAN_WARP) {
             ForwardPlans plans(p, tok, lane);
             for (int round = 0;; ++round) {
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(SOFTMAX_REGS));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(L::SOFTMAX_REGS));
         const int t = warp >> 2, r = tid & 127;
         const unsigned quarter = (unsigned)((warp & 3) * 32) << 16;
         const unsigned s_at = tmem + quarter + L::S_COL + t * KT, o_at = tmem + quarter + L::O_COL + t * D;
@@ -623,11 +625,13 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     }
                     __syncwarp();
                     if (!split) {
-                        store_rows(static_cast<T *>(a.out) + row * a.dim + c, mine, o, a.dim - c, whole);
-                        if (a.low != nullptr) {
+                        T *to = static_cast<T *>(a.out);
+#pragma unroll 1
+                        for (int pass = a.low != nullptr ? 0 : 1; pass < 2; ++pass) {      // out, and what its rounding leaves out
+                            store_rows(to + row * a.dim + c, mine, o, a.dim - c, whole);
+                            to = static_cast<T *>(a.low);
 #pragma unroll
                             for (int e = 0; e < 32; ++e) o[e] = left_out<T>(o[e]);
-                            store_rows(static_cast<T *>(a.low) + row * a.dim + c, mine, o, a.dim - c, whole);
                         }
                     } else if (mine) {
                         float *to = p.part + at * a.dim + c;
