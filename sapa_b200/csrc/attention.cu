@@ -273,17 +273,16 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
 
 // Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(lse_p - max lse).  Grid: a block and group, 16 of its rows; a warp per row, whose
 // lanes first weigh the parts and then take 4 channels each, of every part or (up to 64 channels) of every other one.  Bound by the latency of its few
-// loads: eight parts are on their way at once, and the rows' places are found before the forward has ended.
+// loads: eight parts are on their way at once.
 template <typename T>
 __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_constant__ Args p, int bm, int tok) {
     const sapa_attention &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x % a.groups, D = a.dim;
     const int ways = D <= 64 ? 2 : 1, way = D <= 64 ? lane >> 4 : 0, c = 4 * (D <= 64 ? lane & 15 : lane);
-    // what it reads here came before the forward, which began behind it
-    const Plan plan = split_at<false>(p, blockIdx.x / a.groups, tok, part_tiles(p, tok, lane), lane);
-    const Sequence s = sequence_at(a, plan.it.there ? plan.it.b : 0);
     begin_after_previous();
+    const Plan plan = split_at<false>(p, blockIdx.x / a.groups, tok, part_tiles(p, tok, lane), lane);
     if (!plan.it.there || plan.it.parts == 1) return;
+    const Sequence s = sequence_at(a, plan.it.b);
     const int first = plan.it.block * tok, used = min(tok, s.nq - first) * p.share, parts = plan.it.parts;
     const long long step = (long long)a.groups * bm;                                  // from a part to the next
     for (int r = blockIdx.y * 16 + warp; r < min(used, (int)blockIdx.y * 16 + 16); r += 8) {

@@ -53,13 +53,13 @@ template <auto *KERNEL, int REGISTERS> static int check_registers(const char *na
     return SAPA_OK;
 }
 
-template <typename T, int D, bool WIDE, bool PAGED>
+template <typename T, int D, bool WIDE, bool PAGED, bool LOW>
 static int launch(const Args &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, long long items, cudaStream_t st) {
     using L = um::Lay<D, WIDE>;
     int sms = 0;
-    if (int e = prepare_launch((const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED>, L::SMEM, "sapa_attention_umma_kernel", sms)) return e;
-    if (int e = check_registers<sapa_attention_umma_kernel<T, D, WIDE, PAGED>, REGS>("sapa_attention_umma_kernel")) return e;
-    launch_next(sapa_attention_umma_kernel<T, D, WIDE, PAGED>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), L::SMEM, st, q, k, v, p, (int)items);
+    if (int e = prepare_launch((const void *)sapa_attention_umma_kernel<T, D, WIDE, PAGED, LOW>, L::SMEM, "sapa_attention_umma_kernel", sms)) return e;
+    if (int e = check_registers<sapa_attention_umma_kernel<T, D, WIDE, PAGED, LOW>, REGS>("sapa_attention_umma_kernel")) return e;
+    launch_next(sapa_attention_umma_kernel<T, D, WIDE, PAGED, LOW>, dim3((unsigned)(items < sms ? items : sms)), dim3(um::NT), L::SMEM, st, q, k, v, p, (int)items);
     return check_launch(WIDE ? "sapa_attention_umma_kernel<wide>" : "sapa_attention_umma_kernel<narrow>");
 }
 
@@ -86,14 +86,18 @@ int umma_forward(const Args &p, bool wide, long long items, int dtype, cudaStrea
     const int kb[3] = {1, paged ? rows : KT, 1};
     good = good && encode(&k, a.key, a.dim, paged ? 3 : 2, kd, ks, kb, half) && encode(&v, a.value, a.dim, paged ? 3 : 2, kd, vs, kb, half);
     SAPA_REQUIRE(good, SAPA_ERR_LAUNCH, "sapa_attention_forward: cuTensorMapEncodeTiled failed (%d)", last_encode_result());
-    auto pick = [&](auto t) -> int {
+    auto run = [&](auto t, auto d, auto w) -> int {
         using T = decltype(t);
-        if (a.dim <= 64) {
-            if (wide) return paged ? launch<T, 64, true, true>(p, q, k, v, items, st) : launch<T, 64, true, false>(p, q, k, v, items, st);
-            return paged ? launch<T, 64, false, true>(p, q, k, v, items, st) : launch<T, 64, false, false>(p, q, k, v, items, st);
-        }
-        if (wide) return paged ? launch<T, 128, true, true>(p, q, k, v, items, st) : launch<T, 128, true, false>(p, q, k, v, items, st);
-        return paged ? launch<T, 128, false, true>(p, q, k, v, items, st) : launch<T, 128, false, false>(p, q, k, v, items, st);
+        constexpr int D = decltype(d)::value;
+        constexpr bool W = decltype(w)::value;
+        if (paged) return launch<T, D, W, true, false>(p, q, k, v, items, st);
+        return a.low != nullptr ? launch<T, D, W, false, true>(p, q, k, v, items, st) : launch<T, D, W, false, false>(p, q, k, v, items, st);
+    };
+    auto pick = [&](auto t) -> int {
+        using Narrow = std::integral_constant<int, 64>;
+        using Wide = std::integral_constant<int, 128>;
+        if (a.dim <= 64) return wide ? run(t, Narrow(), std::true_type()) : run(t, Narrow(), std::false_type());
+        return wide ? run(t, Wide(), std::true_type()) : run(t, Wide(), std::false_type());
     };
     return half ? pick(__half()) : pick(__nv_bfloat16());
 }

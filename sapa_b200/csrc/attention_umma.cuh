@@ -125,7 +125,6 @@ template <typename T> __device__ __forceinline__ float2 ex2_by_fma(float2 x) {
     y = fma2(f, y, make_float2(1.f, 1.f));
     return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap *map, unsigned bar, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
@@ -195,7 +194,8 @@ __device__ __forceinline__ bool whole_rows(const void *base, int dim) { return d
 
 }  // namespace um
 
-template <typename T, int D, bool WIDE, bool PAGED>
+// LOW: stores what the rounding of the outputs leaves out too.
+template <typename T, int D, bool WIDE, bool PAGED, bool LOW>
 __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                                                                         const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args p, const int most_items) {
     using namespace um;
@@ -225,11 +225,10 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
         tc_alloc((unsigned)__cvta_generic_to_shared(&tmem_slot), L::TMEM_COLS);
         tc_relinquish();
     }
-    if (warp == LOAD_WARP && lane < 3) prefetch_map(lane == 0 ? &qmap : lane == 1 ? &kmap : &vmap);
     begin_after_previous();
     clear_outside(static_cast<T *>(a.out), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
     if (a.lse != nullptr) clear_outside(a.lse, a.offsets, a.B, a.tokens, a.heads, blockIdx.x, gridDim.x, tid, NT);
-    if (a.low != nullptr) clear_outside(static_cast<T *>(a.low), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
+    if (LOW) clear_outside(static_cast<T *>(a.low), a.offsets, a.B, a.tokens, a.heads * a.dim, blockIdx.x, gridDim.x, tid, NT);
     auto meet = [&]() {
         tc_fence_before();
         __syncthreads();
@@ -589,7 +588,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 const long long at = (long long)w->index * (tok * p.share) + (WIDE ? t * tile_tok * p.share : 0) + r;
                 const float inv = none ? 0.f : lost ? nan : split && sum == 0.f ? 0.f : 1.f / sum;
                 const int odd0 = w->odd_first, odd1 = w->odd_last;
-                const bool whole = whole_rows(a.out, a.dim) && whole_rows(a.low, a.dim);
+                const bool whole = whole_rows(a.out, a.dim) && (!LOW || whole_rows(a.low, a.dim));
                 // WIDE: all channels of this tile's row; otherwise each warpgroup half of them
                 constexpr int WIDTH = WIDE ? D : D / 2;
 #pragma unroll 1
@@ -625,13 +624,11 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     }
                     __syncwarp();
                     if (!split) {
-                        T *to = static_cast<T *>(a.out);
-#pragma unroll 1
-                        for (int pass = a.low != nullptr ? 0 : 1; pass < 2; ++pass) {      // out, and what its rounding leaves out
-                            store_rows(to + row * a.dim + c, mine, o, a.dim - c, whole);
-                            to = static_cast<T *>(a.low);
+                        store_rows(static_cast<T *>(a.out) + row * a.dim + c, mine, o, a.dim - c, whole);
+                        if (LOW) {
 #pragma unroll
                             for (int e = 0; e < 32; ++e) o[e] = left_out<T>(o[e]);
+                            store_rows(static_cast<T *>(a.low) + row * a.dim + c, mine, o, a.dim - c, whole);
                         }
                     } else if (mine) {
                         float *to = p.part + at * a.dim + c;

@@ -127,7 +127,6 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(base + L::ST0 + tile * L::BOX + (rows + e / 8) * 128 + (e % 8) * 16), "r"(0u) : "memory");
         }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    if (warp == LOAD && lane < 4) prefetch_map(lane == 0 ? &own0 : lane == 1 ? &own1 : lane == 2 ? &over0 : &over1);
     begin_after_previous();
     auto meet = [&]() {
         tc_fence_before();
