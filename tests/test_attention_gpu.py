@@ -58,6 +58,22 @@ def test_keys_of_other_lengths(lengths, keys, causal, dtype):
         check(g, want[name], want[name + "_tol"])
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_mostly_padding(dtype):
+    """Two short sequences somewhere in a large padded tensor full of NaN: zeros around them, in the outputs and in every gradient."""
+    T, start, lengths = 3001, 700, [5, 40]
+    q, k, v = (x.requires_grad_() for x in _inputs(T, T, 6, 3, 40, TYPES[dtype]))
+    go = _made((T, 6, 40), TYPES[dtype], 9)
+    with torch.no_grad():
+        for x in (q, k, v, go):
+            x[:start] = x[start + 45:] = math.nan
+    out = sapa_b200.packed_attention(q, k, v, offsets_of(lengths, start))
+    want = oracle.packed(q.detach(), k.detach(), v.detach(), lengths, lengths, True, 40 ** -0.5, go, start, start)
+    check(out.detach(), want["out"], want["out_tol"])
+    for name, g in zip(("gq", "gk", "gv"), torch.autograd.grad(out, (q, k, v), go)):
+        check(g, want[name], want[name + "_tol"])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides(dtype):
     """Parts of one projection's output, heads before tokens, an unaligned view, and broadcast heads: the numbers of dense tensors."""
