@@ -210,33 +210,42 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
         }
         __syncwarp();                          // the 16 threads that share a row are in one warp
         if (!careful) {
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {      // a tile by itself and then to the sum: fewer roundings at the sum's size (over 1500 keys half the error)
+                float4 t[RI];
+#pragma unroll
+                for (int i = 0; i < RI; ++i) t[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-            for (int k = 0; k < KT; k += 4) {
-                float4 w[RI];
+                for (int k = 0; k < KT; k += 4) {
+                    float4 w[RI];
 #pragma unroll
-                for (int i = 0; i < RI; ++i) w[i] = *reinterpret_cast<const float4 *>(sm + L::P0 + (ty + 16 * i) * L::PS + k);
+                    for (int i = 0; i < RI; ++i) w[i] = *reinterpret_cast<const float4 *>(sm + L::P0 + (ty + 16 * i) * L::PS + k);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int j = 0; j < DP / 64; ++j) {
+                    for (int e = 0; e < 4; ++e) {
                         const float4 v = *reinterpret_cast<const float4 *>(sm + L::V0 + (k + e) * DP + 4 * tx + 64 * j);
 #pragma unroll
                         for (int i = 0; i < RI; ++i) {
                             const float x = at(w[i], e);
-                            o[i][4 * j] = fmaf(x, v.x, o[i][4 * j]); o[i][4 * j + 1] = fmaf(x, v.y, o[i][4 * j + 1]);
-                            o[i][4 * j + 2] = fmaf(x, v.z, o[i][4 * j + 2]); o[i][4 * j + 3] = fmaf(x, v.w, o[i][4 * j + 3]);
+                            t[i].x = fmaf(x, v.x, t[i].x); t[i].y = fmaf(x, v.y, t[i].y); t[i].z = fmaf(x, v.z, t[i].z); t[i].w = fmaf(x, v.w, t[i].w);
                         }
                     }
+                }
+#pragma unroll
+                for (int i = 0; i < RI; ++i) { o[i][4 * j] += t[i].x; o[i][4 * j + 1] += t[i].y; o[i][4 * j + 2] += t[i].z; o[i][4 * j + 3] += t[i].w; }
             }
         } else {
-            for (int k = 0; k < n; ++k)
+#pragma unroll 1
+            for (int c = 0; c < DP / 16; ++c) {
+                const int at = 4 * tx + 64 * (c >> 2) + (c & 3);
 #pragma unroll
-                for (int i = 0; i < RI; ++i)
-                    if (k0 + k < lim[i]) {
-                        const float w = sm[L::P0 + (ty + 16 * i) * L::PS + k];
+                for (int i = 0; i < RI; ++i) {
+                    float t = 0.f;
+                    for (int k = 0; k < n; ++k)
+                        if (k0 + k < lim[i]) t = fmaf(sm[L::P0 + (ty + 16 * i) * L::PS + k], sm[L::V0 + k * DP + at], t);
 #pragma unroll
-                        for (int c = 0; c < DP / 16; ++c) o[i][c] = fmaf(w, sm[L::V0 + k * DP + 4 * tx + 64 * (c >> 2) + (c & 3)], o[i][c]);
-                    }
+                    for (int e = 0; e < DP / 16; ++e) o[i][e] += e == c ? t : 0.f;
+                }
+            }
         }
     }
     __syncthreads();
@@ -266,12 +275,12 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
             for (int j = 0; j < DP / 64; ++j)
                 if (4 * tx + 64 * j < D)
                     store4(p.part + at * D + 4 * tx + 64 * j, make_float4(o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv));
-            if (tx == 0) p.part_lse[at] = lost ? nan : sum == 0.f ? -INFINITY : m[i] + log2f(sum);
+            if (tx == 0) p.part_sums[at] = make_float2(sum == 0.f ? -INFINITY : m[i], lost ? nan : sum);
         }
     }
 }
 
-// Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(lse_p - max lse).  Grid: a block and group, 16 of its rows; a warp per row, whose
+// Joins the parts of the split sequences: out = sum w_p out_p / sum w_p, w_p = 2^(m_p - max m) times the part's sum (lse_p as one number would be rounded).  Grid: a block and group, 16 of its rows; a warp per row, whose
 // lanes first weigh the parts and then take 4 channels each, of every part or (up to 64 channels) of every other one.  Bound by the latency of its few
 // loads: eight parts are on their way at once.
 template <typename T>
@@ -290,7 +299,7 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
         const int lim = sees(s, first + r / p.share, a.causal);
         float top = -INFINITY;
         bool lost = false;
-        for (int q = lane; q < parts; q += 32) { const float e = p.part_lse[at + q * step]; top = fmaxf(top, e); lost = lost || e != e; }
+        for (int q = lane; q < parts; q += 32) { const float2 e = p.part_sums[at + q * step]; top = fmaxf(top, e.x); lost = lost || e.y != e.y; }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         lost = __any_sync(0xffffffffu, lost) || (lim > 0 && top == -INFINITY);
@@ -298,8 +307,8 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         const float *from = p.part + at * D + c;
         for (int q0 = 0; q0 < parts; q0 += 32) {
-            const float e = q0 + lane < parts ? p.part_lse[at + (q0 + lane) * step] : -INFINITY;
-            const float mine = e == -INFINITY ? 0.f : exp2f(e - top);
+            const float2 e = q0 + lane < parts ? p.part_sums[at + (q0 + lane) * step] : make_float2(-INFINITY, 0.f);
+            const float mine = e.x == -INFINITY ? 0.f : exp2f(e.x - top) * e.y;
             const int n = min(32, parts - q0);
             for (int q = 0; q < n; q += 8 * ways) {
                 float4 v[8];
@@ -738,7 +747,7 @@ static Shape shape_of(const Args &p, int dtype, int sms) {
         s.split = (s.umma ? (s.narrow ? 2 : 3) : 4) * sms;
         s.grid = s.blocks + s.split;
         s.part = (size_t)s.grid * s.bm * a.dim * sizeof(float);
-        s.lse = (size_t)s.grid * s.bm * sizeof(float);
+        s.lse = (size_t)s.grid * s.bm * sizeof(float2);
         s.bytes = (s.part + s.lse + 255) / 256 * 256;
     }
     return s;
@@ -793,7 +802,7 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
         p.split = s.split;
         p.least = s.umma ? 4 : 1;
         p.part = static_cast<float *>(workspace);
-        p.part_lse = reinterpret_cast<float *>(static_cast<char *>(workspace) + s.part);
+        p.part_sums = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + s.part);
     }
     return SAPA_DISPATCH_FAST(dtype, [&]() -> int {
         int e;

@@ -12,7 +12,8 @@ struct Args {
     float scale_log2, scale_rest;  // scale * log2(e): the softmax runs in base 2; what its rounding left out
     int share;                     // query heads of a key head
     int split, least;              // > 0: items that the keys of all sequences are spread over, and tiles of an item at least, see Plan
-    float *part, *part_lse;        // outputs of the parts of split sequences, float32
+    float *part;                   // outputs of the parts of split sequences, float32
+    float2 *part_sums;             // their maxima and sums, in base 2
 };
 
 // Tokens and keys of a sequence, within the tensors whatever the offsets say.

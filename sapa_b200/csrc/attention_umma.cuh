@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 }
                 if (mine && (WIDE || t == 0)) {
                     const float log = none || (split && sum == 0.f) ? -INFINITY : lost || sum == 0.f ? nan : m + log2f(sum);
-                    if (split) p.part_lse[at] = lost ? nan : log;
+                    if (split) p.part_sums[at] = make_float2(none || sum == 0.f ? -INFINITY : m, none ? 0.f : lost ? nan : sum);
                     else if (a.lse != nullptr) a.lse[row] = log * 0.6931471805599453f;
                 }
             }
