@@ -2,7 +2,7 @@
 //
 // A block an SM, items in turn: 128-row tiles (row = token x query head of one key head) against tiles of 128 keys.
 //   * a warp finds the items, one ahead (they follow from lengths that only the device knows);
-//   * a warp loads queries, keys and values with TMA (rows of 64 channels, 128-byte swizzle; of a paged cache a box a page);
+//   * a warp loads queries and keys, another the values, with TMA (rows of 64 channels, 128-byte swizzle; of a paged cache a box a page);
 //   * a warp issues S = Q K^T (both operands K-major in shared memory) and O += P V (P in tensor memory, V as TMA lands it, MN-major);
 //   * a warpgroup for each of two S / O accumulators: a thread holds a row, 128 scores in registers, so maximum and sum need no shuffles; it writes P,
 //     rounded to the type of V as the second product takes it, over S.  The sum is of the weights before that rounding.
@@ -10,6 +10,9 @@
 // odd key tiles, joined at the end (single tokens and short chunks): while one's softmax runs, the other's products do.
 // O is scaled again only when a row's maximum has grown by more than 2^8 since it last was: weights stay below 2^8 and the sums exact enough, and
 // the warpgroup that owns S owns O too at that time, for S was computed behind the product that last added to O.
+// What bounds it: of long prompts the tensor pipe between the two softmaxes, the exponentials (a quarter of them by FMA units) and
+// the power limit (8192 tokens, 32 heads of 128 channels, causal, bfloat16: 410 us, 1.34 PFLOP/s); of short ones the tiles on the diagonal and an item's start
+// and end; of single tokens reading the cache (209 thousand keys, 8 key heads of 128 channels: 131 us at the copy rate, 150 warm).
 // What a row does not see: its scores are set to -infinity; a value that is not finite would still reach its output as 0 * infinity.  So in tiles that not
 // every row sees whole, what is not finite among the values is replaced with 0 in front of the product, and added to the outputs of the rows that see it.
 #pragma once

@@ -7,10 +7,10 @@
 //     the lanes of tensor memory, so that P^T and dS^T are first operands of dV += P^T dO and dK += dS^T Q as they are;
 //   * otherwise an item holds 128 rows and goes over the keys that they see: S = Q K^T, dP = dO V^T, dQ += dS K.
 // Seven products where five would do with dQ summed by atomics; each operand is in shared memory once, K-major for one product and MN-major for another.
-// What is gone over comes in tiles of 64, so that tensor memory holds S and dP of two: a warpgroup each takes every other tile (a thread a lane, 64 columns) while
+// What is gone over comes in tiles of 64, so that tensor memory holds S and dP of two: two warpgroups take every other tile (a thread a lane, 32 columns) while
 // the products of the other one run, and the item's own operands are in tensor memory.  Those of keys in 128 channels find no room there, and products of
 // 128 x 64 that read both operands from shared memory take 6 KB of it every 32 clocks, more than it gives (128 bytes a clock): there the tiles are of 128, and
-// the warpgroups take half of the columns each (BOTH).  A block an SM goes through its items, as the forward does.
+// the four warpgroups take a quarter of the columns each (BOTH).  A block an SM goes through its items, as the forward does.
 // What a row does not see: P and dS are 0 there, and 0 * infinity must not reach a gradient.  In tiles that are not seen whole, what is not finite in the
 // operand behind P or dS is replaced with 0 once the products that need it as it is have read it.  Values that are not finite in a row of dO are
 // added to the gradients of the values that it sees; those of keys that a row sees make its gradient NaN; a row of Q makes its P NaN by itself.
