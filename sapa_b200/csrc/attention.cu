@@ -398,6 +398,21 @@ __device__ __forceinline__ bool team_or(int team, bool v) {
     asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"(1 + team), "r"((unsigned)v) : "memory");
     return any != 0;
 }
+// all threads of the blocks of a cluster; what they wrote before is seen after it, in each other's shared memory too
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// shared memory of another block of the cluster, at the place of `own` here
+__device__ __forceinline__ unsigned in_block(const float *own, int rank) {
+    unsigned at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(own)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float load_far(unsigned at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
 }  // namespace grad
 
 // float32.  KEYS: gradients of 32 keys and values, over the rows (token x head of a key head) that see them; otherwise those of 32 query rows, over the keys
@@ -405,8 +420,8 @@ __device__ __forceinline__ bool team_or(int team, bool v) {
 // 128 threads take the tiles in turn and add up at the end: a team by itself waits most of the time (1342 tokens, 8 heads of 64 channels: keys 164 us).
 // Threads of a team as 8 x 16: of S and dP the rows ty + 8 i and the columns tx + 16 j, of the sums the rows 4 ty + i and the channels 4 tx + 64 j.
 // What bounds it: the FP32 pipe, in small problems the longest block.
-template <int DP, bool KEYS>
-__global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
+template <int DP, bool KEYS, bool SHARED>
+__global__ void __launch_bounds__(grad::THREADS, 1) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     using namespace grad;
     using T = float;
     using L = grad::Lay<DP>;
@@ -418,6 +433,7 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
     constexpr int ROWS = KEYS ? OVER : OWN;                                                   // of a tile of rows
     const int share = p.share, at_once = min(share, ROWS), tok = ROWS / at_once, turns = (share + at_once - 1) / at_once;      // more heads than rows: in turns
     const int slots = KEYS ? a.groups : a.groups * turns, slot = blockIdx.x % slots, group = slot % a.groups;
+    const int rank = SHARED ? blockIdx.y : 0, ranks = SHARED ? gridDim.y : 1;      // SHARED: the blocks of a cluster share an item's tiles
     begin_after_previous();
     if (threadIdx.x < 32) {
         const Item r = KEYS ? InOrder<false, KeyBlocks>(a, KeyBlocks{a.causal != 0, tok, OWN}, tid).at(blockIdx.x / slots)
@@ -565,7 +581,7 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
         __syncthreads();
         const int from = a.causal ? (int)max(0ll, (long long)first - s.nk + s.nq) : 0;      // the first token that sees one of them
         const int tiles = from < s.nq ? tiles_of(s.nq - from, tok) * turns : 0;
-        for (int i = team; i < tiles; i += TEAMS) {
+        for (int i = rank * TEAMS + team; i < tiles; i += ranks * TEAMS) {
             const int i0 = from + i / turns * tok, h0 = i % turns * at_once, used = min(tok, s.nq - i0) * at_once;
             team_sync(team);
             const bool odd = load(mine + L::B0, mine + L::B1, mine + L::LB, OVER, tid, TEAM, false, 0, i0, h0, used);
@@ -576,15 +592,14 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
         const int tiles = tiles_of(sees(s, first + used / at_once - 1, a.causal), OVER);
         load(sm + L::A0, sm + L::A1, sm + L::LA, OWN, threadIdx.x, THREADS, false, 0, first, h0, used);
         __syncthreads();
-        for (int i = team; i < tiles; i += TEAMS) {
+        for (int i = rank * TEAMS + team; i < tiles; i += ranks * TEAMS) {
             team_sync(team);
             const bool odd = load(mine + L::B0, mine + L::B1, nullptr, OVER, tid, TEAM, true, i * OVER, 0, 0, 0);
             tile(first, h0, used, i * OVER, odd);
         }
     }
-    // the teams' sums, in their order, through their tiles
-    team_sync(team);
-    if (team != 0)
+    // the teams' sums, in their order, through their tiles; then those of the cluster's blocks
+    auto hand_over = [&]() {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -592,18 +607,39 @@ __global__ void __launch_bounds__(grad::THREADS) sapa_attention_rows_grad_kernel
                 mine[(i * (DP / 16) + c) * TEAM + tid] = y[i][c];
                 if (KEYS) mine[(4 * (DP / 16) + i * (DP / 16) + c) * TEAM + tid] = x[i][c];
             }
-    __syncthreads();
-    if (team != 0) return;
-#pragma unroll 1
-    for (int q = 1; q < TEAMS; ++q) {
-        const float *const other = sm + L::TEAM0 + q * L::EACH;
+    };
+    auto add = [&](auto sum_of) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) {
-                y[i][c] += other[(i * (DP / 16) + c) * TEAM + tid];
-                if (KEYS) x[i][c] += other[(4 * (DP / 16) + i * (DP / 16) + c) * TEAM + tid];
+                y[i][c] += sum_of(i * (DP / 16) + c);
+                if (KEYS) x[i][c] += sum_of(4 * (DP / 16) + i * (DP / 16) + c);
             }
+    };
+    team_sync(team);
+    if (team != 0) hand_over();
+    __syncthreads();
+    if (!SHARED && team != 0) return;
+    if (!SHARED || team == 0) {
+#pragma unroll 1
+        for (int q = 1; q < TEAMS; ++q) {
+            const float *const other = sm + L::TEAM0 + q * L::EACH + tid;
+            add([&](int i) { return other[i * TEAM]; });
+        }
+        if (SHARED && rank != 0) hand_over();
+    }
+    if (SHARED) {
+        cluster_sync();
+        if (team + rank == 0) {
+#pragma unroll 1
+            for (int q = 1; q < ranks; ++q) {
+                const unsigned other = in_block(mine + tid, q);
+                add([&](int i) { return load_far(other + 4u * TEAM * i); });
+            }
+        }
+        cluster_sync();                        // the other blocks' memory is there until it has been read
+        if (team + rank != 0) return;
     }
     // the scores' scale is in the gradients of queries and keys
 #pragma unroll
@@ -763,13 +799,37 @@ template <typename T, int RI, int DP> static int run_rows(const Args &p, const S
     return check_launch("sapa_attention_rows_kernel");
 }
 
-template <int DP, bool KEYS> static int run_grad(const Args &p, const Grads &g, long long blocks, cudaStream_t st) {
+template <int DP, bool KEYS, bool SHARED> static int run_grad_by(const Args &p, const Grads &g, long long blocks, int ranks, cudaStream_t st) {
     using L = grad::Lay<DP>;
     int sms = 0;
-    if (blocks == 0) return SAPA_OK;
-    if (int e = tmau::prepare_launch((const void *)sapa_attention_rows_grad_kernel<DP, KEYS>, (int)L::SMEM, "sapa_attention_rows_grad_kernel", sms)) return e;
-    launch_next(sapa_attention_rows_grad_kernel<DP, KEYS>, dim3((unsigned)blocks), dim3(grad::THREADS), L::SMEM, st, p, g);
+    const auto kernel = sapa_attention_rows_grad_kernel<DP, KEYS, SHARED>;
+    if (int e = tmau::prepare_launch((const void *)kernel, (int)L::SMEM, "sapa_attention_rows_grad_kernel", sms)) return e;
+    if (SHARED) {                                    // launch_next, with a cluster
+        cudaLaunchAttribute attributes[2];
+        attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[0].val.programmaticStreamSerializationAllowed = 1;
+        attributes[1].id = cudaLaunchAttributeClusterDimension;
+        attributes[1].val.clusterDim.x = attributes[1].val.clusterDim.z = 1;
+        attributes[1].val.clusterDim.y = (unsigned)ranks;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3((unsigned)blocks, (unsigned)ranks); config.blockDim = dim3(grad::THREADS); config.dynamicSmemBytes = L::SMEM; config.stream = st;
+        config.attrs = attributes; config.numAttrs = 2;
+        (void)cudaLaunchKernelEx(&config, kernel, p, g);      // a failure is what check_launch reads
+    } else {
+        launch_next(kernel, dim3((unsigned)blocks), dim3(grad::THREADS), L::SMEM, st, p, g);
+    }
     return check_launch(KEYS ? "sapa_attention_rows_grad_kernel<keys>" : "sapa_attention_rows_grad_kernel<queries>");
+}
+// Fewer blocks than SMs, and more tiles to an average sequence than a block has teams: clusters of 2 or 4 blocks share the tiles of one.  One sequence of 1000
+// tokens, 4 heads of 128 channels, forward and gradients: 397 us without, 289 with two blocks; of 500, 4 / 2 heads of 64: 164, 109 with up to two, 97 with up
+// to four.  With more blocks than SMs nothing is left to share: four sequences of up to 300 tokens, 16 / 8 heads of 64 channels, 148 and 170 (keys alone shared).
+template <int DP, bool KEYS> static int run_grad(const Args &p, const Grads &g, long long blocks, int sms, cudaStream_t st) {
+    const sapa_attention &a = p.a;
+    if (blocks == 0) return SAPA_OK;
+    const long long tiles = (KEYS ? (long long)a.tokens * p.share : a.keys) / grad::OVER / (a.B > 0 ? a.B : 1);
+    int ranks = 1;
+    while (ranks < 4 && blocks * ranks <= sms && tiles > ranks * grad::TEAMS) ranks *= 2;
+    return ranks > 1 ? run_grad_by<DP, KEYS, true>(p, g, blocks, ranks, st) : run_grad_by<DP, KEYS, false>(p, g, blocks, 1, st);
 }
 
 }  // namespace attn
@@ -861,11 +921,11 @@ extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad
         if (int e = check_launch("sapa_attention_delta_kernel")) return e;
         if (umma) return umma_backward(p, g, dtype, st);
         if (a->dim <= 64) {
-            if (int e = run_grad<64, true>(p, g, key_blocks, st)) return e;
-            return run_grad<64, false>(p, g, query_blocks, st);
+            if (int e = run_grad<64, true>(p, g, key_blocks, sms, st)) return e;
+            return run_grad<64, false>(p, g, query_blocks, sms, st);
         }
-        if (int e = run_grad<128, true>(p, g, key_blocks, st)) return e;
-        return run_grad<128, false>(p, g, query_blocks, st);
+        if (int e = run_grad<128, true>(p, g, key_blocks, sms, st)) return e;
+        return run_grad<128, false>(p, g, query_blocks, sms, st);
     });
 }
 

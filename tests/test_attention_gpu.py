@@ -318,6 +318,20 @@ def test_prompt_then_tokens(dtype):
         lo, hi = hi, [min(n, h + 1) for n, h in zip(total, hi)]
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("tokens, keys, heads, groups, dim", [(1000, 1000, 4, 4, 128), (385, 385, 4, 2, 64), (150, 611, 2, 1, 72), (611, 129, 3, 1, 24), (40, 9000, 1, 1, 64), (9000, 40, 1, 1, 64)])
+def test_gradients_of_few_long_sequences(tokens, keys, heads, groups, dim, causal):
+    """float32: blocks in clusters share the tiles of one item, so there are several sums to join; twice the same bits."""
+    q, k, v = (t.requires_grad_() for t in _inputs(tokens, keys, heads, groups, dim, torch.float32))
+    go = _made((tokens, heads, dim), torch.float32, 9)
+    out = sapa_b200.packed_attention(q, k, v, offsets_of([tokens]), offsets_of([keys]), causal=causal)
+    want = oracle.packed(q.detach(), k.detach(), v.detach(), [tokens], [keys], causal, 1 / math.sqrt(dim), go)
+    first = torch.autograd.grad(out, (q, k, v), go, retain_graph=True)
+    for name, g, again in zip(("gq", "gk", "gv"), first, torch.autograd.grad(out, (q, k, v), go)):
+        check(g, want[name], want[name + "_tol"])
+        assert torch.equal(g, again)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_more_sequences_than_are_sorted(dtype):
     """Hundreds of sequences, some empty, forward, backward and over a cache."""
