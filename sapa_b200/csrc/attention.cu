@@ -419,7 +419,7 @@ __device__ __forceinline__ float load_far(unsigned at) {
 // that they see.  P and dS of a tile of 32 are formed again from the scores, lse and delta: P = 2^(s - lse), dS = P (dP - delta); no atomics.  Four teams of
 // 128 threads take the tiles in turn and add up at the end: a team by itself waits most of the time (1342 tokens, 8 heads of 64 channels: keys 164 us).
 // Threads of a team as 8 x 16: of S and dP the rows ty + 8 i and the columns tx + 16 j, of the sums the rows 4 ty + i and the channels 4 tx + 64 j.
-// What bounds it: the FP32 pipe, in small problems the longest block.
+// What bounds it: the FP32 pipe and the shared-memory reads beside it, in small problems the longest item: with SHARED the blocks of a cluster take its tiles in turn.
 template <int DP, bool KEYS, bool SHARED>
 __global__ void __launch_bounds__(grad::THREADS, 1) sapa_attention_rows_grad_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     using namespace grad;
@@ -820,15 +820,17 @@ template <int DP, bool KEYS, bool SHARED> static int run_grad_by(const Args &p, 
     }
     return check_launch(KEYS ? "sapa_attention_rows_grad_kernel<keys>" : "sapa_attention_rows_grad_kernel<queries>");
 }
-// Fewer blocks than SMs, and more tiles to an average sequence than a block has teams: clusters of 2 or 4 blocks share the tiles of one.  One sequence of 1000
-// tokens, 4 heads of 128 channels, forward and gradients: 397 us without, 289 with two blocks; of 500, 4 / 2 heads of 64: 164, 109 with up to two, 97 with up
-// to four.  With more blocks than SMs nothing is left to share: four sequences of up to 300 tokens, 16 / 8 heads of 64 channels, 148 and 170 (keys alone shared).
+// Hardly more blocks than SMs (the longest decide), and a team's turn of an average sequence more than two tiles: clusters of 2 or 4 blocks share the tiles of
+// one.  Forward and gradients without and with that: one sequence of 1000 tokens, 4 heads of 128 channels, 398 and 290 us; of 500, 4 / 2 heads of 64, 164 and
+// 89; 1342 tokens of three sequences, 8 / 4 heads (176 blocks of keys) 217 and 203.  Where it does not pay: 220 blocks of keys (sequences of some 200
+// tokens, 16 / 8 heads) 148 and 170; sequences of some 260 tokens with a head to each key head (two tiles a turn) 119 and 122; 344 blocks of queries beside those
+// 176 of keys 209 and 241.
 template <int DP, bool KEYS> static int run_grad(const Args &p, const Grads &g, long long blocks, int sms, cudaStream_t st) {
     const sapa_attention &a = p.a;
     if (blocks == 0) return SAPA_OK;
     const long long tiles = (KEYS ? (long long)a.tokens * p.share : a.keys) / grad::OVER / (a.B > 0 ? a.B : 1);
     int ranks = 1;
-    while (ranks < 4 && blocks * ranks <= sms && tiles > ranks * grad::TEAMS) ranks *= 2;
+    while (ranks < 4 && blocks * ranks <= (KEYS ? sms + sms / 4 : sms) && tiles > 2 * ranks * grad::TEAMS) ranks *= 2;
     return ranks > 1 ? run_grad_by<DP, KEYS, true>(p, g, blocks, ranks, st) : run_grad_by<DP, KEYS, false>(p, g, blocks, 1, st);
 }
 
