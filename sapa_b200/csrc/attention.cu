@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_
     const int lane = threadIdx.x & 15, c = 8 * lane, D = a.dim;
     begin_after_previous();
     const long long n = (long long)a.tokens * a.heads;
+    const int begin = a.B > 0 ? a.offsets[0] : 0, end = a.B > 0 ? a.offsets[a.B] : 0;
     for (long long base = (long long)blockIdx.x * 16; base < n; base += (long long)gridDim.x * 16) {
         const long long row = base + (threadIdx.x >> 4);
         const unsigned t = n <= 0x7fffffff ? (unsigned)row / (unsigned)a.heads : (unsigned)(row / a.heads), h = (unsigned)(row - (long long)t * a.heads);
@@ -372,7 +373,8 @@ __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_
         if (g.nlse != nullptr) {
             const long long at = ((long long)(h / p.share) * a.tokens + t) * p.share + h % p.share;
             g.delta[at] = sum;
-            g.nlse[at] = -1.4426950408889634f * a.lse[row];
+            // of no sequence: +infinity, as of a row that sees no key, for what such a row of the query holds shows in nothing else
+            g.nlse[at] = (int)t >= begin && (int)t < end ? -1.4426950408889634f * a.lse[row] : INFINITY;
         } else {
             g.delta[row] = sum;
         }

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                         if (!ok) break;
 #pragma unroll
                         for (int r = 0; r < TN / 32; ++r) { row_lse[st][lane + 32 * r] = e[r]; row_delta[st][lane + 32 * r] = -d[r]; }
-                        // what is not finite in a row of dO is in its delta, and in a row of Q in its lse, if it sees a key at all
+                        // what is not finite in a row of dO is in its delta, and in a row of Q in its lse, if it sees a key; nlse of the others is +infinity
                         bool odd = false;
 #pragma unroll
                         for (int r = 0; r < TN / 32; ++r) odd = odd || !isfinite(d[r]) || !(e[r] < INFINITY);

@@ -1,0 +1,49 @@
+"""What lies beside the tokens of a sequence - padding of one tensor alone, heads of the next group, the rest of a tile - has no part in its
+gradients, whatever it holds."""
+import math
+
+import pytest
+import torch
+
+import attention_oracle as oracle
+import sapa_b200
+from attention_oracle import check, offsets_of
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _made(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _step(q, k, v, go, off, koff=None, **kw):
+    q, k, v = (x.detach().clone().requires_grad_() for x in (q, k, v))
+    out = sapa_b200.packed_attention(q, k, v, off, koff, **kw)
+    return (out.detach(), *torch.autograd.grad(out, (q, k, v), go))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("which", ["query", "grad_out", "both"])
+def test_padding_of_one_tensor(which, dim, dtype):
+    """Rows of no sequence in the query alone, in its gradient alone (zeros or numbers in the other) and in both."""
+    lengths, start, t = [150, 37], 5, TYPES[dtype]
+    T = start + sum(lengths) + 30
+    q, go = (_made((T, 4, dim), t, s) for s in (0, 9))
+    k, v = (_made((T, 2, dim), t, s) for s in (1, 2))
+    off = offsets_of(lengths, start)
+    outside = torch.ones(T, dtype=torch.bool, device="cuda")
+    outside[start:start + sum(lengths)] = False
+    want = oracle.packed(q, k, v, lengths, lengths, True, dim ** -0.5, go, start, start)
+    clean = _step(q, k, v, go, off)
+    for name, x in zip(("out", "gq", "gk", "gv"), clean):
+        check(x, want[name], want[name + "_tol"])
+    for rest in (0.0, 1.0):
+        for what in (math.nan, math.inf, -math.inf):
+            qq, gg = q.clone(), go.clone()
+            qq[outside] = what if which != "grad_out" else rest
+            gg[outside] = what if which != "query" else rest
+            for a, b in zip(_step(qq, k, v, gg, off), clean):
+                assert torch.equal(a, b)
