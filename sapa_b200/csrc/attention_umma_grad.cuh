@@ -238,10 +238,12 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                     auto fetch = [&]() {
 #pragma unroll
                         for (int r = 0; r < TN / 32; ++r) {
-                            const int row = lane + 32 * r;
-                            const long long at = at0 + (token + row / at_once) * p.share + part * at_once + row % at_once;
-                            e[r] = row < rows && at < end ? g.nlse[at] : -INFINITY;      // P = 0 where no row is
-                            d[r] = row < rows && at < end ? g.delta[at] : 0.f;
+                            const int row = lane + 32 * r, head = part * at_once + row % at_once;
+                            const long long at = at0 + (token + row / at_once) * p.share + head;
+                            const bool mine = row < rows && at < end && head < p.share;
+                            e[r] = mine ? g.nlse[at] : -INFINITY;                       // P = 0 where no row is
+                            d[r] = mine ? g.delta[at] : 0.f;
+                            if (row < rows && head >= p.share) e[r] = INFINITY;         // heads of the next key head, whatever they hold
                         }
                         if (++part == w->turns) { part = 0; token -= tok; }
                     };

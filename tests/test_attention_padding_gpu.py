@@ -47,3 +47,22 @@ def test_padding_of_one_tensor(which, dim, dtype):
             gg[outside] = what if which != "query" else rest
             for a, b in zip(_step(qq, k, v, gg, off), clean):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim", [40, 64])
+@pytest.mark.parametrize("which", ["query", "grad_out"])
+def test_heads_of_the_next_group(which, dim, dtype):
+    """More query heads to a key head than a tile has rows: the last tile of a token reaches into the heads of the next key head."""
+    T, share, t = 30, 70, TYPES[dtype]
+    q, go = (_made((T, 2 * share, dim), t, s) for s in (0, 9))
+    k, v = (_made((T, 2, dim), t, s) for s in (1, 2))
+    off = offsets_of([18, 12])
+    clean = _step(q, k, v, go, off)
+    for what in (math.nan, math.inf):
+        qq, gg = q.clone(), go.clone()
+        (qq if which == "query" else gg)[7, share + 5, 3] = what
+        out, gq, gk, gv = _step(qq, k, v, gg, off)
+        assert torch.equal(gk[:, 0], clean[2][:, 0]) and torch.equal(gv[:, 0], clean[3][:, 0])
+        assert torch.equal(gk[18:], clean[2][18:]) and torch.equal(gv[18:], clean[3][18:])
+        assert not bool(gv[:8, 1, 3].isfinite().any())
