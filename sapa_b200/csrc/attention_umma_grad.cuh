@@ -373,7 +373,8 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
             }
             for (int i = L::BOTH ? 0 : t; i < n; i += SLOTS) {
                 const unsigned load = loads + i, st = load % NST, stage = base + L::ST0 + st * L::HALF;
-                // columns [lo, hi) of the tile are what the lane sees, or is seen by; part: not all for every lane
+                // columns [lo, hi) of the tile are what the lane sees, or is seen by; part: not all for every lane; masked: of this warpgroup's, or some are of no row
+                // (0, but 0 * infinity is not)
                 int lo = 0, hi;
                 bool part;
                 if (KEYS) {
@@ -387,6 +388,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                     hi = lim - i * TN;
                     part = (i + 1) * TN > least;
                 }
+                const bool masked = part || (KEYS && col0 + N > rows);
                 float x[N], y[N];
                 if (KEYS) {                                           // lse, ahead of the scores
                     if (!mbar_wait_warp(full + 8 * st, (load / NST) & 1)) { ok = false; break; }
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                     x[c] = ex2_ftz(u.x); x[c + 1] = ex2_ftz(u.y);
                 }
                 if (KEYS) {
-                    if (part) {
+                    if (masked) {
 #pragma unroll
                         for (int c = 0; c < N; ++c) x[c] = col0 + c >= lo && col0 + c < hi ? x[c] : 0.f;
                     }
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                     const float2 v = mul2(make_float2(x[c + 2], x[c + 3]), add2(make_float2(y[c + 2], y[c + 3]), make_float2(d.z, d.w)));
                     y[c] = u.x; y[c + 1] = u.y; y[c + 2] = v.x; y[c + 3] = v.y;
                 }
-                if (part) {
+                if (masked) {
 #pragma unroll
                     for (int c = 0; c < N; ++c) y[c] = col0 + c >= lo && col0 + c < hi ? y[c] : 0.f;
                 }

@@ -66,3 +66,24 @@ def test_heads_of_the_next_group(which, dim, dtype):
         assert torch.equal(gk[:, 0], clean[2][:, 0]) and torch.equal(gv[:, 0], clean[3][:, 0])
         assert torch.equal(gk[18:], clean[2][18:]) and torch.equal(gv[18:], clean[3][18:])
         assert not bool(gv[:8, 1, 3].isfinite().any())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads, groups", [(3, 1), (12, 2), (5, 1), (7, 1), (70, 1)])
+def test_key_without_weight(heads, groups, dim, dtype):
+    """A key whose scores are all -infinity has gradients of zero, also where the query heads that share it do not divide a tile."""
+    T, t = 200, TYPES[dtype]
+    q = _made((T, heads, dim), t, 0).abs()
+    k, v = (_made((T, groups, dim), t, s).abs() for s in (1, 2))
+    go = _made((T, heads, dim), t, 9)
+    keep = [j for j in range(T) if j != 50]
+    want = oracle.packed(q, k[keep], v[keep], [T], [T - 1], False, dim ** -0.5, go)
+    k[50, :, 5] = -math.inf
+    out, gq, gk, gv = _step(q, k, v, go, offsets_of([T]), causal=False)
+    check(out, want["out"], want["out_tol"])
+    for name, x in (("gk", gk), ("gv", gv)):
+        assert bool((x[50] == 0).all())
+        check(x[keep], want[name], want[name + "_tol"])
+    rest = [c for c in range(dim) if c != 5]             # there 0 * infinity
+    check(gq[..., rest], want["gq"][..., rest], want["gq_tol"][..., rest])
