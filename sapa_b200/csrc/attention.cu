@@ -779,6 +779,7 @@ static Shape shape_of(const Args &p, int dtype, int sms) {
     s.blocks = most_blocks(a, a.tokens, s.tok) * a.groups;
     s.rows = (a.tokens < s.tok ? a.tokens : s.tok) * p.share;
     s.grid = s.blocks;
+    if (a.B == 0) return s;                          // no sequence: nothing to split
     // few blocks: their keys are split so that every SM has items
     const long long keys = a.page_table != nullptr ? (long long)a.max_pages * a.page : a.keys;
     if (s.blocks < 2ll * sms && keys > (s.umma ? 8 : 2) * TILE) {
@@ -844,7 +845,7 @@ using namespace sapa::attn;
 
 extern "C" size_t sapa_attention_workspace(const sapa_attention *a, int dtype) {
     int sms = 0;
-    if (check(a, dtype, "sapa_attention_workspace") != SAPA_OK || a->tokens == 0 || a->B == 0 || sm_count("sapa_attention_workspace", sms) != SAPA_OK) return 0;
+    if (check(a, dtype, "sapa_attention_workspace") != SAPA_OK || a->tokens == 0 || sm_count("sapa_attention_workspace", sms) != SAPA_OK) return 0;
     return shape_of(args_of(a), dtype, sms).bytes;
 }
 

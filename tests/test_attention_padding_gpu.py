@@ -87,3 +87,15 @@ def test_key_without_weight(heads, groups, dim, dtype):
         check(x[keep], want[name], want[name + "_tol"])
     rest = [c for c in range(dim) if c != 5]             # there 0 * infinity
     check(gq[..., rest], want["gq"][..., rest], want["gq_tol"][..., rest])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T", [90, 3000])
+def test_no_sequence(T, dtype):
+    """Offsets of one entry: every row is of no sequence, however many there are."""
+    q, go = (_made((T, 8, 64), TYPES[dtype], s) for s in (0, 9))
+    k, v = (_made((T, 2, 64), TYPES[dtype], s) for s in (1, 2))
+    with torch.no_grad():
+        assert bool((sapa_b200.packed_attention(q, k, v, offsets_of([])) == 0).all())
+    for x in _step(q, k, v, go, offsets_of([])):
+        assert bool((x == 0).all())
