@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(rows::NT) sapa_attention_rows_kernel(const __g
     const int least = sees(s, first, a.causal), most = sees(s, first + used / p.share - 1, a.causal);      // of the block's tokens
     const int room = min(most, s.bad);                                                   // positions that are there to be read
     const long long from = (long long)it.part * plan.tiles * TILE, upto = min((long long)room, from + (long long)plan.tiles * TILE);
-    if (tid == 0 && s.bad < most) bad_page = s.bad;
+    if (tid == 0 && s.bad < most) atomicMin(&bad_page, s.bad);       // other threads may have found an earlier one
 
     for (int e = tid; e < L::BM * (DP / 4); e += NT) {
         const int r = e / (DP / 4), c = e % (DP / 4) * 4;
