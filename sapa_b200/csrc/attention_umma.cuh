@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                     if (!mbar_wait_warp(full + 8 * stage, (load / NST) & 1)) { ok = false; break; }
                     if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r) && k0 + r < seen) { atomicMin(&w->odd_first, k0 + r); atomicMax(&w->odd_last, k0 + r); }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();                                     // lanes that found something went another way: tensor memory is read by whole warps
                 }
                 if (busy) {
                     float x[KT];
@@ -597,6 +598,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
 #pragma unroll 1
                 for (int c = WIDE ? 0 : t * WIDTH; c < (WIDE ? D : (t + 1) * WIDTH) && c < a.dim; c += 32) {
                     float o[32];
+                    __syncwarp();                                     // behind the stores of the channels before, which not every lane makes
                     if (all > 0) tc_ld32(WIDE ? o_at + c : tmem + quarter + L::O_COL + c, o);
                     tc_wait_ld();
                     if (!WIDE) {

@@ -426,6 +426,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                         if (clean_box<T, D, TN>(stage, r) && i * TN + r < s.nk) { atomicMin(&w->odd_first, i * TN + r); atomicMax(&w->odd_last, i * TN + r); }
                     }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();                                     // lanes that found something went another way: tensor memory is used by whole warps
                 }
                 if (KEYS) {
                     tc_wait_st();
@@ -474,6 +475,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                 T *const to = KEYS ? static_cast<T *>(values ? g.gv : g.gk) + ((long long)(s.k0 + key) * a.groups + w->group) * a.dim
                                    : static_cast<T *>(g.gq) + ((long long)(s.q0 + token) * a.heads + w->group * p.share + r % p.share) * a.dim;
                 float o[32];
+                __syncwarp();                                         // behind the stores of the unit before, which not every lane makes
                 if (n > 0) {
                     tc_ld32(at + c, o);
                     tc_wait_ld();
