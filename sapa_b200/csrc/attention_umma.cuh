@@ -205,14 +205,14 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
     using L = um::Lay<D, WIDE>;
     constexpr int NST = L::NST;
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) unsigned long long bars[2 + 2 * NST + 6 + 4 + 4];
+    __shared__ __align__(8) unsigned long long bars[2 + 2 * NST + 6 + 4 + 4 + 2];
     __shared__ unsigned tmem_slot;
     __shared__ Work queue[2];
     __shared__ float handed[WIDE ? 1 : 2][ROWS];                      // maximum, then sum, of the even and the odd tiles
     const sapa_attention &a = p.a;
     const unsigned base = ((unsigned)__cvta_generic_to_shared(smem_dyn) + 1023u) & ~1023u;
     const unsigned qfull = (unsigned)__cvta_generic_to_shared(bars), qempty = qfull + 8, full = qempty + 8, empty = full + 8 * NST, sfull = empty + 8 * NST, pfull = sfull + 16;
-    const unsigned posted = pfull + 32, taken = posted + 16, pair = taken + 16;
+    const unsigned posted = pfull + 32, taken = posted + 16, pair = taken + 16, done = pair + 32;
     const int tid = threadIdx.x, warp = (int)warp_uniform(tid >> 5), lane = tid & 31;
     const int tile_tok = ROWS / p.share, tok = WIDE ? 2 * tile_tok : tile_tok;
 
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
         if (lane == 0) {
             mbar_init(qfull, 1); mbar_init(qempty, 1);
             for (int i = 0; i < NST; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
-            for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 16 * i, 128); mbar_init(pfull + 16 * i + 8, 128); mbar_init(posted + 8 * i, 1); mbar_init(taken + 8 * i, 11); }
+            for (int i = 0; i < 2; ++i) { mbar_init(sfull + 8 * i, 1); mbar_init(done + 8 * i, 1); mbar_init(pfull + 16 * i, 128); mbar_init(pfull + 16 * i + 8, 128); mbar_init(posted + 8 * i, 1); mbar_init(taken + 8 * i, 11); }
             for (int i = 0; i < 4; ++i) mbar_init(pair + 8 * i, 256);
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
@@ -385,6 +385,8 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 }
                 if (t == 0) pph0 ^= 1; else pph1 ^= 1;
             };
+            // An item's last outputs have a barrier of their own: the next item's first scores come right behind them, and a warp that has not yet seen one phase
+            // of a barrier end when the next one does waits for ever.  Everything else is behind weights (pfull) that come from who has seen it.
             while (Work *w = next_work()) {
                 const int all = (int)warp_uniform(w->all), n0 = (int)warp_uniform(w->n0), n1 = (int)warp_uniform(w->n1);
                 if (all > 0) {
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                                 if (!ok) break;
                                 scores(t, k);
                             }
-                            tc_commit_by(leader, sfull + 8 * t);
+                            tc_commit_by(leader, (j + 1 < nt ? sfull : done) + 8 * t);
                         }
                         if (!ok) break;
                         tc_commit_by(leader, empty + 8 * v);
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                             tc_commit_by(leader, empty + 8 * k);
                             if (i + 3 == all) tc_commit_by(leader, qempty);
                         }
-                        tc_commit_by(leader, sfull + 8 * t);
+                        tc_commit_by(leader, (i + 2 < all ? sfull : done) + 8 * t);
                     }
                 }
                 if (!ok) break;
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
         const bool in_tile = r < tile_tok * p.share;
         const bool turned = p.scale_log2 <= 0.f;                      // the largest score is not the largest product
         const float scale = turned ? 1.f : p.scale_log2;
-        int sph = 0;
+        int sph = 0, done_ph = 0;
         unsigned loads = 0;                                           // stages that the items before took
         while (Work *w = next_work()) {
             const Sequence s = w->s;
@@ -560,8 +562,8 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
             }
             loads += 2 * all;
             if (ok && steps > 0) {                                    // the outputs are complete
-                ok = mbar_wait_warp(sfull + 8 * t, sph);
-                sph ^= 1;
+                ok = mbar_wait_warp(done + 8 * t, done_ph);
+                done_ph ^= 1;
             }
             tc_fence_after();
             if (!(m < INFINITY)) sum = __int_as_float(0x7fffffff);    // infinity less infinity, or a NaN
