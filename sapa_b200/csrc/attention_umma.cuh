@@ -132,14 +132,16 @@ __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-// Replaces what is not finite in 128 bytes of a row of a landed tile with 0; whether there was any.  All are read before they are looked at.
-template <typename T> __device__ __forceinline__ bool clean_line(unsigned line, int row) {
+// Replaces what is not finite in 128 bytes of a row of a landed tile with 0; whether there was any.  All are read before they are looked at.  Two row tiles clean the
+// same values, and the one that finds zeros must find the note of them too: `note` comes in front of the stores.
+template <typename T, typename Note> __device__ __forceinline__ bool clean_line(unsigned line, int row, Note note) {
     unsigned v[32];
 #pragma unroll
     for (int c = 0; c < 8; ++c)                                       // in another order in every row: no two on the same banks
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[4 * c]), "=r"(v[4 * c + 1]), "=r"(v[4 * c + 2]), "=r"(v[4 * c + 3])
                      : "r"(line + ((c ^ (row & 7)) << 4)) : "memory");
     if (finite::all_finite<T, 32>(v)) return false;
+    note();
 #pragma unroll
     for (int c = 0; c < 8; ++c)
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(line + ((c ^ (row & 7)) << 4)), "r"(finite::or_zero<T>(v[4 * c])),
@@ -147,11 +149,9 @@ template <typename T> __device__ __forceinline__ bool clean_line(unsigned line, 
     return true;
 }
 // The same for a row of a tile of 128 rows
-template <typename T, int D> __device__ __forceinline__ bool clean_row(unsigned tile, int row) {
-    bool any = false;
+template <typename T, int D, typename Note> __device__ __forceinline__ void clean_row(unsigned tile, int row, Note note) {
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) any = clean_line<T>(tile + b * BLOCK_BYTES + row * 128, row) || any;
-    return any;
+    for (int b = 0; b < D / 64; ++b) (void)clean_line<T>(tile + b * BLOCK_BYTES + row * 128, row, note);
 }
 // 32 channels of a row each of a warp's lanes, from float32, those below `left`; `mine`: whether the lane has one.  A row in every lane is a line in every
 // lane, and a store takes a cycle for each: so two lanes write halves of one row and then of the other, 32 bytes each (`whole`: rows begin on 32
@@ -485,7 +485,10 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 if (part) {
                     const unsigned load = loads + L::stage_of(j - j0, all, false), stage = load % NST;
                     if (!mbar_wait_warp(full + 8 * stage, (load / NST) & 1)) { ok = false; break; }
-                    if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r) && k0 + r < seen) { atomicMin(&w->odd_first, k0 + r); atomicMax(&w->odd_last, k0 + r); }
+                    clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r, [&]() {
+                        if (k0 + r < seen) { atomicMin(&w->odd_first, k0 + r); atomicMax(&w->odd_last, k0 + r); }
+                        __threadfence_block();
+                    });
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     __syncwarp();                                     // lanes that found something went another way: tensor memory is read by whole warps
                 }

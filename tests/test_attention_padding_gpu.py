@@ -99,3 +99,23 @@ def test_no_sequence(T, dtype):
         assert bool((sapa_b200.packed_attention(q, k, v, offsets_of([])) == 0).all())
     for x in _step(q, k, v, go, offsets_of([])):
         assert bool((x == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_values_at_the_diagonal_of_two_row_tiles(dim, dtype):
+    """Tiles that both row tiles of a block clean: the tokens from an infinite value on have it, the others not a bit of it, each time."""
+    T, t = 700, TYPES[dtype]
+    q = _made((T, 4, dim), t, 0)
+    k, v = (_made((T, 2, dim), t, s) for s in (1, 2))
+    off = offsets_of([T])
+    with torch.no_grad():
+        clean = sapa_b200.packed_attention(q, k, v, off)
+        at = [63, 64, 127, 130, 255, 300, 500, 639, 699]
+        for i, j in enumerate(at):
+            v[j, 1, i] = math.inf if i % 2 == 0 else -math.inf
+        for _ in range(50):
+            out = sapa_b200.packed_attention(q, k, v, off)
+            assert torch.equal(out[:, :2], clean[:, :2]) and torch.equal(out[:, 2:, len(at):], clean[:, 2:, len(at):])
+            for i, j in enumerate(at):
+                assert torch.equal(out[:j, 2:, i], clean[:j, 2:, i]) and bool((out[j:, 2:, i] == v[j, 1, i]).all())
