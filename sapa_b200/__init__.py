@@ -9,7 +9,8 @@ working unchanged, put :func:`compat_path` on ``sys.path``.
 """
 import os as _os
 
-from .attention import PackedAttentionFunction, packed_attention, paged_attention, paged_write
+from .attention import (PackedAttentionFunction, PagedAttentionFunction, PagedWriteFunction, packed_attention, paged_attention,
+                        paged_write)
 from .deform_functions import (DeformAVFunction, DeformQKFunction, DeformSapaFusedFunction, deform_av, deform_qk,
                                deform_sapa_fused)
 from .functions import AVFunction, QKFunction, SapaFusedFunction, av, qk, sapa_fused, sapa_fused_nhwc
@@ -20,7 +21,7 @@ from .projection import project
 __all__ = ["qk", "av", "sapa_fused", "sapa_fused_nhwc", "deform_qk", "deform_av", "deform_sapa_fused", "SAPA", "SAPADeform",
            "QKFunction", "AVFunction", "SapaFusedFunction", "DeformQKFunction", "DeformAVFunction",
            "DeformSapaFusedFunction", "GraphedForward", "project", "packed_attention", "paged_attention", "paged_write",
-           "PackedAttentionFunction", "compat_path"]
+           "PackedAttentionFunction", "PagedAttentionFunction", "PagedWriteFunction", "compat_path"]
 
 
 def compat_path() -> str:

@@ -7,7 +7,7 @@ the autograd node are native (``csrc/host_attention.inc``), the kernels are in `
 """
 from __future__ import annotations
 
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import _lib
 
@@ -54,11 +54,50 @@ def paged_attention(query, key_pages, value_pages, page_table, key_lengths, offs
 
     Entries of the table behind a sequence's last page are not read.  A token that sees a position whose page number lies outside the
     cache, or that the table has no entry for, gets NaN; the page is not read."""
+    if _lib.transformed():
+        return PagedAttentionFunction.apply(query, key_pages, value_pages, page_table, key_lengths, offsets, causal, scale)
     return (_lib.host or _lib.load_host()).paged_attention(query, key_pages, value_pages, page_table, key_lengths, offsets, causal, scale)
+
+
+class PagedAttentionFunction(Function):
+    """``paged_attention`` for traces; under transforms it raises."""
+
+    @staticmethod
+    def forward(ctx, query, key_pages, value_pages, page_table, key_lengths, offsets, causal, scale):
+        _forward_only("paged_attention", ctx)
+        return _lib.load_host().paged_attention(query, key_pages, value_pages, page_table, key_lengths, offsets, causal, scale)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        raise NotImplementedError("paged_attention is forward only")
 
 
 def paged_write(key, value, key_pages, value_pages, page_table, key_lengths, offsets):
     """Put new keys and values, [T, groups, dim] packed by ``offsets``, into the cache in place: token i of the Lq new ones of sequence b goes to
     position ``key_lengths[b] - Lq + i``, so ``key_lengths`` already counts them.  Positions below 0 or without a page inside the cache
     are skipped; nothing else of the cache is touched.  No two tokens of a call may go to the same slot."""
+    if _lib.transformed():
+        if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (key, value, key_pages, value_pages)):
+            raise NotImplementedError("paged_write is not differentiable")      # here: the Function would first write
+        PagedWriteFunction.apply(key, value, key_pages, value_pages, page_table, key_lengths, offsets)
+        return
     (_lib.host or _lib.load_host()).paged_write(key, value, key_pages, value_pages, page_table, key_lengths, offsets)
+
+
+class PagedWriteFunction(Function):
+    """``paged_write`` for traces, as a step without a result that is used; under transforms it raises."""
+
+    @staticmethod
+    def forward(ctx, key, value, key_pages, value_pages, page_table, key_lengths, offsets):
+        _forward_only("paged_write", ctx)
+        _lib.load_host().paged_write(key, value, key_pages, value_pages, page_table, key_lengths, offsets)
+        return key.new_empty(0)                          # a trace keeps no step without one
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        raise NotImplementedError("paged_write is not differentiable")
+
+
+def _forward_only(name, ctx):
+    if any(ctx.needs_input_grad):
+        raise NotImplementedError(f"{name} has no gradients")
