@@ -345,34 +345,55 @@ __global__ void __launch_bounds__(256) sapa_attention_join_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------------------------- backward
-// delta, and what lies outside the sequences: 16 lanes per token and head, 8 channels each.  Reads grad_out, out and what its rounding left out once, which
-// bounds it (8262 tokens x 16 heads x 128 channels, bfloat16: 28 us, 3.6 TB/s; with two rows to a thread 29, with four 44).
-template <typename T>
-__global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
+// delta, and what lies outside the sequences: 8 or 16 lanes (up to 64 or 128 channels) per token and head, 8 channels each.  Reads grad_out, out and what its
+// rounding left out once, which bounds it (8262 tokens x 16 heads x 128 channels, bfloat16: 28 us, 3.6 TB/s; with two rows to a thread 29, with four 44).  In
+// float16 also sums of squares, for which blocks behind those of the queries read the values.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256, 8) sapa_attention_delta_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     const sapa_attention &a = p.a;
+    constexpr bool SQUARES = std::is_same<T, __half>::value;
     constexpr bool RESTS = !std::is_same<T, float>::value;            // `out` before its rounding: by itself that would make the gradients a third less exact
-    const int lane = threadIdx.x & 15, c = 8 * lane, D = a.dim;
+    constexpr int ROWS = 256 / LANES;                                 // of a block
+    const int lane = threadIdx.x % LANES, c = 8 * lane, D = a.dim;
+    auto squares = [](const float4 (&x)[2]) {
+        return fmaf(x[1].w, x[1].w, fmaf(x[1].z, x[1].z, fmaf(x[1].y, x[1].y, fmaf(x[1].x, x[1].x, fmaf(x[0].w, x[0].w, fmaf(x[0].z, x[0].z, fmaf(x[0].y, x[0].y, x[0].x * x[0].x)))))));
+    };
     begin_after_previous();
-    const long long n = (long long)a.tokens * a.heads;
+    const long long n = (long long)a.tokens * a.heads, query_blocks = (n + ROWS - 1) / ROWS, m = SQUARES ? (long long)a.keys * a.groups : 0;
     const int begin = a.B > 0 ? a.offsets[0] : 0, end = a.B > 0 ? a.offsets[a.B] : 0;
-    for (long long base = (long long)blockIdx.x * 16; base < n; base += (long long)gridDim.x * 16) {
-        const long long row = base + (threadIdx.x >> 4);
+    for (long long block = blockIdx.x; block < query_blocks + (m + ROWS - 1) / ROWS; block += gridDim.x) {
+        if (SQUARES && block >= query_blocks) {
+            const long long row = (block - query_blocks) * ROWS + threadIdx.x / LANES;
+            const unsigned t = m <= 0x7fffffff ? (unsigned)row / (unsigned)a.groups : (unsigned)(row / a.groups), group = (unsigned)(row - (long long)t * a.groups);
+            float4 v[2];
+            rows::load8(static_cast<const T *>(a.value) + t * a.value_strides[0] + group * a.value_strides[1] + c, row < m && c < D, v);
+            float square = squares(v);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
+            if (lane == 0 && row < m) g.value_squares[(long long)group * a.keys + t] = square;
+            continue;
+        }
+        const long long row = block * ROWS + threadIdx.x / LANES;
         const unsigned t = n <= 0x7fffffff ? (unsigned)row / (unsigned)a.heads : (unsigned)(row / a.heads), h = (unsigned)(row - (long long)t * a.heads);
         const bool there = row < n && c < D;
         float4 u[2], v[2], low[2];
         rows::load8(static_cast<const T *>(a.out) + row * D + c, there, u);
         rows::load8(static_cast<const T *>(g.go) + t * g.go_strides[0] + h * g.go_strides[1] + c, there, v);
         rows::load8(static_cast<const T *>(a.low) + row * D + c, there && RESTS, low);
-        float sum = 0.f;
+        float sum = 0.f, square = SQUARES ? squares(v) : 0.f;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             sum = fmaf(u[e].w + low[e].w, v[e].w, fmaf(u[e].z + low[e].z, v[e].z, fmaf(u[e].y + low[e].y, v[e].y, fmaf(u[e].x + low[e].x, v[e].x, sum))));
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (SQUARES) square += __shfl_xor_sync(0xffffffffu, square, o);
+        }
         if (lane != 0 || row >= n) continue;
         if (g.nlse != nullptr) {
             const long long at = ((long long)(h / p.share) * a.tokens + t) * p.share + h % p.share;
             g.delta[at] = sum;
+            if (SQUARES) g.squares[at] = square;
             // of no sequence: +infinity, as of a row that sees no key, for what such a row of the query holds shows in nothing else
             g.nlse[at] = (int)t >= begin && (int)t < end ? -1.4426950408889634f * a.lse[row] : INFINITY;
         } else {
@@ -382,6 +403,43 @@ __global__ void __launch_bounds__(256) sapa_attention_delta_kernel(const __grid_
     clear_outside(static_cast<T *>(g.gq), a.offsets, a.B, a.tokens, a.heads * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
     clear_outside(static_cast<T *>(g.gk), a.key_offsets, a.B, a.keys, a.groups * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
     clear_outside(static_cast<T *>(g.gv), a.key_offsets, a.B, a.keys, a.groups * D, blockIdx.x, gridDim.x, threadIdx.x, 256);
+}
+
+// float16.  The power of two that dS of a sequence and key head (a block's) is multiplied with to be held in 16 bits: |dS| = |P_j sum_k P_k (dP_j - dP_k)| is at most
+// a quarter of the range of dP, that is half the product of the longest rows of grad_out and of value, and comes to 2^14 at most.  The scores' weights, around
+// 1 / keys, leave it among the normal numbers then, whatever size the gradients have.  Rows that are not finite do not count.
+__global__ void __launch_bounds__(1024) sapa_attention_factor_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
+    const sapa_attention &a = p.a;
+    __shared__ float most[2][32];
+    const int b = blockIdx.x / a.groups, group = blockIdx.x % a.groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    begin_after_previous();
+    const Sequence s = sequence_at(a, b);
+    auto largest = [&](const float *x, long long n) {
+        float top[4] = {0.f, 0.f, 0.f, 0.f};
+        for (long long i = threadIdx.x; i < n; i += 4 * 1024)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = i + 1024 * e < n ? x[i + 1024 * e] : 0.f;
+                top[e] = isfinite(v) ? fmaxf(top[e], v) : top[e];
+            }
+        float r = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
+        return r;
+    };
+    const float x = largest(g.squares + ((long long)group * a.tokens + s.q0) * p.share, (long long)s.nq * p.share);
+    const float y = largest(g.value_squares + (long long)group * a.keys + s.k0, s.nk);
+    if (lane == 0) { most[0][warp] = x; most[1][warp] = y; }
+    __syncthreads();
+    if (warp != 0) return;
+    float u = most[0][lane], v = most[1][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    }
+    const int j = (int)(__float_as_uint(u) >> 23), k = (int)(__float_as_uint(v) >> 23);      // sums below 2^(j - 126), 2^(k - 126); none is subnormal, as squares of float16
+    if (lane == 0) g.factor[blockIdx.x] = j == 0 || k == 0 ? 1.f : __int_as_float((127 + 15 - ((j + k - 252 + 1) >> 1)) << 23);
 }
 
 namespace grad {
@@ -881,10 +939,15 @@ extern "C" int sapa_attention_forward(const sapa_attention *a, void *workspace, 
     });
 }
 
+// floats in a workspace: delta, in 16 bits lse in another order, in float16 the squares and factors too
+static size_t floats(size_t n) { return (n * sizeof(float) + 255) / 256 * 256; }
+static size_t row_floats(const sapa_attention *a) { return floats((size_t)a->tokens * a->heads); }
+static size_t value_floats(const sapa_attention *a) { return floats((size_t)a->keys * a->groups); }
+
 extern "C" size_t sapa_attention_backward_workspace(const sapa_attention *a, int dtype) {
     if (check(a, dtype, "sapa_attention_backward_workspace") != SAPA_OK) return 0;
-    // delta, and in 16 bits lse in another order
-    return ((size_t)a->tokens * a->heads * sizeof(float) + 255) / 256 * 256 * (dtype == SAPA_F32 ? 1 : 2);
+    if (dtype == SAPA_F16) return 3 * row_floats(a) + value_floats(a) + floats((size_t)a->B * a->groups);
+    return row_floats(a) * (dtype == SAPA_F32 ? 1 : 2);
 }
 
 extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad_out, long long grad_token_stride, long long grad_head_stride,
@@ -913,17 +976,30 @@ extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad
         return check_launch("memset");
     }
     const bool umma = dtype != SAPA_F32;
-    Grads g{grad_out, {grad_token_stride, grad_head_stride}, grad_query, grad_key, grad_value, static_cast<float *>(workspace),
-            umma ? reinterpret_cast<float *>(static_cast<char *>(workspace) + need / 2) : nullptr};
+    char *const ws = static_cast<char *>(workspace);
+    Grads g{grad_out, {grad_token_stride, grad_head_stride}, grad_query, grad_key, grad_value, reinterpret_cast<float *>(ws), nullptr, nullptr, nullptr, nullptr};
+    if (umma) g.nlse = reinterpret_cast<float *>(ws + row_floats(a));
+    if (dtype == SAPA_F16) {
+        g.squares = reinterpret_cast<float *>(ws + 2 * row_floats(a));
+        g.value_squares = reinterpret_cast<float *>(ws + 3 * row_floats(a));
+        g.factor = reinterpret_cast<float *>(ws + 3 * row_floats(a) + value_floats(a));
+    }
     int sms = 0;
     if (int e = sm_count(fn, sms)) return e;
-    const long long rows16 = ((long long)a->tokens * a->heads + 15) / 16, delta_grid = rows16 < (1ll << 20) ? rows16 : 1ll << 20;
+    const int delta_rows = a->dim <= 64 ? 32 : 16;                    // of a block
+    const long long delta_blocks = ((long long)a->tokens * a->heads + delta_rows - 1) / delta_rows + (dtype == SAPA_F16 ? ((long long)a->keys * a->groups + delta_rows - 1) / delta_rows : 0);
+    const dim3 delta_grid((unsigned)(delta_blocks < (1ll << 20) ? delta_blocks : 1ll << 20));
     const int at_once = p.share < grad::OWN ? p.share : grad::OWN, slots = (p.share + at_once - 1) / at_once, tok = grad::OWN / at_once;
     const long long key_blocks = most_blocks(*a, a->keys, grad::OWN) * a->groups, query_blocks = most_blocks(*a, a->tokens, tok) * a->groups * slots;
-    SAPA_REQUIRE(key_blocks < 0x7fffffffll && query_blocks < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
+    SAPA_REQUIRE(key_blocks < 0x7fffffffll && query_blocks < 0x7fffffffll && (long long)a->B * a->groups < 0x7fffffffll, SAPA_ERR_UNSUPPORTED, "%s: too many blocks", fn);
     return SAPA_DISPATCH_FAST(dtype, [&]() -> int {
-        launch_next(sapa_attention_delta_kernel<scalar_t>, dim3((unsigned)delta_grid), dim3(256), 0, st, p, g);
+        if (a->dim <= 64) launch_next(sapa_attention_delta_kernel<scalar_t, 8>, delta_grid, dim3(256), 0, st, p, g);
+        else launch_next(sapa_attention_delta_kernel<scalar_t, 16>, delta_grid, dim3(256), 0, st, p, g);
         if (int e = check_launch("sapa_attention_delta_kernel")) return e;
+        if (dtype == SAPA_F16 && a->B > 0) {
+            launch_next(sapa_attention_factor_kernel, dim3((unsigned)(a->B * a->groups)), dim3(1024), 0, st, p, g);
+            if (int e = check_launch("sapa_attention_factor_kernel")) return e;
+        }
         if (umma) return umma_backward(p, g, dtype, st);
         if (a->dim <= 64) {
             if (int e = run_grad<64, true>(p, g, key_blocks, sms, st)) return e;

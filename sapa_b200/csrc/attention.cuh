@@ -232,6 +232,9 @@ struct Grads {
     void *gq, *gk, *gv;
     float *delta;                  // sum over channels of grad_out * out: [tokens, heads], or like nlse where that is there
     float *nlse;                   // -log2(e) lse as the tensor-core kernels read it: [groups, tokens, heads of a group]; or NULL
+    // float16, otherwise NULL: sums of squares of the rows of grad_out (like nlse) and of value ([groups, keys]), and from them the factor of dS of each
+    // sequence and key head ([B, groups])
+    float *squares, *value_squares, *factor;
 };
 
 // Tensor-core forward (attention_umma.cu): what it takes, and its launch; wide: two row tiles a block.

@@ -2,7 +2,7 @@
 // attention_umma.cu behind attention_umma.cuh.
 //
 // P and dS of a tile are formed again: P = 2^(scale s - lse), dS = P (dP - delta), rounded to the inputs' type for the products that take them from
-// tensor memory; the sums are float32.  Two launches of one kernel, without atomics, so that results do not depend on the order of anything:
+// tensor memory (dS in float16 by a power of two, see sapa_attention_factor_kernel); the sums are float32.  Two launches of one kernel, without atomics, so that results do not depend on the order of anything:
 //   * KEYS: an item holds 128 keys and values and goes over the rows (token x query head) that see them.  S^T = K Q^T and dP^T = V dO^T have the keys in
 //     the lanes of tensor memory, so that P^T and dS^T are first operands of dV += P^T dO and dK += dS^T Q as they are;
 //   * otherwise an item holds 128 rows and goes over the keys that they see: S = Q K^T, dP = dO V^T, dQ += dS K.
@@ -51,6 +51,7 @@ struct Work {
     int from, turns;               // KEYS: the first token that sees a key; tiles that the heads of a token take
     Sequence s;
     int odd_first, odd_last;       // rows or keys with something not finite, of tiles that are not seen whole
+    float factor, rescale;         // of dS; of the gradients of queries and keys
 };
 
 // S[128 x TN] = A B^T, both K-major in shared memory, or A in tensor memory
@@ -93,6 +94,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
     using L = umg::Lay<D, KEYS>;
     using Work = umg::Work;
     constexpr int NST = L::NST, TN = L::TN, SLOTS = L::SLOTS;
+    constexpr bool SCALED = std::is_same<T, __half>::value;           // dS by a power of two: float16 holds neither the small nor the large ones
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(16) float row_lse[KEYS ? NST : 1][TN], row_delta[KEYS ? NST : 1][TN];      // as nlse, -delta
     __shared__ __align__(8) unsigned long long bars[2 + 4 * NST + 8 + 4 + 3];
@@ -161,6 +163,8 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                         w.b = it.b; w.group = index % a.groups;
                         w.s = sequence_at(a, it.b);
                         w.fine = max(w.s.nq, w.s.nk) <= FINE;
+                        w.factor = SCALED ? g.factor[(long long)w.b * a.groups + w.group] : 1.f;
+                        w.rescale = a.scale / w.factor;               // a power of two
                         if (KEYS) {
                             w.first = it.block * KT;
                             w.from = a.causal ? (int)max(0ll, (long long)w.first - w.s.nk + w.s.nq) : 0;
@@ -232,6 +236,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                 while (Work *w = next_work()) {
                     const int n = w->n;
                     const long long at0 = ((long long)w->group * a.tokens + w->s.q0 + w->from) * p.share, end = (long long)a.tokens * a.heads;
+                    const float factor = SCALED ? w->factor : 1.f;
                     float e[TN / 32], d[TN / 32];
                     int part = 0;
                     long long token = (long long)(n / max(w->turns, 1) - 1) * tok;
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                         ok = mbar_wait_warp(empty + 8 * st, ph ^ 1);
                         if (!ok) break;
 #pragma unroll
-                        for (int r = 0; r < TN / 32; ++r) { row_lse[st][lane + 32 * r] = e[r]; row_delta[st][lane + 32 * r] = -d[r]; }
+                        for (int r = 0; r < TN / 32; ++r) { row_lse[st][lane + 32 * r] = e[r]; row_delta[st][lane + 32 * r] = SCALED ? -d[r] * factor : -d[r]; }
                         // what is not finite in a row of dO is in its delta, and in a row of Q in its lse, if it sees a key; nlse of the others is +infinity
                         bool odd = false;
 #pragma unroll
@@ -351,6 +356,9 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                 const long long row = ((long long)w->group * a.tokens + s.q0 + first) * p.share + r;
                 nlse = g.nlse[row]; delta = g.delta[row];
             }
+            const float2 factor = SCALED ? make_float2(w->factor, w->factor) : make_float2(1.f, 1.f);
+            if (SCALED) delta *= factor.x;
+            auto less = [&](float2 dp, float2 minus_delta) { return SCALED ? fma2(dp, factor, minus_delta) : add2(dp, minus_delta); };
             if (L::IN_TMEM && n > 0) {                                // the item's own operands, half of one by each warpgroup; what was there has been used: `done`
                 if (!mbar_wait_warp(ownfull, own_ph)) { ok = false; break; }
                 own_ph ^= 1;
@@ -441,8 +449,8 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
 #pragma unroll
                 for (int c = 0; c < N; c += 4) {
                     const float4 d = KEYS ? *reinterpret_cast<const float4 *>(&row_delta[KEYS ? st : 0][col0 + c]) : make_float4(-delta, -delta, -delta, -delta);
-                    const float2 u = mul2(make_float2(x[c], x[c + 1]), add2(make_float2(y[c], y[c + 1]), make_float2(d.x, d.y)));
-                    const float2 v = mul2(make_float2(x[c + 2], x[c + 3]), add2(make_float2(y[c + 2], y[c + 3]), make_float2(d.z, d.w)));
+                    const float2 u = mul2(make_float2(x[c], x[c + 1]), less(make_float2(y[c], y[c + 1]), make_float2(d.x, d.y)));
+                    const float2 v = mul2(make_float2(x[c + 2], x[c + 3]), less(make_float2(y[c + 2], y[c + 3]), make_float2(d.z, d.w)));
                     y[c] = u.x; y[c + 1] = u.y; y[c + 2] = v.x; y[c + 3] = v.y;
                 }
                 if (masked) {
@@ -471,7 +479,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                 const int c = unit % (D / 32) * 32;
                 if (c >= a.dim) continue;
                 const unsigned at = tmem + quarter + L::ACC_COL + unit * 32 - c;
-                const float factor = values ? 1.f : a.scale;
+                const float by = values ? 1.f : w->rescale;
                 T *const to = KEYS ? static_cast<T *>(values ? g.gv : g.gk) + ((long long)(s.k0 + key) * a.groups + w->group) * a.dim
                                    : static_cast<T *>(g.gq) + ((long long)(s.q0 + token) * a.heads + w->group * p.share + r % p.share) * a.dim;
                 float o[32];
@@ -481,7 +489,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                     tc_wait_ld();
                 }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = n > 0 && (KEYS || lim > 0) ? o[e] * factor : 0.f;
+                for (int e = 0; e < 32; ++e) o[e] = n > 0 && (KEYS || lim > 0) ? o[e] * by : 0.f;
                 if (odd1 >= 0 && mine && (values || !KEYS)) {         // rare: what is not finite and was taken out of the products
                     for (int i = odd0; i <= odd1; ++i)
                         for (int k = 0; k < (KEYS ? rows : 1); ++k) {
