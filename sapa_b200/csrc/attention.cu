@@ -63,9 +63,10 @@ __device__ __forceinline__ float exponent(const Args &p, float s, float base) {
     const float x = fmaf(s, p.scale_log2, -base);
     return isfinite(x) ? fmaf(s, p.scale_rest, x) : x;
 }
-// lse of a row from the maximum and the sum of its softmax in base 2, and in float32 what its rounding leaves out
+// lse of a row from the maximum and the sum of its softmax in base 2, and in float32 what its rounding leaves out: that of the logarithm too, which would
+// put all weights of the row off by up to 3e-7
 __device__ __forceinline__ void put_lse(const sapa_attention &a, long long row, bool none, bool lost, float m, float sum, bool rest = true) {
-    const double lse = ((double)m + (double)log2f(sum)) * 0.6931471805599453;
+    const double lse = ((double)m + (rest ? log2((double)sum) : (double)log2f(sum))) * 0.6931471805599453;
     const float high = none ? -INFINITY : lost ? __int_as_float(0x7fffffff) : (float)lse;
     a.lse[row] = high;
     if (rest && a.low != nullptr) static_cast<float *>(a.low)[row] = isfinite(high) ? (float)(lse - high) : 0.f;
