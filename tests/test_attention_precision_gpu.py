@@ -4,9 +4,73 @@ import math
 import pytest
 import torch
 
+import attention_oracle as oracle
+import attention_rounding as rounding
+import sapa_b200
 from attention_oracle import offsets_of
 
 pytestmark = pytest.mark.gpu
+HALF = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _made(shape, dtype, seed, scale=1.0, mean=0.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (mean + torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _errors(q, k, v, go, lengths, dtype, rounded_dscores):
+    """Norms of the errors of the three gradients over all sequences, in those to expect."""
+    x = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(sapa_b200.packed_attention(*x, offsets_of(lengths)), x, go)
+    had, model, at = [0.0] * 3, [0.0] * 3, 0
+    for n in lengths:
+        rows = slice(at, at + n)
+        at += n
+        for i, (want, square) in enumerate(rounding.gradients(q[rows], k[rows], v[rows], go[rows], dtype, rounded_dscores)):
+            had[i] += float((got[i][rows].double() - want).square().sum())
+            model[i] += square
+    return [math.sqrt(a / b) for a, b in zip(had, model)]
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens, keys", [(300, 1000), (700, 700), (64, 6000), (2, 9000)])
+def test_outputs_with_what_rounding_left_out(tokens, keys, dim, dtype):
+    """In 16 bits out + low is the output before its rounding, with whole and with split keys.  Values around 1, so that the weights' roundings average out
+    and the outputs' own does not: the error's norm is that of the weights (0.6 of even half steps in a restatement on the CPU); that of the outputs' rounding
+    alone is above 4 times as much."""
+    t = HALF[dtype]
+    q, k, v = _made((tokens, 4, dim), t, 0, 1.5), _made((keys, 2, dim), t, 1), _made((keys, 2, dim), t, 2, 0.1, 1.0)
+    out, _, low, _ = _forward(q, k, v, [tokens], [keys], False)
+    had = square = 0.0
+    for h in range(4):
+        p = torch.softmax(q[:, h].double() @ k[:, h // 2].double().T * dim ** -0.5, 1)
+        vv = v[:, h // 2].double()
+        had += float((out[:, h].double() + low[:, h].double() - p @ vv).square().sum())
+        square += oracle.HALF_STEP[t] ** 2 / 3 * float((p.square() @ vv.square()).sum())
+    assert had <= square
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("dim", [64, 128])
+def test_delta_is_that_of_the_unrounded_outputs(dim, dtype):
+    """Values around 1 make delta large beside dP - delta: from rounded outputs the gradients of queries and keys would be twice as far off as the bound (a
+    restatement on the CPU: 0.3 to 0.5 of it as the kernels do it, 2.0 to 3.1 from rounded outputs)."""
+    t, T = HALF[dtype], 1500
+    q, k, v = _made((T, 2, dim), t, 0, 1.5), _made((T, 1, dim), t, 1), _made((T, 1, dim), t, 2, 0.1, 1.0)
+    assert max(_errors(q, k, v, _made((T, 2, dim), t, 9), [T], t, True)) <= 1
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("dim", [64, 128])
+def test_short_sequences_do_not_pay_for_the_rounding_of_dscores(dim, dtype):
+    """Up to 64 tokens dS goes into its products with what its rounding leaves out.  In a restatement on the CPU the gradients of queries and keys are 0.59 to 0.62 of
+    the expected errors off with that, 0.81 to 0.88 without."""
+    t, lengths = HALF[dtype], [8 + 4 * i for i in range(15)] * 4
+    T = sum(lengths)
+    q, k, v = _made((T, 2, dim), t, 0, 1.5), _made((T, 2, dim), t, 1), _made((T, 2, dim), t, 2)
+    errors = _errors(q, k, v, _made((T, 2, dim), t, 9), lengths, t, False)
+    assert max(errors[:2]) <= 0.71 and errors[2] <= 1
 
 
 def _forward(q, k, v, lengths, key_lengths, causal):
