@@ -772,10 +772,13 @@ __global__ void __launch_bounds__(256) sapa_paged_write_kernel(const __grid_cons
 }
 
 // ---------------------------------------------------------------------------------- host side
+constexpr int MOST_ROWS = 0x7fffff00;
 static int check(const sapa_attention *a, int dtype, const char *fn) {
     SAPA_REQUIRE(a != nullptr, SAPA_ERR_ARGUMENT, "%s: the arguments are NULL", fn);
     SAPA_REQUIRE(dtype == SAPA_F32 || dtype == SAPA_F16 || dtype == SAPA_BF16, SAPA_ERR_DTYPE, "%s: dtype code %d is not supported", fn, dtype);
     SAPA_REQUIRE(a->B >= 0 && a->tokens >= 0 && a->keys >= 0, SAPA_ERR_ARGUMENT, "%s: negative size", fn);
+    // a tile may begin at the last row: its end has to be a number too
+    SAPA_REQUIRE(a->tokens < MOST_ROWS && a->keys < MOST_ROWS, SAPA_ERR_UNSUPPORTED, "%s: more than 2^31 - 256 tokens or keys", fn);
     SAPA_REQUIRE(a->heads > 0 && a->groups > 0 && a->heads % a->groups == 0, SAPA_ERR_ARGUMENT, "%s: %d heads do not share %d key heads evenly", fn, a->heads, a->groups);
     SAPA_REQUIRE(a->heads / a->groups <= 128, SAPA_ERR_UNSUPPORTED, "%s: more than 128 heads share a key head", fn);
     SAPA_REQUIRE(a->dim > 0 && a->dim <= 128 && a->dim % 8 == 0, SAPA_ERR_UNSUPPORTED, "%s: dim %d is not a multiple of 8 up to 128", fn, a->dim);
@@ -784,7 +787,7 @@ static int check(const sapa_attention *a, int dtype, const char *fn) {
     if (a->page_table != nullptr) {
         SAPA_REQUIRE(a->key_lengths != nullptr, SAPA_ERR_ARGUMENT, "%s: key_lengths is NULL", fn);
         SAPA_REQUIRE(a->pages > 0 && a->page > 0 && a->max_pages > 0, SAPA_ERR_ARGUMENT, "%s: pages, page and max_pages must be positive", fn);
-        SAPA_REQUIRE((long long)a->max_pages * a->page < 0x7fffff00ll, SAPA_ERR_UNSUPPORTED, "%s: more than 2^31 positions", fn);
+        SAPA_REQUIRE((long long)a->max_pages * a->page < MOST_ROWS, SAPA_ERR_UNSUPPORTED, "%s: more than 2^31 positions", fn);
     } else {
         SAPA_REQUIRE(a->key_offsets != nullptr, SAPA_ERR_ARGUMENT, "%s: key_offsets is NULL", fn);
     }

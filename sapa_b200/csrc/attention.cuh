@@ -150,7 +150,7 @@ struct KeyBlocks {
         const int n = tiles_of(s.nk, tile), last = s.nq - (w - 1) * tok - 1;          // the last token that a block may begin with
         if (w == 0) return n;
         if (last < 0) return 0;
-        const int key = last + s.nk - s.nq;                                           // the last key that it sees
+        const int key = last - s.nq + s.nk;                                           // the last key that it sees
         return !causal ? n : key < 0 ? 0 : min(n, (int)((unsigned)key / (unsigned)tile) + 1);
     }
 };
