@@ -132,16 +132,14 @@ __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-// Replaces what is not finite in 128 bytes of a row of a landed tile with 0; whether there was any.  All are read before they are looked at.  Two row tiles clean the
-// same values, and the one that finds zeros must find the note of them too: `note` comes in front of the stores.
-template <typename T, typename Note> __device__ __forceinline__ bool clean_line(unsigned line, int row, Note note) {
+// Replaces what is not finite in 128 bytes of a row of a landed tile with 0; whether there was any.  All are read before they are looked at.
+template <typename T> __device__ __forceinline__ bool clean_line(unsigned line, int row) {
     unsigned v[32];
 #pragma unroll
     for (int c = 0; c < 8; ++c)                                       // in another order in every row: no two on the same banks
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[4 * c]), "=r"(v[4 * c + 1]), "=r"(v[4 * c + 2]), "=r"(v[4 * c + 3])
                      : "r"(line + ((c ^ (row & 7)) << 4)) : "memory");
     if (finite::all_finite<T, 32>(v)) return false;
-    note();
 #pragma unroll
     for (int c = 0; c < 8; ++c)
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(line + ((c ^ (row & 7)) << 4)), "r"(finite::or_zero<T>(v[4 * c])),
@@ -149,9 +147,11 @@ template <typename T, typename Note> __device__ __forceinline__ bool clean_line(
     return true;
 }
 // The same for a row of a tile of 128 rows
-template <typename T, int D, typename Note> __device__ __forceinline__ void clean_row(unsigned tile, int row, Note note) {
+template <typename T, int D> __device__ __forceinline__ bool clean_row(unsigned tile, int row) {
+    bool any = false;
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) (void)clean_line<T>(tile + b * BLOCK_BYTES + row * 128, row, note);
+    for (int b = 0; b < D / 64; ++b) any = clean_line<T>(tile + b * BLOCK_BYTES + row * 128, row) || any;
+    return any;
 }
 // 32 channels of a row each of a warp's lanes, from float32, those below `left`; `mine`: whether the lane has one.  A row in every lane is a line in every
 // lane, and a store takes a cycle for each: so two lanes write halves of one row and then of the other, 32 bytes each (`whole`: rows begin on 32
@@ -481,14 +481,12 @@ __global__ void __launch_bounds__(um::NT, 1) sapa_attention_umma_kernel(const __
                 if (!mbar_wait_warp(sfull + 8 * t, sph)) { ok = false; break; }
                 sph ^= 1;
                 tc_fence_after();
-                // the values of a tile that not every row sees; behind the scores, which came behind the last use of the stage before this one
-                if (part) {
+                // the values of a tile that not every row sees; behind the scores, which came behind the last use of the stage before this one.  One row tile
+                // cleans a tile of keys: the products of the second come behind those of the first, which sees fewer keys and so has cleaned all that it takes.
+                if (part && (!WIDE || t == 0 || i >= *const_cast<volatile int *>(&w->n0))) {      // read here: no register for it
                     const unsigned load = loads + L::stage_of(j - j0, all, false), stage = load % NST;
                     if (!mbar_wait_warp(full + 8 * stage, (load / NST) & 1)) { ok = false; break; }
-                    clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r, [&]() {
-                        if (k0 + r < seen) { atomicMin(&w->odd_first, k0 + r); atomicMax(&w->odd_last, k0 + r); }
-                        __threadfence_block();
-                    });
+                    if (clean_row<T, D>(base + L::KV0 + stage * L::STAGE, r) && k0 + r < seen) { atomicMin(&w->odd_first, k0 + r); atomicMax(&w->odd_last, k0 + r); }
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     __syncwarp();                                     // lanes that found something went another way: tensor memory is read by whole warps
                 }

@@ -80,7 +80,7 @@ template <typename T> __device__ __forceinline__ void store_packed(unsigned tadd
 template <typename T, int D, int TN> __device__ __forceinline__ bool clean_box(unsigned tile, int row) {
     bool any = false;
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) any = clean_line<T>(tile + b * TN * 128 + row * 128, row, [] {}) || any;
+    for (int b = 0; b < D / 64; ++b) any = clean_line<T>(tile + b * TN * 128 + row * 128, row) || any;
     return any;
 }
 
