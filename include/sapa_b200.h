@@ -403,12 +403,14 @@ int sapa_deform_fused_backward(const void *grad_out, const void *query, const vo
  * `heads` query heads share `groups` key / value heads: query head h reads head h / (heads / groups).
  *   out[t, h, :] = sum_j softmax_j(scale * <query[t, h], key[j]>) value[j]          (0 where a token sees no key)
  * What a token does not see has no part in its output, whatever it holds.  The lengths are read on the device and taken within bounds: an
- * offset outside the tensor counts as the nearest one inside, a sequence whose end lies before its begin as empty.  A page number outside
+ * offset outside the tensor counts as the nearest one inside, a sequence whose end lies before its begin as empty.  Offsets that decrease are
+ * no more than safe: rows of sequences that overlap, or that the last offset leaves out, hold any numbers.  A page number outside
  * [0, pages), or a position that the table has no page for, is never read: tokens that see it get NaN.
  *
  * Rows (dim channels) are dense; all other strides are free, in elements, and multiples of 16 bytes, as the addresses are.  `out` and the
  * gradients are dense [tokens, heads, dim] and overwritten, `lse` is [tokens, heads] float32; in rows of no sequence all of them are 0.
- * dtype: SAPA_F32, SAPA_F16, SAPA_BF16; dim: a multiple of 8 up to 128; heads / groups up to 128. */
+ * dtype: SAPA_F32, SAPA_F16, SAPA_BF16; dim: a multiple of 8 up to 128; heads / groups up to 128; tokens, keys and max_pages * page below
+ * 2^31 - 256.  16-bit pages whose size is not a power of two from 8 up are served by the kernel of float32, many times slower. */
 typedef struct sapa_attention {
     const void *query, *key, *value;
     void *out;

@@ -23,7 +23,13 @@ def packed_attention(query, key, value, offsets, key_offsets=None, causal=True, 
 
     A token that sees no key gets 0, and so do rows of no sequence.  What a token does not see has no part in its output or in any
     gradient, not even if it is infinite or NaN.  The lengths stay on the device: the call can be captured into a graph and replayed with
-    others.  Deterministic."""
+    others.  Deterministic.
+
+    ``offsets`` do not decrease.  Where they do, nothing outside the tensors is read or written, but rows of sequences that overlap, or that the last offset
+    leaves out, hold any numbers.  In 16 bits the softmax's weights, and dS in the gradients, are rounded to the type for the products that take them (up
+    to 64 tokens dS keeps what that leaves out; in float16 it is held by a power of two, so that gradients of any size neither vanish nor overflow on the
+    way), and a quarter of the forward's exponentials are off by up to 1.0e-4 (bfloat16) or 2.8e-6 (float16) of themselves; sums, statistics and delta are
+    float32."""
     if _lib.transformed():
         return PackedAttentionFunction.apply(query, key, value, offsets, key_offsets, causal, scale)
     return (_lib.host or _lib.load_host()).packed_attention(query, key, value, offsets, key_offsets, causal, scale)
@@ -51,6 +57,9 @@ def paged_attention(query, key_pages, value_pages, page_table, key_lengths, offs
     multiples of 16 bytes; ``page_table`` [B, most pages] and ``key_lengths`` [B], int32 on the device.  Position p of sequence b lies in slot
     ``p % page`` of page ``page_table[b, p // page]``; its keys are the positions below ``key_lengths[b]``, which counts the new tokens: with ``causal``
     token i of Lq sees the positions up to ``key_lengths[b] - Lq + i``.
+
+    In 16 bits pages of 8, 16, 32, ... slots (powers of two) go through the tensor cores.  Pages of other sizes are served by the kernel of float32, which takes
+    15 times as long for single tokens and 40 times for chunks (48 sequences of up to 8190 keys: 150 and 2200 us; six chunks of 512 tokens: 165 and 6500).
 
     Entries of the table behind a sequence's last page are not read.  A token that sees a position whose page number lies outside the
     cache, or that the table has no entry for, gets NaN; the page is not read."""

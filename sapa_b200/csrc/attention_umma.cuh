@@ -11,8 +11,8 @@
 // O is scaled again only when a row's maximum has grown by more than 2^8 since it last was: weights stay below 2^8 and the sums exact enough, and
 // the warpgroup that owns S owns O too at that time, for S was computed behind the product that last added to O.
 // What bounds it: of long prompts the tensor pipe between the two softmaxes, the exponentials (a quarter of them by FMA units) and
-// the power limit (8192 tokens, 32 heads of 128 channels, causal, bfloat16: 410 us, 1.34 PFLOP/s); of short ones the tiles on the diagonal and an item's start
-// and end; of single tokens reading the cache (209 thousand keys, 8 key heads of 128 channels: 131 us at the copy rate, 150 warm).
+// the power limit (8192 tokens, 32 heads of 128 channels, causal, bfloat16: 412 us, 1.33 PFLOP/s); of short ones an item's start and end and how
+// evenly the items share the SMs; of single tokens reading the cache (209 thousand keys, 8 key heads of 128 channels: 131 us at the copy rate, 150 warm).
 // What a row does not see: its scores are set to -infinity; a value that is not finite would still reach its output as 0 * infinity.  So in tiles that not
 // every row sees whole, what is not finite among the values is replaced with 0 in front of the product, and added to the outputs of the rows that see it.
 #pragma once
@@ -45,7 +45,7 @@ template <int D, bool WIDE> struct Lay {
     static constexpr int SOFTMAX_REGS = WIDE ? 208 : 224, OTHER_REGS = WIDE ? 88 : 56;
     static_assert(8 * 32 * SOFTMAX_REGS + 4 * 32 * OTHER_REGS <= NT * REGS, "a block draws on what it was launched with");
     // whether the second product begins with half of a tile's weights.  In 64 channels it is short, and waiting for the stores twice costs more than that
-    // gains: one prompt of 8192 tokens, 32 heads, bfloat16: 64 channels 358 us with halves, 330 without; 128 channels 410 and 428.
+    // gains: one prompt of 8192 tokens, 32 heads, bfloat16: 64 channels 374 us with halves, 358 without; 128 channels 414 and 436.
     static constexpr bool HALVES = D == 128;
     // place in the order of loads of an item's tile, of `all`
     static __device__ __forceinline__ unsigned stage_of(int tile, int all, bool keys) {

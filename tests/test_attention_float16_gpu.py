@@ -64,3 +64,27 @@ def test_sequences_do_not_see_each_others_sizes(dim):
         heads = a.shape[1] // 2
         assert torch.equal(a[:300, :heads], b[:300, :heads]) and torch.equal(a[370:], b[370:])
         assert bool((a[870:] == 0).all())
+
+
+def test_captured_and_replayed_with_other_sizes():
+    """The factor of dS is found anew in every replay: other lengths, gradients and values a thousand times as large and as small."""
+    T = 400
+    q, k, v = (x.requires_grad_() for x in (_made((T, 4, 64), 0), _made((T, 2, 64), 1), _made((T, 2, 64), 2)))
+    go, off = _made((T, 4, 64), 9), offsets_of([250, 100, 50])
+
+    def step():
+        return torch.autograd.grad(sapa_b200.packed_attention(q, k, v, off), (q, k, v), go)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i, (size, lengths) in enumerate(((1e-3, [30, 300, 70]), (1e3, [1, 2, 397]), (1.0, [0, 0, 17]))):
+        go.copy_(_made((T, 4, 64), 10 + i, size))
+        off.copy_(offsets_of(lengths))
+        graph.replay()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
