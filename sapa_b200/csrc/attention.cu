@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(256, 8) sapa_attention_delta_kernel(const __gr
 // float16.  The power of two that dS of a sequence and key head is multiplied with to be held in 16 bits: |dS| = |P_j sum_k P_k (dP_j - dP_k)| is at most a quarter
 // of the range of dP, that is half the product of the longest rows of grad_out and of value, and comes to 2^14 at most.  The scores' weights, around
 // 1 / keys, leave it among the normal numbers then, whatever size the gradients have.  Rows that are not finite do not count.  A block of 1024 threads to each,
-// or of short sequences a warp (2000 sequences of up to 20 tokens, 12 heads: forward and gradients 1874 us with blocks, 1727 with warps).
+// or a warp where there are more than two rounds of blocks (2000 sequences of up to 20 tokens, 12 heads: forward and gradients 1874 us with blocks, 1727 with warps;
+// 8 sequences of up to 1024 tokens: 172 and 175).
 template <bool WARPS>
 __global__ void __launch_bounds__(WARPS ? 256 : 1024) sapa_attention_factor_kernel(const __grid_constant__ Args p, const __grid_constant__ Grads g) {
     const sapa_attention &a = p.a;
@@ -1008,7 +1009,7 @@ extern "C" int sapa_attention_backward(const sapa_attention *a, const void *grad
         if (int e = check_launch("sapa_attention_delta_kernel")) return e;
         if (dtype == SAPA_F16 && a->B > 0) {
             const unsigned factors = (unsigned)(a->B * a->groups);
-            if ((long long)a->tokens * p.share <= 1024ll * a->B) launch_next(sapa_attention_factor_kernel<true>, dim3((factors + 7) / 8), dim3(256), 0, st, p, g);
+            if (factors > 4u * (unsigned)sms) launch_next(sapa_attention_factor_kernel<true>, dim3((factors + 7) / 8), dim3(256), 0, st, p, g);
             else launch_next(sapa_attention_factor_kernel<false>, dim3(factors), dim3(1024), 0, st, p, g);
             if (int e = check_launch("sapa_attention_factor_kernel")) return e;
         }

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(umg::THREADS, 1) sapa_attention_umma_grad_kern
                         w.s = sequence_at(a, it.b);
                         w.fine = max(w.s.nq, w.s.nk) <= FINE;
                         w.factor = SCALED ? g.factor[(long long)w.b * a.groups + w.group] : 1.f;
-                        w.rescale = a.scale / w.factor;               // a power of two
+                        w.rescale = a.scale / w.factor;               // exact: by a power of two
                         if (KEYS) {
                             w.first = it.block * KT;
                             w.from = a.causal ? (int)max(0ll, (long long)w.first - w.s.nk + w.s.nq) : 0;

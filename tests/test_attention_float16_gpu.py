@@ -88,3 +88,23 @@ def test_captured_and_replayed_with_other_sizes():
         graph.replay()
         for a, b in zip(held, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("size", [1e-4, 3000.0])
+def test_many_sequences(size):
+    """Hundreds of sequences, some empty, whose factors are found by warps: the bits of calls on few of them, whose factors are found by blocks."""
+    lengths = [(7 * i) % 23 for i in range(900)]
+    T = sum(lengths)
+    q, k, v, go = _made((T, 2, 64), 0), _made((T, 1, 64), 1), _made((T, 1, 64), 2), _made((T, 2, 64), 9, size)
+    off = offsets_of(lengths)
+    together = _grads(q, k, v, go, off)
+    for first in (0, 300, 820):
+        some = off[first:first + 81].contiguous()
+        rows = slice(int(some[0]), int(some[-1]))
+        for a, b in zip(_grads(q, k, v, go, some), together):
+            assert bool(b[rows].isfinite().all()) and torch.equal(a[rows], b[rows])
+
+
+def test_no_wait_gave_up():
+    from sapa_b200 import _lib
+    assert _lib.wait_timeout_flags("cuda") == 0

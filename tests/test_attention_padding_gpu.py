@@ -119,3 +119,8 @@ def test_infinite_values_at_the_diagonal_of_two_row_tiles(dim, dtype):
             assert torch.equal(out[:, :2], clean[:, :2]) and torch.equal(out[:, 2:, len(at):], clean[:, 2:, len(at):])
             for i, j in enumerate(at):
                 assert torch.equal(out[:j, 2:, i], clean[:j, 2:, i]) and bool((out[j:, 2:, i] == v[j, 1, i]).all())
+
+
+def test_no_wait_gave_up():
+    from sapa_b200 import _lib
+    assert _lib.wait_timeout_flags("cuda") == 0

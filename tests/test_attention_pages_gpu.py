@@ -29,3 +29,8 @@ def test_a_bad_page_and_a_table_that_ends_early(new, page, dtype):
             rows = slice(b * new, (b + 1) * new)
             check(out[rows], want["out"][rows], want["out_tol"][rows])
         assert bool(out[new:2 * new].isnan().all())      # each sees position `page` at least
+
+
+def test_no_wait_gave_up():
+    from sapa_b200 import _lib
+    assert _lib.wait_timeout_flags("cuda") == 0

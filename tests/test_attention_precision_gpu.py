@@ -87,3 +87,8 @@ def test_logarithms_of_sums(tokens, keys, causal):
     out, lse, low, _ = _forward(q, k, v, [tokens], [keys], causal)
     count = (torch.arange(tokens, device="cuda", dtype=torch.float64) + 1 if causal else torch.full((tokens,), float(keys), device="cuda", dtype=torch.float64))[:, None]
     assert float((lse.double() + low.double() - count.log()).abs().max()) <= 2.0 ** -44
+
+
+def test_no_wait_gave_up():
+    from sapa_b200 import _lib
+    assert _lib.wait_timeout_flags("cuda") == 0

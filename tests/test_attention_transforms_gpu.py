@@ -89,3 +89,8 @@ def test_paged_refusals():
         torch.jit.trace(_step, (q.requires_grad_(), k, v, c.key, c.value, *rest), check_trace=False)
     with pytest.raises(NotImplementedError):
         torch.jit.trace(lambda k, v: sapa_b200.paged_write(k, v, c.key, c.value, *rest), (k.requires_grad_(), v), check_trace=False)
+
+
+def test_no_wait_gave_up():
+    from sapa_b200 import _lib
+    assert _lib.wait_timeout_flags("cuda") == 0
